@@ -260,6 +260,63 @@ int sa3_attention(const void* q, const void* k, const void* v, const void* q2, c
                   long long ldo, int window_left, int window_right, float softmax_scale, int dtype,
                   float* amax_out, void* stream);
 
+/* ---------------------------------------------- rotary positions, general form
+ *
+ * The rotation of Attention.apply_rotary_pos_emb (transformer.py:302-322) for any even part of a head, both pair
+ * layouts, any frequencies and any row, without the qk-norm of sa3_qk_norm_rope; and its gradient.
+ * For every row r, head h and pair i < rot_dim / 2 with theta = pos(r) * inv_freq[i]:
+ *   (a, b) -> scale * (a cos theta - b sin theta, b cos theta + a sin theta)
+ * where the pair is columns (i, i + rot_dim/2) of the head, or (2i, 2i+1) when `interleaved`; columns rot_dim.. pass
+ * through. `inverse` rotates by -theta: with the same scale that is the transpose, i.e. the backward pass.
+ * pos(r) = row_pos[r] (int32, any value) if row_pos, else offset + r % rows_per_batch (rows_per_batch 0: offset + r).
+ * theta is formed and reduced in fp64, so far positions lose nothing; data is computed in fp32 and rounded once.
+ * q [rows, heads * head_dim] -> q_out and, unless k is NULL, k [rows, kv_heads * head_dim] -> k_out (kv_heads 0 and
+ * k_out NULL otherwise). dtype SA3_DT_BF16, SA3_DT_F16 or SA3_DT_F32. An output may be its input (same pointer and
+ * row stride); no other overlap. head_dim <= 512. inv_freq: fp64 [rot_dim / 2], 8-byte aligned. Buffers need only
+ * their element's alignment; wider common alignment of pointers, strides and head parts is used where it is there.
+ */
+int sa3_rotary(const void* q, void* q_out, const void* k, void* k_out, int dtype, long long rows, int heads,
+               int kv_heads, int head_dim, int rot_dim, long long ldq, long long ldqo, long long ldk, long long ldko,
+               const double* inv_freq, const int* row_pos, long long rows_per_batch, long long offset, int interleaved,
+               int inverse, float scale, void* stream);
+
+/* ---------------------------------------------- attention to an encoder's states, forward and backward
+ *
+ * out = softmax(softmax_scale * q k^T) v over the visible keys, without a window: the cross-attention call of
+ * TransformerBlock.forward (transformer.py:1031-1035) with grouped heads, wider heads, key lengths and key masks,
+ * and with what a backward pass needs.
+ * Token rows as in sa3_attention; query head h sits at columns h * head_dim of q and reads key head
+ * h / (heads / kv_heads) of k and v. head_dim 64 or 128; SA3_DT_BF16 or SA3_DT_F16; rows 16-byte aligned.
+ * Sequences: rows [b*max_seqlen, (b+1)*max_seqlen) where cu_seqlens_q / cu_seqlens_k (each on its own) is NULL (then
+ * total = batch * max_seqlen), else rows [cu[b], cu[b+1]), of which at most max_seqlen are taken.
+ * A key is visible if it is one of the first k_lens[b] of its sequence (k_lens: int32 [batch] or NULL) and its byte
+ * of key_mask (uint8 [total_k] or NULL) is nonzero. Hidden keys may hold anything. A row without visible keys gives
+ * out = 0, lse = -inf and zero gradients. Rows outside all sequences are left as they are.
+ * lse (fp32 [heads, total_q], or NULL): natural log of the sum of the exponentials.
+ * softmax_scale > 0. Zero lengths and batches are valid.
+ * At most 16 query rows a key head (max_seqlen_q * heads / kv_heads, e.g. one decoded token) take a kernel that
+ * splits the keys over a cluster; the rest take a tcgen05 kernel.
+ *
+ * sa3_cross_attention_bwd: dq, dk, dv of the sum of out * dout, from the forward's out and lse. dk and dv are summed
+ * over the query heads of a group, in a fixed order (the same bits in every run). workspace: 16-byte aligned device
+ * memory of at least the bytes that sa3_cross_attention_bwd_workspace reports for the current device, used by this
+ * call alone until it has run.
+ */
+int sa3_cross_attention(const void* q, const void* k, const void* v, void* out, float* lse, const int* cu_seqlens_q,
+                        const int* cu_seqlens_k, const int* k_lens, const unsigned char* key_mask, int batch,
+                        int max_seqlen_q, int max_seqlen_k, int total_q, int total_k, int heads, int kv_heads,
+                        int head_dim, long long ldq, long long ldk, long long ldv, long long ldo, float softmax_scale,
+                        int dtype, void* stream);
+int sa3_cross_attention_bwd_workspace(int batch, int max_seqlen_q, int max_seqlen_k, int total_q, int total_k,
+                                      int heads, int kv_heads, int head_dim, long long* bytes);
+int sa3_cross_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                            const float* lse, void* dq, void* dk, void* dv, const int* cu_seqlens_q,
+                            const int* cu_seqlens_k, const int* k_lens, const unsigned char* key_mask, int batch,
+                            int max_seqlen_q, int max_seqlen_k, int total_q, int total_k, int heads, int kv_heads,
+                            int head_dim, long long lddo, long long ldq, long long ldk, long long ldv, long long ldo,
+                            long long lddq, long long lddk, long long lddv, float softmax_scale, int dtype,
+                            void* workspace, long long workspace_bytes, void* stream);
+
 /* ---------------------------------------------- allocation-free FP8 linear
  *
  * No counterpart in the reference: an addition for callers that cannot

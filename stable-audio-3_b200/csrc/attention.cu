@@ -36,6 +36,7 @@
 // masked key tiles are never loaded or multiplied; tiles that lie entirely
 // inside every row's band skip masking, edge tiles mask with a bit mask.
 // Shared memory: per unit Q 2x16 KB + K 3x16 KB + V 2x16 KB = 112 KB.
+#include "attn_tile.cuh"
 #include "common.cuh"
 #include "host_util.h"
 
@@ -94,108 +95,6 @@ __device__ __forceinline__ Unit make_unit(const AttnParams& p, int b, int tile) 
     u.ntiles = j_hi > u.j_lo ? (j_hi - u.j_lo + ATT_BN - 1) / ATT_BN : 0;
   }
   return u;
-}
-
-__device__ __forceinline__ uint32_t pack_2(float lo, float hi, bool f16) {
-  if (f16) {
-    __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&h);
-  }
-  return pack_bf16x2(lo, hi);
-}
-
-// Packed pairs of fp32 (sm_100 f32x2 arithmetic: one instruction per two lanes of data).
-__device__ __forceinline__ uint64_t f2(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 f2_split(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
-constexpr uint32_t NEG_INF_BITS = 0xff800000u;
-
-// Edge tile: scores of columns outside [lo, hi) (chunk-relative) become -inf.
-__device__ __forceinline__ void mask_chunk(uint32_t (&s)[32], int lo, int hi) {
-  const int a = min(max(lo, 0), 32), b = min(max(hi, 0), 32);
-  const uint32_t below_b = b >= 32 ? 0xffffffffu : ((1u << b) - 1u);
-  const uint32_t below_a = a >= 32 ? 0xffffffffu : ((1u << a) - 1u);
-  const uint32_t m = below_b & ~below_a;
-#pragma unroll
-  for (int e = 0; e < 32; ++e) s[e] = (m >> e) & 1u ? s[e] : NEG_INF_BITS;
-}
-
-// Running maxima over one chunk, eight independent chains.
-__device__ __forceinline__ void max_chunk(const uint32_t (&s)[32], float (&m)[8]) {
-#pragma unroll
-  for (int t = 0; t < 8; ++t)
-    m[t] = fmax3(fmax3(m[t], __uint_as_float(s[4 * t]), __uint_as_float(s[4 * t + 1])),
-                 __uint_as_float(s[4 * t + 2]), __uint_as_float(s[4 * t + 3]));
-}
-
-// P = exp2(s * scale - m) for one chunk as packed 16-bit pairs, row sums into four f32x2 chains.
-__device__ __forceinline__ void exp_chunk(const uint32_t (&s)[32], uint64_t scale2, uint64_t negm2,
-                                          uint64_t (&acc)[4], uint32_t (&w)[16], bool f16) {
-#pragma unroll
-  for (int e = 0; e < 32; e += 2) {
-    const float2 x = f2_split(ffma2(f2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, negm2));
-    const float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
-    acc[(e >> 1) & 3] = fadd2(acc[(e >> 1) & 3], f2(p0, p1));
-    w[e >> 1] = pack_2(p0, p1, f16);
-  }
-}
-
-// tcgen05.mma / commit issued by one elected lane of a converged warp, descriptors given as (low
-// word, shared high word): the issue loop only adds constants to the low word (the start-address
-// field). Running the issue loop on the whole warp keeps its operands warp-uniform, which lets the
-// MMAs go out back to back (from a single lane in a divergent branch the 64-wide P V steps issue at
-// about 60% of the tensor rate).
-__device__ __forceinline__ void mma_ss_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
-                                          uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t.reg .b64 da, db;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "mov.b64 da, {%1, %3};\n\t"
-      "mov.b64 db, {%2, %3};\n\t"
-      "elect.sync r|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts_lo(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi,
-                                          uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t.reg .b64 db;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "mov.b64 db, {%2, %3};\n\t"
-      "elect.sync r|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void commit_elect(uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t"
-      "elect.sync r|e, 0xffffffff;\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
-      : "memory");
-}
-// mbar_wait on every lane of a converged warp; the warp agrees on the outcome.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int site) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, site));
 }
 
 // Work item = (pair of consecutive query tiles, head, sequence), query tile fastest. Unit u of the

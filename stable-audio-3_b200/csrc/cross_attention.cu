@@ -1,0 +1,1185 @@
+// Attention of queries to an encoder's states of another length, forward and backward, on tcgen05 for sm_100a:
+// key heads shared by groups of query heads, heads of 64 or 128 columns, packed or uniform batches, per-sequence
+// key lengths and a key mask.
+//
+//   S = scale * Q K^T, hidden keys -inf;  P = softmax(S);  O = P V;  lse = log sum exp S
+//   delta = rowsum(dO * O);  dP = dO V^T;  dS = P * (dP - delta)
+//   dQ = scale * dS K;  dK = scale * dS^T Q;  dV = P^T dO      (dK, dV summed over the query heads of the group)
+//
+// A row without visible keys gives O = 0, lse = -inf and no gradient. What stands in hidden keys and behind the
+// ends of sequences may be anything, NaN included: scores of hidden keys are replaced, never scaled, and rows that
+// a contraction would multiply by a zero probability (V and K of hidden keys, Q and dO behind a sequence's end)
+// are zeroed in shared memory before the tensor core reads them.
+//
+// Sums, softmax statistics and accumulators are fp32; P and dS are rounded once to the operands' 16-bit type, the
+// type of the matrix instructions.
+#include "attn_tile.cuh"
+#include "common.cuh"
+#include "cross_attention.h"
+#include "host_util.h"
+
+namespace sa3 {
+SA3_DEFINE_ERROR_READER(read_error_cross)
+
+constexpr int XA_BM = 128;  // rows of the wide side of a tile: queries (forward, dQ) or keys (dK / dV)
+constexpr int XA_BN = 64;   // rows of the walked side: keys (forward, dQ) or queries (dK / dV)
+constexpr float XA_LOG2E = 1.4426950408889634f;
+constexpr float XA_RESCALE_LOG2 = 8.f;  // move the reference maximum only when it grows by more than this
+constexpr int XA_SUB_M = XA_BM * 128;   // bytes of a 64-column sub-tile of the wide side
+constexpr int XA_SUB_N = XA_BN * 128;   // ... of the walked side
+
+// One sequence: row offsets and lengths, clamped to the buffers so that no offset reaches outside them.
+struct XSeq {
+  int qs, lq, ks, lk, seen;  // seen: keys before the sequence's key length (a key mask may hide more)
+};
+
+__device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
+
+__device__ __forceinline__ XSeq make_seq(const XParams& p, int b) {
+  XSeq s;
+  if (p.cu_q) {
+    s.qs = clampi(__ldg(p.cu_q + b), 0, p.total_q);
+    s.lq = clampi(__ldg(p.cu_q + b + 1) - s.qs, 0, min(p.total_q - s.qs, p.Lq));
+  } else {
+    s.qs = b * p.Lq;
+    s.lq = p.Lq;
+  }
+  if (p.cu_k) {
+    s.ks = clampi(__ldg(p.cu_k + b), 0, p.total_k);
+    s.lk = clampi(__ldg(p.cu_k + b + 1) - s.ks, 0, min(p.total_k - s.ks, p.Lk));
+  } else {
+    s.ks = b * p.Lk;
+    s.lk = p.Lk;
+  }
+  s.seen = p.k_lens ? clampi(__ldg(p.k_lens + b), 0, s.lk) : s.lk;
+  return s;
+}
+
+// Bit i: key j0 + i of the sequence is visible (i < 64). All lanes of a warp call it and get the same word.
+__device__ __forceinline__ uint64_t visible64(const XParams& p, const XSeq& s, int j0, int lane) {
+  const int n = s.seen - j0;
+  bool a = lane < n, b = lane + 32 < n;
+  if (p.key_mask) {
+    const uint8_t* m = p.key_mask + s.ks + j0;
+    a = a && __ldg(m + lane) != 0;
+    b = b && __ldg(m + lane + 32) != 0;
+  }
+  const uint32_t lo = __ballot_sync(0xffffffffu, a), hi = __ballot_sync(0xffffffffu, b);
+  return ((uint64_t)hi << 32) | lo;
+}
+
+// A whole warp zeroes the rows of an XA_BN-row tile (subs sub-tiles of 64 columns) whose bit in `keep` is clear. A row is
+// 128 contiguous bytes of a sub-tile: the 128-byte swizzle only permutes its 16-byte chunks.
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int subs, int rows, uint64_t keep, int lane) {
+  const int chunk = lane & 7;
+  for (int r = lane >> 3; r < rows; r += 4)
+    if (!((keep >> r) & 1))
+      for (int c = 0; c < subs; ++c)
+        *reinterpret_cast<uint4*>(tile + c * XA_SUB_N + r * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+__device__ __forceinline__ float unpack_lo(uint32_t w, bool f16) {
+  return f16 ? __half2float(__ushort_as_half((unsigned short)(w & 0xffffu))) : __uint_as_float(w << 16);
+}
+__device__ __forceinline__ float unpack_hi(uint32_t w, bool f16) {
+  return f16 ? __half2float(__ushort_as_half((unsigned short)(w >> 16))) : __uint_as_float(w & 0xffff0000u);
+}
+
+// scores of hidden columns become -inf
+__device__ __forceinline__ void hide32(uint32_t (&s)[32], uint32_t vis) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e) s[e] = (vis >> e) & 1u ? s[e] : NEG_INF_BITS;
+}
+
+// D columns of one TMEM lane times f, rounded to 16 bits, to a row in memory
+template <int D>
+__device__ __forceinline__ void store_row16(uint32_t t_o, float f, bool f16, bool store, void* dst) {
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld32_async(t_o + 32 * c, o);
+    tmem_wait_ld();
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      w[e] = pack_2(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f, f16);
+    if (store) {
+      uint4* d = reinterpret_cast<uint4*>(dst) + 4 * c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+    }
+  }
+}
+template <int D>
+__device__ __forceinline__ void zero_row16(void* dst) {
+#pragma unroll
+  for (int e = 0; e < D / 8; ++e) reinterpret_cast<uint4*>(dst)[e] = make_uint4(0, 0, 0, 0);
+}
+
+constexpr int XA_THREADS = 192;  // warps 0..3 softmax (TMEM lane quarters), 4 TMA, 5 MMA
+
+// ------------------------------------------------------------------------------------------------ forward
+// Persistent, two CTAs an SM: while one CTA's softmax warps exponentiate, the other's tensor core and loads run.
+// Work item = (query tile of 128 rows, head, sequence), query tile fastest, so CTAs that run together share K/V in
+// L2. TMEM (256 columns): two score buffers of 64 columns, P (packed pairs) over the buffer of its scores, O behind.
+// S of key tile t + 1 is multiplied while the softmax works on tile t. Bound by the exponentials at D = 64 (64 * 128
+// of them take 512 cycles of the SM's 16 a cycle, the two products 320), by the shared-memory reads of the products
+// at D = 128.
+template <int D>
+struct XFwd {
+  static constexpr int SUBS = D / 64;
+  static constexpr int QS = D == 64 ? 2 : 1, KS = D == 64 ? 4 : 2, VS = KS;
+  static constexpr int Q_BYTES = SUBS * XA_SUB_M, T_BYTES = SUBS * XA_SUB_N;
+  static constexpr int TILES = QS * Q_BYTES + (KS + VS) * T_BYTES;
+  static constexpr int SMEM = TILES + 1024 + 512;
+};
+
+template <int D>
+__global__ void __launch_bounds__(XA_THREADS, 2)
+    cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const XParams p, int num_items, int qtiles) {
+  using C = XFwd<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  auto sQ = [&](int s) { return smem + s * C::Q_BYTES; };
+  auto sK = [&](int s) { return smem + C::QS * C::Q_BYTES + s * C::T_BYTES; };
+  auto sV = [&](int s) { return smem + C::QS * C::Q_BYTES + (C::KS + s) * C::T_BYTES; };
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::TILES);
+  uint64_t* q_full = bars;        // [QS]
+  uint64_t* q_empty = bars + 2;   // [QS]
+  uint64_t* k_full = bars + 4;    // [KS]
+  uint64_t* k_empty = bars + 8;   // [KS]
+  uint64_t* v_full = bars + 12;   // [VS]
+  uint64_t* v_empty = bars + 16;  // [VS]
+  uint64_t* s_full = bars + 20;   // [2] scores of a tile are in TMEM
+  uint64_t* p_full = bars + 22;   // [2] its probabilities are (4 arrivals)
+  // [2] P V of a tile is done. Two, since the softmax skips most of these phases: when it waits for tile g's it
+  // knows that tile g - 2's is over, so the parity on the tile's own barrier cannot be that of an older phase.
+  uint64_t* o_full = bars + 24;
+  uint64_t* o_empty = bars + 26;  // the softmax has read an item's O (4 arrivals)
+  uint64_t* done = bars + 27;
+  constexpr int NBARS = 28;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < NBARS; ++i) mbar_init(&bars[i], (i == 22 || i == 23 || i == 26) ? 4 : 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dep_wait();
+
+  if (warp == 4) {
+    if (lane == 0) {
+      int g = 0, qc = 0;
+      bool ok = true, v_out = true;  // v_out: V of the last counted tile was issued
+      for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
+        const int tile = item % qtiles, rest = item / qtiles;
+        const int h = rest % p.heads, b = rest / p.heads;
+        const XSeq s = make_seq(p, b);
+        const int T = tile * XA_BM < s.lq ? (s.seen + XA_BN - 1) / XA_BN : 0;
+        if (T == 0) continue;
+        const int cq = h * D, ck = (h / p.group) * D;
+        const int qs = qc % C::QS;
+        if (qc >= C::QS && !mbar_wait(&q_empty[qs], ((qc / C::QS) - 1) & 1, abort_flag, 100)) break;
+        mbar_arrive_expect_tx(&q_full[qs], C::Q_BYTES);
+        for (int c = 0; c < C::SUBS; ++c)
+          tma_load_2d(sQ(qs) + c * XA_SUB_M, &tmQ, &q_full[qs], cq + 64 * c, s.qs + tile * XA_BM);
+        qc++;
+        for (int t = 0; t < T; ++t, ++g) {
+          const int ks = g % C::KS;
+          if (g >= C::KS && !mbar_wait(&k_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 101)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&k_full[ks], C::T_BYTES);
+          for (int c = 0; c < C::SUBS; ++c)
+            tma_load_2d(sK(ks) + c * XA_SUB_N, &tmK, &k_full[ks], ck + 64 * c, s.ks + t * XA_BN);
+          if (g >= C::VS && !mbar_wait(&v_empty[ks], ((g / C::VS) - 1) & 1, abort_flag, 102)) {
+            g++;
+            ok = v_out = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&v_full[ks], C::T_BYTES);
+          for (int c = 0; c < C::SUBS; ++c)
+            tma_load_2d(sV(ks) + c * XA_SUB_N, &tmV, &v_full[ks], ck + 64 * c, s.ks + t * XA_BN);
+        }
+      }
+      if (*abort_flag) {
+        // wait (bounded, ignoring the abort flag) for the last loads this thread issued
+        volatile int never = 0;
+        for (int c = max(qc - C::QS, 0); c < qc; ++c) mbar_wait(&q_full[c % C::QS], (c / C::QS) & 1, &never, 103);
+        for (int c = max(g - C::KS, 0); c < g; ++c) {
+          mbar_wait(&k_full[c % C::KS], (c / C::KS) & 1, &never, 103);
+          if (c + 1 < g || v_out) mbar_wait(&v_full[c % C::VS], (c / C::VS) & 1, &never, 103);
+        }
+      }
+    }
+  } else if (warp == 5) {
+    const int fmt = p.f16 ? 0 : 1;
+    const uint32_t base = smem_u32(smem);
+    const uint64_t dk = sdesc_kmajor_sw128(base), dv = sdesc_mnmajor_sw128(base, XA_SUB_N);
+    const uint32_t k_hi = (uint32_t)(dk >> 32), k_lo = (uint32_t)dk;
+    const uint32_t v_hi = (uint32_t)(dv >> 32), v_lo = (uint32_t)dv;
+    const uint32_t idesc_o = make_idesc(128, D, fmt, fmt, 0, 1);
+    const uint32_t t_o = tmem + 128;
+    auto off16 = [&](const uint8_t* x) { return (smem_u32(x) - base) >> 4; };
+    int g = 0, qc = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
+      const int tile = item % qtiles, rest = item / qtiles;
+      const int b = rest / p.heads;
+      const XSeq s = make_seq(p, b);
+      const int T = tile * XA_BM < s.lq ? (s.seen + XA_BN - 1) / XA_BN : 0;
+      if (T == 0) continue;
+      ok = warp_wait(&q_full[qc % C::QS], (qc / C::QS) & 1, abort_flag, 104);
+      auto scores = [&](int t) {
+        const int n = g + (t > 0 ? 1 : 0), ks = n % C::KS;
+        if (!warp_wait(&k_full[ks], (n / C::KS) & 1, abort_flag, 105)) return false;
+        tc_fence_after();
+        const int cols = (min(XA_BN, s.seen - t * XA_BN) + 15) & ~15;
+        const uint32_t idesc = make_idesc(128, cols, fmt, fmt, 0, 0);
+        const uint32_t qlo = k_lo + off16(sQ(qc % C::QS)), klo = k_lo + off16(sK(ks));
+        const uint32_t t_s = tmem + 64 * (n & 1);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_ss_lo(t_s, qlo + (k >> 2) * (XA_SUB_M >> 4) + 2 * (k & 3), klo + (k >> 2) * (XA_SUB_N >> 4) + 2 * (k & 3),
+                    k_hi, idesc, k != 0);
+        commit_elect(&s_full[n & 1]);
+        commit_elect(&k_empty[ks]);
+        if (t == T - 1) commit_elect(&q_empty[qc % C::QS]);
+        return true;
+      };
+      ok = ok && scores(0);
+      for (int t = 0; t < T && ok; ++t, ++g) {
+        if (t + 1 < T && !scores(t + 1)) {
+          ok = false;
+          break;
+        }
+        const int vs = g % C::VS;
+        const int keys = min(XA_BN, s.seen - t * XA_BN), steps = (keys + 15) >> 4;
+        const uint64_t vis = visible64(p, s, t * XA_BN, lane);
+        ok = warp_wait(&v_full[vs], (g / C::VS) & 1, abort_flag, 106);
+        if (!ok) break;
+        const uint64_t all = steps == 4 ? ~0ull : (1ull << (16 * steps)) - 1;
+        if ((vis & all) != all) zero_rows(sV(vs), C::SUBS, 16 * steps, vis, lane);
+        ok = warp_wait(&p_full[g & 1], (g >> 1) & 1, abort_flag, 107) &&
+             (t > 0 || qc == 0 || warp_wait(o_empty, (qc - 1) & 1, abort_flag, 108));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t vlo = v_lo + off16(sV(vs)), t_p = tmem + 64 * (g & 1);
+        for (int k = 0; k < steps; ++k)
+          mma_ts_lo(t_o, t_p + 8 * k, vlo + k * (2048 >> 4), v_hi, idesc_o, (t > 0 || k > 0) ? 1u : 0u);
+        commit_elect(&o_full[g & 1]);
+        commit_elect(&v_empty[vs]);
+      }
+      qc++;
+    }
+    commit_elect(done);
+    volatile int never = 0;
+    warp_wait(done, 0, &never, 109);
+  } else {
+    const int r = warp * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    const uint32_t t_o = tmem + lane_off + 128;
+    const float NEG_INF = -INFINITY;
+    const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
+    int g = 0;
+    for (int item = blockIdx.x; item < num_items; item += gridDim.x) {
+      const int tile = item % qtiles, rest = item / qtiles;
+      const int h = rest % p.heads, b = rest / p.heads;
+      const XSeq s = make_seq(p, b);
+      if (tile * XA_BM >= s.lq) continue;
+      const int T = (s.seen + XA_BN - 1) / XA_BN;
+      const int i = tile * XA_BM + r;
+      const bool row_ok = i < s.lq;
+      const long long row = s.qs + i;
+      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + h * D;
+      float* lse = p.lse ? p.lse + (long long)h * p.total_q + row : nullptr;
+      if (T == 0) {
+        if (row_ok) {
+          zero_row16<D>(dst);
+          if (lse) *lse = NEG_INF;
+        }
+        continue;
+      }
+      bool bad = false;
+      float m = NEG_INF, l = 0.f;
+      for (int t = 0; t < T; ++t, ++g) {
+        const uint64_t vis = visible64(p, s, t * XA_BN, lane);
+        const uint32_t t_s = tmem + lane_off + 64 * (g & 1);
+        if (!mbar_wait(&s_full[g & 1], (g >> 1) & 1, abort_flag, 110)) bad = true;
+        tc_fence_after();
+        uint32_t sa[32], sb[32];
+        tmem_ld32_async(t_s, sa);
+        tmem_ld32_async(t_s + 32, sb);
+        tmem_wait_ld();
+        if (vis != ~0ull) {
+          hide32(sa, (uint32_t)vis);
+          hide32(sb, (uint32_t)(vis >> 32));
+        }
+        float mx8[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx8[e] = NEG_INF;
+        max_chunk(sa, mx8);
+        max_chunk(sb, mx8);
+        const float mx =
+            fmaxf(fmax3(fmax3(mx8[0], mx8[1], mx8[2]), mx8[3], mx8[4]), fmax3(mx8[5], mx8[6], mx8[7]));
+        const float m_tile = mx * p.scale_log2;  // scale > 0; -inf when the row sees none of these keys
+        const bool move = m_tile > m + XA_RESCALE_LOG2;
+        const float alpha = move ? fast_exp2(m - m_tile) : 1.f;
+        l *= alpha;
+        if (__any_sync(0xffffffffu, move && m != NEG_INF)) {
+          // some row of this warp moves a finite maximum: rescale O once P V of the last tile is done
+          if (!mbar_wait(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 111)) bad = true;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32], w[16];
+            tmem_ld32_async(t_o + 32 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(o[16 * hh + e]) * alpha);
+              tmem_st16(t_o + 32 * c + 16 * hh, w);
+            }
+          }
+        }
+        if (move) m = m_tile;
+        const float mu = m == NEG_INF ? 0.f : m;
+        const uint64_t negm2 = f2(-mu, -mu);
+        uint64_t acc[4] = {0, 0, 0, 0};
+        uint32_t w[16];
+        exp_chunk(sa, scale2, negm2, acc, w, p.f16);
+        tmem_st16(t_s, w);
+        exp_chunk(sb, scale2, negm2, acc, w, p.f16);
+        tmem_st16(t_s + 16, w);
+        const float2 sum = f2_split(fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3])));
+        l += sum.x + sum.y;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g & 1]);
+      }
+      if (!mbar_wait(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 112)) bad = true;
+      tc_fence_after();
+      const bool store = row_ok && !bad && !*abort_flag;
+      store_row16<D>(t_o, l > 0.f ? 1.f / l : 0.f, p.f16, store, dst);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_empty);
+      if (store && lse) *lse = l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : NEG_INF;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, 256);
+}
+
+// ------------------------------------------------------------------------------------------------ dQ
+// The forward's walk again: a CTA holds Q and dO of a query tile, walks the keys, recomputes P from the stored lse
+// and accumulates dQ in TMEM. It also forms delta = rowsum(dO * O), which the dK / dV kernel reads, so O and dO are
+// read once here and delta needs no launch of its own. TMEM (256 columns): S, dP, dQ; dS (packed pairs) gets columns
+// of its own where they fit (D = 64), so that S and dP of the next tile are multiplied while this one's dS is
+// formed; at D = 128 it lies over S.
+template <int D>
+struct XDq {
+  static constexpr int SUBS = D / 64;
+  static constexpr bool SEP = D == 64;
+  static constexpr int QS = SEP ? 2 : 1, KS = SEP ? 2 : 1;
+  static constexpr int Q_BYTES = SUBS * XA_SUB_M, T_BYTES = SUBS * XA_SUB_N;
+  static constexpr int TILES = 2 * QS * Q_BYTES + 2 * KS * T_BYTES;
+  static constexpr int SMEM = TILES + 1024 + 512;
+  static constexpr int COL_DQ = 128, COL_DS = SEP ? 192 : 0;
+};
+
+template <int D>
+__global__ void __launch_bounds__(XA_THREADS, 2)
+    cross_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
+                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const XParams p,
+                    const XGrad gr, int num_items, int qtiles) {
+  using C = XDq<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  auto sQ = [&](int s) { return smem + s * C::Q_BYTES; };
+  auto sDO = [&](int s) { return smem + (C::QS + s) * C::Q_BYTES; };
+  auto sK = [&](int s) { return smem + 2 * C::QS * C::Q_BYTES + s * C::T_BYTES; };
+  auto sV = [&](int s) { return smem + 2 * C::QS * C::Q_BYTES + (C::KS + s) * C::T_BYTES; };
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::TILES);
+  uint64_t* q_full = bars;          // [QS] Q and dO
+  uint64_t* q_empty = bars + 2;     // [QS]
+  uint64_t* k_full = bars + 4;      // [KS]
+  uint64_t* k_empty = bars + 6;     // [KS]
+  uint64_t* v_full = bars + 8;      // [KS]
+  uint64_t* v_empty = bars + 10;    // [KS]
+  uint64_t* sdp_full = bars + 12;   // S and dP of a tile are in TMEM
+  uint64_t* sdp_empty = bars + 13;  // the softmax holds them in registers (4 arrivals)
+  uint64_t* ds_full = bars + 14;    // dS is in TMEM (4 arrivals)
+  uint64_t* dq_full = bars + 15;    // one phase per dS K
+  uint64_t* dq_empty = bars + 16;   // the softmax has read an item's dQ (4 arrivals)
+  uint64_t* done = bars + 17;
+  constexpr int NBARS = 18;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < NBARS; ++i) mbar_init(&bars[i], (i == 13 || i == 14 || i == 16) ? 4 : 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmDO);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dep_wait();
+
+  if (warp == 4) {
+    if (lane == 0) {
+      int g = 0, qc = 0;
+      bool ok = true, v_out = true;  // v_out: V of the last counted tile was issued
+      for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
+        const int tile = item % qtiles, rest = item / qtiles;
+        const int h = rest % p.heads, b = rest / p.heads;
+        const XSeq s = make_seq(p, b);
+        const int T = tile * XA_BM < s.lq ? (s.seen + XA_BN - 1) / XA_BN : 0;
+        if (T == 0) continue;
+        const int cq = h * D, ck = (h / p.group) * D;
+        const int qs = qc % C::QS;
+        if (qc >= C::QS && !mbar_wait(&q_empty[qs], ((qc / C::QS) - 1) & 1, abort_flag, 120)) break;
+        mbar_arrive_expect_tx(&q_full[qs], 2 * C::Q_BYTES);
+        for (int c = 0; c < C::SUBS; ++c) {
+          tma_load_2d(sQ(qs) + c * XA_SUB_M, &tmQ, &q_full[qs], cq + 64 * c, s.qs + tile * XA_BM);
+          tma_load_2d(sDO(qs) + c * XA_SUB_M, &tmDO, &q_full[qs], cq + 64 * c, s.qs + tile * XA_BM);
+        }
+        qc++;
+        for (int t = 0; t < T; ++t, ++g) {
+          const int ks = g % C::KS;
+          if (g >= C::KS && !mbar_wait(&v_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 121)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&v_full[ks], C::T_BYTES);
+          for (int c = 0; c < C::SUBS; ++c)
+            tma_load_2d(sV(ks) + c * XA_SUB_N, &tmV, &v_full[ks], ck + 64 * c, s.ks + t * XA_BN);
+          if (g >= C::KS && !mbar_wait(&k_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 122)) {
+            g++;
+            ok = v_out = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&k_full[ks], C::T_BYTES);
+          for (int c = 0; c < C::SUBS; ++c)
+            tma_load_2d(sK(ks) + c * XA_SUB_N, &tmK, &k_full[ks], ck + 64 * c, s.ks + t * XA_BN);
+        }
+      }
+      if (*abort_flag) {
+        volatile int never = 0;
+        for (int c = max(qc - C::QS, 0); c < qc; ++c) mbar_wait(&q_full[c % C::QS], (c / C::QS) & 1, &never, 123);
+        for (int c = max(g - C::KS, 0); c < g; ++c) {
+          mbar_wait(&v_full[c % C::KS], (c / C::KS) & 1, &never, 123);
+          if (c + 1 < g || v_out) mbar_wait(&k_full[c % C::KS], (c / C::KS) & 1, &never, 123);
+        }
+      }
+    }
+  } else if (warp == 5) {
+    const int fmt = p.f16 ? 0 : 1;
+    const uint32_t base = smem_u32(smem);
+    const uint64_t dk = sdesc_kmajor_sw128(base), dm = sdesc_mnmajor_sw128(base, XA_SUB_N);
+    const uint32_t k_hi = (uint32_t)(dk >> 32), k_lo = (uint32_t)dk;
+    const uint32_t m_hi = (uint32_t)(dm >> 32), m_lo = (uint32_t)dm;
+    const uint32_t idesc_q = make_idesc(128, D, fmt, fmt, 0, 1);
+    auto off16 = [&](const uint8_t* x) { return (smem_u32(x) - base) >> 4; };
+    int g = 0, qc = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
+      const int tile = item % qtiles, rest = item / qtiles;
+      const int b = rest / p.heads;
+      const XSeq s = make_seq(p, b);
+      const int T = tile * XA_BM < s.lq ? (s.seen + XA_BN - 1) / XA_BN : 0;
+      if (T == 0) continue;
+      const int qs = qc % C::QS;
+      ok = warp_wait(&q_full[qs], (qc / C::QS) & 1, abort_flag, 124);
+      // S = Q K^T and dP = dO V^T of tile t, which is tile n of the walk
+      auto products = [&](int t, int n) {
+        const int ks = n % C::KS;
+        const int keys = min(XA_BN, s.seen - t * XA_BN), cols = (keys + 15) & ~15;
+        const uint64_t vis = visible64(p, s, t * XA_BN, lane);
+        if (!warp_wait(&k_full[ks], (n / C::KS) & 1, abort_flag, 125) ||
+            !warp_wait(&v_full[ks], (n / C::KS) & 1, abort_flag, 125))
+          return false;
+        const uint64_t all = cols == 64 ? ~0ull : (1ull << cols) - 1;
+        if ((vis & all) != all) zero_rows(sK(ks), C::SUBS, cols, vis, lane);  // dS K multiplies them by zero
+        tc_fence_after();
+        const uint32_t idesc = make_idesc(128, cols, fmt, fmt, 0, 0);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t alo = k_lo + off16(half ? sDO(qs) : sQ(qs)), blo = k_lo + off16(half ? sV(ks) : sK(ks));
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_ss_lo(tmem + 64 * half, alo + (k >> 2) * (XA_SUB_M >> 4) + 2 * (k & 3),
+                      blo + (k >> 2) * (XA_SUB_N >> 4) + 2 * (k & 3), k_hi, idesc, k != 0);
+        }
+        commit_elect(sdp_full);
+        commit_elect(&v_empty[ks]);
+        if (t == T - 1) commit_elect(&q_empty[qs]);
+        return true;
+      };
+      // S and dP of the last item's last tile: their readers are done once its dS was written
+      ok = ok && products(0, g);
+      for (int t = 0; t < T && ok; ++t, ++g) {
+        if (C::SEP && t + 1 < T)
+          ok = warp_wait(sdp_empty, g & 1, abort_flag, 126) && products(t + 1, g + 1);
+        ok = ok && warp_wait(ds_full, g & 1, abort_flag, 127) &&
+             (t > 0 || qc == 0 || warp_wait(dq_empty, (qc - 1) & 1, abort_flag, 128));
+        if (!ok) break;
+        tc_fence_after();
+        const int ks = g % C::KS, steps = (min(XA_BN, s.seen - t * XA_BN) + 15) >> 4;
+        const uint32_t mlo = m_lo + off16(sK(ks));
+        for (int k = 0; k < steps; ++k)
+          mma_ts_lo(tmem + C::COL_DQ, tmem + C::COL_DS + 8 * k, mlo + k * (2048 >> 4), m_hi, idesc_q,
+                    (t > 0 || k > 0) ? 1u : 0u);
+        commit_elect(dq_full);
+        commit_elect(&k_empty[ks]);
+        if (!C::SEP && t + 1 < T) ok = products(t + 1, g + 1);
+      }
+      qc++;
+    }
+    commit_elect(done);
+    volatile int never = 0;
+    warp_wait(done, 0, &never, 129);
+  } else {
+    const int r = warp * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    const uint32_t t_s = tmem + lane_off, t_ds = t_s + C::COL_DS, t_dq = t_s + C::COL_DQ;
+    const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
+    int g = 0;
+    for (int item = blockIdx.x; item < num_items; item += gridDim.x) {
+      const int tile = item % qtiles, rest = item / qtiles;
+      const int h = rest % p.heads, b = rest / p.heads;
+      const XSeq s = make_seq(p, b);
+      if (tile * XA_BM >= s.lq) continue;
+      const int T = (s.seen + XA_BN - 1) / XA_BN;
+      const int i = tile * XA_BM + r;
+      const bool row_ok = i < s.lq;
+      const long long row = s.qs + i;
+      float delta = 0.f, lse = -INFINITY;
+      if (row_ok) {
+        const uint4* po = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.out) + row * p.ldo + h * D);
+        const uint4* pd =
+            reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(gr.dout) + row * gr.lddo + h * D);
+        lse = __ldg(p.lse + (long long)h * p.total_q + row);
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 a = __ldg(po + c), d = __ldg(pd + c);
+          const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, dw[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[e] = fmaf(unpack_hi(aw[e], p.f16), unpack_hi(dw[e], p.f16),
+                          fmaf(unpack_lo(aw[e], p.f16), unpack_lo(dw[e], p.f16), acc[e]));
+        }
+        delta = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+        gr.delta[(long long)h * p.total_q + row] = delta;
+      }
+      uint16_t* dst = reinterpret_cast<uint16_t*>(gr.dq) + row * gr.lddq + h * D;
+      if (T == 0) {
+        if (row_ok) zero_row16<D>(dst);
+        continue;
+      }
+      // a row that saw no key has lse = -inf: with +inf instead its probabilities come out as zero
+      const float l2 = lse == -INFINITY ? INFINITY : lse * XA_LOG2E;
+      const uint64_t negl2 = f2(-l2, -l2), negd2 = f2(-delta, -delta);
+      bool bad = false;
+      for (int t = 0; t < T; ++t, ++g) {
+        const uint64_t vis = visible64(p, s, t * XA_BN, lane);
+        if (!mbar_wait(sdp_full, g & 1, abort_flag, 130)) bad = true;
+        tc_fence_after();
+        uint32_t w[2][16];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t sc[32], dp[32];
+          tmem_ld32_async(t_s + 32 * c, sc);
+          tmem_ld32_async(t_s + 64 + 32 * c, dp);
+          tmem_wait_ld();
+          if (c == 1 && C::SEP) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sdp_empty);
+          }
+          const uint32_t v = (uint32_t)(vis >> (32 * c));
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 x = f2_split(ffma2(f2(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), scale2, negl2));
+            const uint64_t pr = f2(fast_exp2(x.x), fast_exp2(x.y));
+            float2 d = f2_split(fmul2(pr, fadd2(f2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), negd2)));
+            if (v != 0xffffffffu) {
+              d.x = (v >> e) & 1u ? d.x : 0.f;
+              d.y = (v >> (e + 1)) & 1u ? d.y : 0.f;
+            }
+            w[c][e >> 1] = pack_2(d.x, d.y, p.f16);
+          }
+        }
+        // dS of the last tile must have been multiplied before its columns are written again
+        if (C::SEP && g > 0 && !mbar_wait(dq_full, (g - 1) & 1, abort_flag, 131)) bad = true;
+        tmem_st16(t_ds, w[0]);
+        tmem_st16(t_ds + 16, w[1]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_full);
+      }
+      if (!mbar_wait(dq_full, (g - 1) & 1, abort_flag, 132)) bad = true;
+      tc_fence_after();
+      store_row16<D>(t_dq, p.scale, p.f16, row_ok && !bad && !*abort_flag, dst);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dq_empty);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, 256);
+}
+
+// ------------------------------------------------------------------------------------------------ dK, dV
+// A CTA (one an SM) holds K and V of 128 keys of one key head and walks the query tiles of 64 rows of every head of
+// the group, or a part of them when there are fewer key tiles than SMs: the parts are then written in fp32 and added
+// in a fixed order by a second launch, so results never depend on the order in which CTAs finish. The products are
+// taken transposed (S^T = K Q^T, dP^T = V dO^T), which puts P^T and dS^T into TMEM in the form of the A operand of
+// dV += P^T dO and dK += dS^T Q, with dO and Q read as they lie. Two score buffers, each with a softmax warpgroup of
+// its own: one forms P and dS while the tensor core works on the other. TMEM (512 columns): 2 x (S^T 64, dP^T 64),
+// dV, dK.
+constexpr int XB_THREADS = 320;  // warps 0..7 softmax, 8 loads, 9 MMA
+template <int D>
+struct XDkv {
+  static constexpr int SUBS = D / 64;
+  static constexpr int STAGES = 4;
+  static constexpr int K_BYTES = SUBS * XA_SUB_M, T_BYTES = SUBS * XA_SUB_N;
+  static constexpr int TILES = 2 * K_BYTES + STAGES * 2 * T_BYTES;
+  static constexpr int STATS = STAGES * 2 * XA_BN * 4;
+  static constexpr int SMEM = TILES + STATS + 1024 + 512;
+  static constexpr int COL_DV = 256, COL_DK = 256 + D;
+};
+
+template <int D>
+__global__ void __launch_bounds__(XB_THREADS, 1)
+    cross_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
+                     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const XParams p,
+                     const XGrad gr, int ktiles, int splits) {
+  using C = XDkv<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sK = smem;
+  uint8_t* sV = smem + C::K_BYTES;
+  auto sQ = [&](int s) { return smem + 2 * C::K_BYTES + 2 * s * C::T_BYTES; };
+  auto sDO = [&](int s) { return smem + 2 * C::K_BYTES + (2 * s + 1) * C::T_BYTES; };
+  float* stats = reinterpret_cast<float*>(smem + C::TILES);  // per stage: -lse * log2(e) [64], -delta [64]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::TILES + C::STATS);
+  uint64_t* kv_full = bars;
+  uint64_t* full = bars + 1;      // [STAGES]
+  uint64_t* empty = bars + 5;     // [STAGES]
+  uint64_t* sdp_full = bars + 9;  // [2]
+  uint64_t* ds_full = bars + 11;  // [2] 4 arrivals
+  uint64_t* done = bars + 13;
+  constexpr int NBARS = 14;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < NBARS; ++i) mbar_init(&bars[i], (i == 11 || i == 12) ? 4 : 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmDO);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dep_wait();
+
+  const int part = blockIdx.x % splits;
+  const int kt = (blockIdx.x / splits) % ktiles;
+  const int rest = blockIdx.x / splits / ktiles;
+  const int hk = rest % p.kv_heads, b = rest / p.kv_heads;
+  const XSeq s = make_seq(p, b);
+  const int j0 = kt * XA_BM;
+  const int qtiles = (s.lq + XA_BN - 1) / XA_BN;
+  const long long steps_all = (long long)p.group * qtiles;
+  const int t0 = (int)(steps_all * part / splits);
+  const int t1 = j0 < s.seen ? (int)(steps_all * (part + 1) / splits) : t0;  // hidden keys get zeros
+  const int T = j0 < s.lk ? t1 - t0 : 0;
+
+  if (warp == 8) {
+    if (T > 0) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(kv_full, 2 * C::K_BYTES);
+        for (int c = 0; c < C::SUBS; ++c) {
+          tma_load_2d(sK + c * XA_SUB_M, &tmK, kv_full, hk * D + 64 * c, s.ks + j0);
+          tma_load_2d(sV + c * XA_SUB_M, &tmV, kv_full, hk * D + 64 * c, s.ks + j0);
+        }
+      }
+      int t = 0;
+      for (; t < T; ++t) {
+        const int st = t % C::STAGES;
+        const int h = hk * p.group + (t0 + t) / qtiles, i0 = ((t0 + t) % qtiles) * XA_BN;
+        // the row statistics travel with the tile; rows behind the end get probability zero
+        float l2[2], dl[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = i0 + lane + 32 * e;
+          float lse = -INFINITY, d = 0.f;
+          if (i < s.lq) {
+            const long long at = (long long)h * p.total_q + s.qs + i;
+            lse = __ldg(p.lse + at);
+            d = gr.delta[at];
+          }
+          l2[e] = lse == -INFINITY ? -INFINITY : -lse * XA_LOG2E;
+          dl[e] = -d;
+        }
+        if (t >= C::STAGES && !warp_wait(&empty[st], ((t / C::STAGES) - 1) & 1, abort_flag, 140)) break;
+        float* sp = stats + st * 2 * XA_BN;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          sp[lane + 32 * e] = l2[e];
+          sp[XA_BN + lane + 32 * e] = dl[e];
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&full[st], 2 * C::T_BYTES);
+          for (int c = 0; c < C::SUBS; ++c) {
+            tma_load_2d(sQ(st) + c * XA_SUB_N, &tmQ, &full[st], h * D + 64 * c, s.qs + i0);
+            tma_load_2d(sDO(st) + c * XA_SUB_N, &tmDO, &full[st], h * D + 64 * c, s.qs + i0);
+          }
+        }
+      }
+      if (*abort_flag && lane == 0) {
+        volatile int never = 0;
+        mbar_wait(kv_full, 0, &never, 141);
+        for (int c = max(t - C::STAGES, 0); c < t; ++c) mbar_wait(&full[c % C::STAGES], (c / C::STAGES) & 1, &never, 141);
+      }
+    }
+  } else if (warp == 9) {
+    const int fmt = p.f16 ? 0 : 1;
+    const uint32_t base = smem_u32(smem);
+    const uint64_t dk = sdesc_kmajor_sw128(base), dm = sdesc_mnmajor_sw128(base, XA_SUB_N);
+    const uint32_t k_hi = (uint32_t)(dk >> 32), k_lo = (uint32_t)dk;
+    const uint32_t m_hi = (uint32_t)(dm >> 32), m_lo = (uint32_t)dm;
+    const uint32_t idesc_s = make_idesc(128, XA_BN, fmt, fmt, 0, 0), idesc_g = make_idesc(128, D, fmt, fmt, 0, 1);
+    auto off16 = [&](const uint8_t* x) { return (smem_u32(x) - base) >> 4; };
+    bool ok = T > 0 && warp_wait(kv_full, 0, abort_flag, 142);
+    auto products = [&](int t) {
+      const int st = t % C::STAGES;
+      if (!warp_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 143)) return false;
+      const int rows = s.lq - ((t0 + t) % qtiles) * XA_BN;
+      if (rows < XA_BN) {
+        // rows behind the end: dV and dK multiply them by zero probabilities
+        zero_rows(sQ(st), C::SUBS, XA_BN, (1ull << rows) - 1, lane);
+        zero_rows(sDO(st), C::SUBS, XA_BN, (1ull << rows) - 1, lane);
+      }
+      tc_fence_after();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t alo = k_lo + off16(half ? sV : sK), blo = k_lo + off16(half ? sDO(st) : sQ(st));
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_ss_lo(tmem + 128 * (t & 1) + 64 * half, alo + (k >> 2) * (XA_SUB_M >> 4) + 2 * (k & 3),
+                    blo + (k >> 2) * (XA_SUB_N >> 4) + 2 * (k & 3), k_hi, idesc_s, k != 0);
+      }
+      commit_elect(&sdp_full[t & 1]);
+      return true;
+    };
+    ok = ok && products(0) && (T < 2 || products(1));
+    for (int t = 0; t < T && ok; ++t) {
+      ok = warp_wait(&ds_full[t & 1], (t >> 1) & 1, abort_flag, 144);
+      if (!ok) break;
+      tc_fence_after();
+      const int st = t % C::STAGES;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t mlo = m_lo + off16(half ? sQ(st) : sDO(st));
+#pragma unroll
+        for (int k = 0; k < XA_BN / 16; ++k)
+          mma_ts_lo(tmem + (half ? C::COL_DK : C::COL_DV), tmem + 128 * (t & 1) + 64 * half + 8 * k,
+                    mlo + k * (2048 >> 4), m_hi, idesc_g, (t > 0 || k > 0) ? 1u : 0u);
+      }
+      commit_elect(&empty[st]);
+      if (t + 2 < T) ok = products(t + 2);
+    }
+    commit_elect(done);
+    volatile int never = 0;
+    warp_wait(done, 0, &never, 145);
+  } else {
+    const int grp = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lane_off + 128 * grp;
+    const int j = j0 + r;
+    const long long row = s.ks + j;
+    bool vis = j < s.seen;
+    if (vis && p.key_mask) vis = __ldg(p.key_mask + row) != 0;
+    const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
+    bool bad = false;
+    for (int t = grp; t < T; t += 2) {
+      const int st = t % C::STAGES;
+      const float* sp = stats + st * 2 * XA_BN;
+      if (!mbar_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 146)) bad = true;
+      if (!mbar_wait(&sdp_full[grp], (t >> 1) & 1, abort_flag, 147)) bad = true;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t sc[32], dp[32], wp[16], wd[16];
+        tmem_ld32_async(t_s + 32 * c, sc);
+        tmem_ld32_async(t_s + 64 + 32 * c, dp);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 l4 = *reinterpret_cast<const float4*>(sp + 32 * c + e);
+          const float4 d4 = *reinterpret_cast<const float4*>(sp + XA_BN + 32 * c + e);
+#pragma unroll
+          for (int f = 0; f < 4; f += 2) {
+            const uint64_t nl = f ? f2(l4.z, l4.w) : f2(l4.x, l4.y), nd = f ? f2(d4.z, d4.w) : f2(d4.x, d4.y);
+            const float2 x =
+                f2_split(ffma2(f2(__uint_as_float(sc[e + f]), __uint_as_float(sc[e + f + 1])), scale2, nl));
+            const float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
+            const float2 d = f2_split(
+                fmul2(f2(p0, p1), fadd2(f2(__uint_as_float(dp[e + f]), __uint_as_float(dp[e + f + 1])), nd)));
+            wp[(e + f) >> 1] = vis ? pack_2(p0, p1, p.f16) : 0u;
+            wd[(e + f) >> 1] = vis ? pack_2(d.x, d.y, p.f16) : 0u;
+          }
+        }
+        tmem_st16(t_s + 16 * c, wp);
+        tmem_st16(t_s + 64 + 16 * c, wd);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ds_full[grp]);
+    }
+    // warpgroup 0 stores dV, warpgroup 1 dK
+    if (!mbar_wait(done, 0, abort_flag, 148)) bad = true;
+    tc_fence_after();
+    const bool store = j < s.lk && !bad && !*abort_flag;
+    const uint32_t t_g = tmem + lane_off + (grp ? C::COL_DK : C::COL_DV);
+    const float f = grp ? p.scale : 1.f;
+    if (splits == 1) {
+      uint16_t* dst = reinterpret_cast<uint16_t*>(grp ? gr.dk : gr.dv) + row * (grp ? gr.lddk : gr.lddv) + hk * D;
+      if (T > 0)
+        store_row16<D>(t_g, f, p.f16, store, dst);
+      else if (store)
+        zero_row16<D>(dst);
+    } else {
+      const long long width = (long long)p.kv_heads * D;
+      float* dst = gr.partial + ((long long)(part * 2 + grp) * p.total_k + row) * width + hk * D;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (T > 0) {
+          tmem_ld32_async(t_g + 32 * c, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        if (store)
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(dst + 32 * c + e) =
+                make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 2]) * f,
+                            __uint_as_float(o[e + 3]) * f);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// dK and dV from the parts of the walk, in part order. Rows that belong to no sequence are left alone: a row is
+// written when some sequence of the batch covers it (uniform batches cover every row).
+__global__ void __launch_bounds__(256) cross_join_kernel(const XParams p, const XGrad gr, int splits, int width) {
+  grid_dep_wait();
+  const int vecs = width / 4;
+  const long long n = (long long)p.total_k * vecs;
+  const long long first = p.cu_k ? clampi(__ldg(p.cu_k), 0, p.total_k) : 0;
+  const long long last = p.cu_k ? clampi(__ldg(p.cu_k + p.batch), 0, p.total_k) : p.total_k;
+  for (long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x; at < 2 * n;
+       at += (long long)gridDim.x * blockDim.x) {
+    const int w = at >= n;
+    const long long i = at - w * n, row = i / vecs, c = (i - row * vecs) * 4;
+    if (row < first || row >= last) continue;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int sp = 0; sp < splits; ++sp) {
+      const float4 v = *reinterpret_cast<const float4*>(gr.partial + ((long long)(sp * 2 + w) * p.total_k + row) * width + c);
+      a.x += v.x;
+      a.y += v.y;
+      a.z += v.z;
+      a.w += v.w;
+    }
+    uint16_t* dst = reinterpret_cast<uint16_t*>(w ? gr.dk : gr.dv) + row * (w ? gr.lddk : gr.lddv) + c;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_2(a.x, a.y, p.f16), pack_2(a.z, a.w, p.f16));
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+static int sm_count() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 0;
+  return sms;
+}
+
+// Parts of the dK / dV walk: the number that ends soonest when every wave of CTAs costs its longest walk plus the
+// set-up, epilogue and joining of a part (about 6 tiles). One part writes its result at once.
+static int dkv_splits(long long ctas, long long tiles, int sms) {
+  long long best = 1, cost = -1;
+  for (long long n = 1; n <= 32 && n <= tiles; ++n) {
+    const long long waves = (ctas * n + sms - 1) / sms;
+    const long long c = waves * ((tiles + n - 1) / n + 6) + (n > 1 ? 6 : 0);
+    if (cost < 0 || c < cost) {
+      cost = c;
+      best = n;
+    }
+  }
+  return (int)best;
+}
+
+static int check_common(const void* q, const void* k, const void* v, const void* out, const int* cu_q, const int* cu_k,
+                        int batch, int max_q, int max_k, int total_q, int total_k, int heads, int kv_heads, int head_dim,
+                        long long ldq, long long ldk, long long ldv, long long ldo, float scale, int dtype) {
+  if (batch < 0 || max_q < 0 || max_k < 0 || total_q < 0 || total_k < 0 || heads <= 0 || kv_heads <= 0 ||
+      heads % kv_heads != 0)
+    return SA3_ERR_ARG;
+  if (!(scale > 0.f) || scale > 3.4e38f) return SA3_ERR_ARG;
+  if (head_dim != 64 && head_dim != 128) return SA3_ERR_UNSUPPORTED;
+  if (dtype != SA3_DT_BF16 && dtype != SA3_DT_F16) return SA3_ERR_DTYPE;
+  if (!cu_q && (long long)batch * max_q != total_q) return SA3_ERR_ARG;
+  if (!cu_k && (long long)batch * max_k != total_k) return SA3_ERR_ARG;
+  const long long wq = (long long)heads * head_dim, wk = (long long)kv_heads * head_dim;
+  if (ldq < wq || ldo < wq || ldk < wk || ldv < wk) return SA3_ERR_ARG;
+  if (total_q > 0 && (!q || !out)) return SA3_ERR_ARG;
+  if (total_k > 0 && (!k || !v)) return SA3_ERR_ARG;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || ((ldq | ldk | ldv | ldo) & 7))
+    return SA3_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(cu_k)) & 3) return SA3_ERR_ALIGN;
+  // grid and item counts stay in 32 bits
+  const long long items = ((long long)max_q / XA_BM + 1) * heads * (batch > 0 ? batch : 1);
+  const long long kitems = ((long long)max_k / XA_BM + 1) * kv_heads * (batch > 0 ? batch : 1);
+  if (heads > 65535 || items > (1LL << 30) || kitems > (1LL << 25)) return SA3_ERR_UNSUPPORTED;
+  return SA3_OK;
+}
+
+static XParams make_params(void* out, float* lse, const int* cu_q, const int* cu_k, const int* k_lens,
+                           const unsigned char* key_mask, int batch, int max_q, int max_k, int total_q, int total_k,
+                           int heads, int kv_heads, long long ldo, float scale, int dtype) {
+  XParams p = {};
+  p.cu_q = cu_q;
+  p.cu_k = cu_k;
+  p.k_lens = k_lens;
+  p.key_mask = key_mask;
+  p.batch = batch;
+  p.Lq = max_q;
+  p.Lk = max_k;
+  p.total_q = total_q;
+  p.total_k = total_k;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.group = heads / kv_heads;
+  p.scale = scale;
+  p.scale_log2 = scale * XA_LOG2E;
+  p.f16 = dtype == SA3_DT_F16;
+  p.out = out;
+  p.ldo = ldo;
+  p.lse = lse;
+  return p;
+}
+
+// Tensor map of a token-row buffer with boxes of 64 columns x `box` rows. A buffer without rows is never read:
+// its map is taken over `other`.
+static int token_map(CUtensorMap* m, const void* x, const void* other, int f16, long long width, long long rows,
+                     long long ld, int box) {
+  const auto dt = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return make_tmap_2d(m, rows > 0 ? x : other, dt, 2, width, rows > 0 ? rows : 1, ld, 64, box);
+}
+
+template <int D>
+static int launch_fwd(const XParams& p, const void* q, const void* k, const void* v, long long ldq, long long ldk,
+                      long long ldv, cudaStream_t st) {
+  CUtensorMap mq, mk, mv;
+  int rc;
+  const long long wq = (long long)p.heads * D, wk = (long long)p.kv_heads * D;
+  if ((rc = token_map(&mq, q, q, p.f16, wq, p.total_q, ldq, XA_BM))) return rc;
+  if ((rc = token_map(&mk, k, q, p.f16, wk, p.total_k, ldk, XA_BN))) return rc;
+  if ((rc = token_map(&mv, v, q, p.f16, wk, p.total_k, ldv, XA_BN))) return rc;
+  const int sms = sm_count();
+  if (sms <= 0) return SA3_ERR_LAUNCH;
+  const int qtiles = (p.Lq + XA_BM - 1) / XA_BM;
+  const int items = qtiles * p.heads * p.batch;
+  if ((rc = ensure_smem(cross_fwd_kernel<D>, XFwd<D>::SMEM))) return rc;
+  launch_ex(cross_fwd_kernel<D>, dim3(items < 2 * sms ? items : 2 * sms), dim3(XA_THREADS), XFwd<D>::SMEM, st, 1, mq,
+            mk, mv, p, items, qtiles);
+  return launch_status();
+}
+
+template <int D>
+static int launch_bwd(const XParams& p, const XGrad& g, const void* q, const void* k, const void* v, long long ldq,
+                      long long ldk, long long ldv, int splits, int sms, cudaStream_t st) {
+  CUtensorMap q128, do128, q64, do64, k64, v64, k128, v128;
+  int rc;
+  const long long wq = (long long)p.heads * D, wk = (long long)p.kv_heads * D;
+  const void* any = p.total_q > 0 ? q : k;
+  if ((rc = token_map(&q128, q, any, p.f16, wq, p.total_q, ldq, XA_BM))) return rc;
+  if ((rc = token_map(&q64, q, any, p.f16, wq, p.total_q, ldq, XA_BN))) return rc;
+  if ((rc = token_map(&do128, g.dout, any, p.f16, wq, p.total_q, g.lddo, XA_BM))) return rc;
+  if ((rc = token_map(&do64, g.dout, any, p.f16, wq, p.total_q, g.lddo, XA_BN))) return rc;
+  if ((rc = token_map(&k64, k, any, p.f16, wk, p.total_k, ldk, XA_BN))) return rc;
+  if ((rc = token_map(&v64, v, any, p.f16, wk, p.total_k, ldv, XA_BN))) return rc;
+  if ((rc = token_map(&k128, k, any, p.f16, wk, p.total_k, ldk, XA_BM))) return rc;
+  if ((rc = token_map(&v128, v, any, p.f16, wk, p.total_k, ldv, XA_BM))) return rc;
+  if (p.total_q > 0 && p.Lq > 0) {
+    const int qtiles = (p.Lq + XA_BM - 1) / XA_BM;
+    const int items = qtiles * p.heads * p.batch;
+    if ((rc = ensure_smem(cross_dq_kernel<D>, XDq<D>::SMEM))) return rc;
+    launch_ex(cross_dq_kernel<D>, dim3(items < 2 * sms ? items : 2 * sms), dim3(XA_THREADS), XDq<D>::SMEM, st, 1, q128,
+              do128, k64, v64, p, g, items, qtiles);
+    if ((rc = launch_status())) return rc;
+  }
+  if (p.total_k > 0 && p.Lk > 0) {
+    const int ktiles = (p.Lk + XA_BM - 1) / XA_BM;
+    if ((rc = ensure_smem(cross_dkv_kernel<D>, XDkv<D>::SMEM))) return rc;
+    launch_ex(cross_dkv_kernel<D>, dim3((unsigned)(ktiles * p.kv_heads * p.batch * splits)), dim3(XB_THREADS),
+              XDkv<D>::SMEM, st, 1, q64, do64, k128, v128, p, g, ktiles, splits);
+    if ((rc = launch_status())) return rc;
+    if (splits > 1) {
+      const long long vecs = 2LL * p.total_k * p.kv_heads * D / 4;
+      const long long blocks = (vecs + 255) / 256;
+      launch_ex(cross_join_kernel, dim3((unsigned)(blocks < 8LL * sms ? blocks : 8LL * sms)), dim3(256), 0, st, 1, p, g,
+                splits, p.kv_heads * D);
+      if ((rc = launch_status())) return rc;
+    }
+  }
+  return SA3_OK;
+}
+
+// delta first, the parts of dK and dV behind it at a 16-byte boundary
+static long long delta_bytes(int heads, int total_q) { return (((long long)heads * total_q * 4) + 15) & ~15LL; }
+
+static int bwd_splits(int batch, int max_q, int max_k, int heads, int kv_heads, int sms) {
+  const long long ctas = (long long)((max_k + XA_BM - 1) / XA_BM) * kv_heads * batch;
+  const long long tiles = (long long)(heads / kv_heads) * ((max_q + XA_BN - 1) / XA_BN);
+  return ctas > 0 && tiles > 0 ? dkv_splits(ctas, tiles, sms) : 1;
+}
+
+}  // namespace sa3
+
+using namespace sa3;
+
+extern "C" int sa3_cross_attention(const void* q, const void* k, const void* v, void* out, float* lse,
+                                   const int* cu_seqlens_q, const int* cu_seqlens_k, const int* k_lens,
+                                   const unsigned char* key_mask, int batch, int max_seqlen_q, int max_seqlen_k,
+                                   int total_q, int total_k, int heads, int kv_heads, int head_dim, long long ldq,
+                                   long long ldk, long long ldv, long long ldo, float softmax_scale, int dtype,
+                                   void* stream) {
+  int rc = check_common(q, k, v, out, cu_seqlens_q, cu_seqlens_k, batch, max_seqlen_q, max_seqlen_k, total_q, total_k,
+                        heads, kv_heads, head_dim, ldq, ldk, ldv, ldo, softmax_scale, dtype);
+  if (rc) return rc;
+  if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(k_lens)) & 3) return SA3_ERR_ALIGN;
+  if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return SA3_OK;
+  const XParams p = make_params(out, lse, cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, batch, max_seqlen_q,
+                                max_seqlen_k, total_q, total_k, heads, kv_heads, ldo, softmax_scale, dtype);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int sms = sm_count();
+  if (sms <= 0) return SA3_ERR_LAUNCH;
+  if ((long long)max_seqlen_q * p.group <= XT_MAX_ROWS)
+    return cross_token(p, q, k, v, ldq, ldk, ldv, head_dim, sms, st);
+  return head_dim == 64 ? launch_fwd<64>(p, q, k, v, ldq, ldk, ldv, st) : launch_fwd<128>(p, q, k, v, ldq, ldk, ldv, st);
+}
+
+extern "C" int sa3_cross_attention_bwd_workspace(int batch, int max_seqlen_q, int max_seqlen_k, int total_q, int total_k,
+                                                 int heads, int kv_heads, int head_dim, long long* bytes) {
+  if (!bytes || batch < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || total_q < 0 || total_k < 0 || heads <= 0 ||
+      kv_heads <= 0 || heads % kv_heads != 0)
+    return SA3_ERR_ARG;
+  if (head_dim != 64 && head_dim != 128) return SA3_ERR_UNSUPPORTED;
+  const int sms = sm_count();
+  if (sms <= 0) return SA3_ERR_LAUNCH;
+  const int n = bwd_splits(batch, max_seqlen_q, max_seqlen_k, heads, kv_heads, sms);
+  *bytes = delta_bytes(heads, total_q) + (n > 1 ? 8LL * n * total_k * kv_heads * head_dim : 0);
+  return SA3_OK;
+}
+
+extern "C" int sa3_cross_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                                       const float* lse, void* dq, void* dk, void* dv, const int* cu_seqlens_q,
+                                       const int* cu_seqlens_k, const int* k_lens, const unsigned char* key_mask,
+                                       int batch, int max_seqlen_q, int max_seqlen_k, int total_q, int total_k, int heads,
+                                       int kv_heads, int head_dim, long long lddo, long long ldq, long long ldk,
+                                       long long ldv, long long ldo, long long lddq, long long lddk, long long lddv,
+                                       float softmax_scale, int dtype, void* workspace, long long workspace_bytes,
+                                       void* stream) {
+  int rc = check_common(q, k, v, out, cu_seqlens_q, cu_seqlens_k, batch, max_seqlen_q, max_seqlen_k, total_q, total_k,
+                        heads, kv_heads, head_dim, ldq, ldk, ldv, ldo, softmax_scale, dtype);
+  if (rc) return rc;
+  const long long wq = (long long)heads * head_dim, wk = (long long)kv_heads * head_dim;
+  if (lddo < wq || lddq < wq || lddk < wk || lddv < wk) return SA3_ERR_ARG;
+  if (total_q > 0 && (!dout || !dq || !lse)) return SA3_ERR_ARG;
+  if (total_k > 0 && (!dk || !dv)) return SA3_ERR_ARG;
+  if (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !aligned16(workspace) ||
+      ((lddo | lddq | lddk | lddv) & 7))
+    return SA3_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(k_lens)) & 3) return SA3_ERR_ALIGN;
+  if (batch == 0 || (total_q == 0 && total_k == 0)) return SA3_OK;
+  const int sms = sm_count();
+  if (sms <= 0) return SA3_ERR_LAUNCH;
+  const int splits = bwd_splits(batch, max_seqlen_q, max_seqlen_k, heads, kv_heads, sms);
+  const long long at = delta_bytes(heads, total_q);
+  const long long need = at + (splits > 1 ? 8LL * splits * total_k * kv_heads * head_dim : 0);
+  if (workspace_bytes < need || (need > 0 && !workspace)) return SA3_ERR_ARG;
+  const XParams p = make_params(const_cast<void*>(out), const_cast<float*>(lse), cu_seqlens_q, cu_seqlens_k, k_lens,
+                                key_mask, batch, max_seqlen_q, max_seqlen_k, total_q, total_k, heads, kv_heads, ldo,
+                                softmax_scale, dtype);
+  XGrad g = {};
+  g.dout = dout;
+  g.lddo = lddo;
+  g.dq = dq;
+  g.lddq = lddq;
+  g.dk = dk;
+  g.lddk = lddk;
+  g.dv = dv;
+  g.lddv = lddv;
+  g.delta = static_cast<float*>(workspace);
+  g.partial = splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(workspace) + at) : nullptr;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return head_dim == 64 ? launch_bwd<64>(p, g, q, k, v, ldq, ldk, ldv, splits, sms, st)
+                        : launch_bwd<128>(p, g, q, k, v, ldq, ldk, ldv, splits, sms, st);
+}

@@ -21,6 +21,7 @@ SA3_DEFINE_ERROR_READER(read_error_gemm)
 int read_error_glue(int* out);
 int read_error_attention(int* out);
 int read_error_peer(int* out);
+int read_error_cross(int* out);
 
 constexpr int GEMM_BM = 128;
 constexpr int GEMM_BN = 256;
@@ -1748,11 +1749,11 @@ extern "C" int sa3_version(void) { return 100; }
 extern "C" int sa3_get_device_error(int* err) {
   if (!err) return SA3_ERR_ARG;
   if (cudaDeviceSynchronize() != cudaSuccess) return SA3_ERR_LAUNCH;
-  int a = 0, b = 0, c = 0, d = 0, rc;
+  int a = 0, b = 0, c = 0, d = 0, e = 0, rc;
   if ((rc = read_error_gemm(&a)) || (rc = read_error_glue(&b)) || (rc = read_error_attention(&c)) ||
-      (rc = read_error_peer(&d)))
+      (rc = read_error_peer(&d)) || (rc = read_error_cross(&e)))
     return rc;
-  *err = a ? a : (b ? b : (c ? c : d));
+  *err = a ? a : (b ? b : (c ? c : (d ? d : e)));
   return SA3_OK;
 }
 

@@ -83,6 +83,15 @@ SIGNATURES = {
     "sa3_attention": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int,
                       c_int, c_int, c_ll, c_ll, c_ll, c_ll, c_int, c_int, c_float, c_int, c_vp, c_vp],
     "sa3_diff_attn_swa": [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_vp],
+    "sa3_rotary": [c_vp, c_vp, c_vp, c_vp, c_int, c_ll, c_int, c_int, c_int, c_int, c_ll, c_ll, c_ll, c_ll, c_vp, c_vp,
+                   c_ll, c_ll, c_int, c_int, c_float, c_vp],
+    "sa3_cross_attention": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int,
+                            c_int, c_int, c_int, c_ll, c_ll, c_ll, c_ll, c_float, c_int, c_vp],
+    "sa3_cross_attention_bwd_workspace": [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                          ctypes.POINTER(c_ll)],
+    "sa3_cross_attention_bwd": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int,
+                                c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_ll, c_ll, c_ll, c_ll, c_ll, c_ll,
+                                c_ll, c_ll, c_float, c_int, c_vp, c_ll, c_vp],
     "sa3_fp8_linear_noalloc": [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_ll, c_ll, c_ll, c_vp],
     "sa3_peer_box_bytes": [],
     "sa3_peer_box_alloc": [ctypes.POINTER(c_vp)],

@@ -301,6 +301,226 @@ def diff_attn_swa(q_bat: torch.Tensor, k_bat: torch.Tensor, v_bat: torch.Tensor,
     return out
 
 
+# ---------------------------------------------------------------------- rotary positions, cross-attention
+def _one_device(*ts: Optional[torch.Tensor]) -> torch.device:
+    """The device of the tensors, which must be CUDA tensors of one device."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("sa3_b200 ops run on CUDA tensors only (no CPU path)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError(f"tensors on {dev} and {t.device}: one call works on one device")
+    return dev
+
+
+def _rows_view(t: torch.Tensor, rows: Optional[int], cols: int, name: str, dtype: torch.dtype) -> int:
+    """Row stride of a token-row view [rows, cols]; refuses other shapes, types and strides."""
+    if t.dtype != dtype:
+        raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 2 or t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
+        raise RuntimeError(f"{name} must be [{'rows' if rows is None else rows}, {cols}], got {tuple(t.shape)}")
+    if t.stride(1) != 1 and t.shape[1] > 1 and t.numel() > 0:
+        raise RuntimeError(f"{name} must be a row-major view, got strides {t.stride()}")
+    # a single row has no stride of its own: torch may report anything there
+    return t.stride(0) if t.shape[0] > 1 else cols
+
+
+def _index(t: Optional[torch.Tensor], n: int, name: str) -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of {n} elements")
+    return t.data_ptr()
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0,
+                       original_length: int = 0, low_turns: float = 1.0, high_turns: float = 32.0, device="cuda"):
+    """(inv_freq fp64 [rot_dim / 2], scale) of a rotation, for `rotary`.
+
+    scaling: None       base^(-2i / rot_dim), scale 1
+             "linear"   all frequencies divided by `factor` (positions squeezed into the trained range)
+             "base"     the base raised to base * factor^(rot_dim / (rot_dim - 2)): the slowest pair is divided by
+                        `factor`, the fastest is kept
+             "ramp"     pairs that turn fewer than `low_turns` times within `original_length` positions are divided
+                        by `factor`, those that turn more than `high_turns` times are kept, a linear ramp over the
+                        turns joins them, and scale = 0.1 ln(factor) + 1
+    """
+    if rot_dim <= 0 or rot_dim % 2:
+        raise RuntimeError("rot_dim must be positive and even")
+    if not (base > 0 and factor > 0):
+        raise RuntimeError("base and factor must be positive")
+    if scaling == "base":
+        if rot_dim < 4:
+            raise RuntimeError("scaling the base needs rot_dim >= 4")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    f = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    scale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "ramp":
+        if original_length <= 0 or not high_turns > low_turns:
+            raise RuntimeError("ramp scaling needs original_length > 0 and high_turns > low_turns")
+        keep = ((original_length * f / (2 * math.pi) - low_turns) / (high_turns - low_turns)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+        scale = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "base"):
+        raise RuntimeError(f"unknown scaling {scaling!r}: None, 'linear', 'base' or 'ramp'")
+    return f.to(device), scale
+
+
+def rotary(q: torch.Tensor, inv_freq: torch.Tensor, *, heads: int, head_dim: int = 64,
+           k: Optional[torch.Tensor] = None, kv_heads: int = 0, row_pos: Optional[torch.Tensor] = None,
+           rows_per_batch: int = 0, offset: int = 0, interleaved: bool = False, scale: float = 1.0,
+           inverse: bool = False, out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None):
+    """q (and k) rotated by their positions: bf16, fp16 or fp32 token rows [rows, heads * head_dim].
+
+    inv_freq: fp64 [rot_dim / 2] (`rotary_frequencies`); the first rot_dim columns of every head are rotated, in pairs
+    (i, i + rot_dim/2), or (2i, 2i + 1) when interleaved, and multiplied by `scale`; the rest pass through. Row r has
+    position row_pos[r] (int32), or offset + r % rows_per_batch (0: one sequence). inverse=True rotates back, with the
+    same scale: the gradient. out / k_out may be q / k themselves. Returns out, or (out, k_out) when k is given.
+    """
+    dev = _one_device(q, inv_freq, k, row_pos, out, k_out)
+    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise RuntimeError(f"rotary works on bf16, fp16 or fp32, got {q.dtype}")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise RuntimeError("inv_freq must be a contiguous float64 tensor [rot_dim / 2]")
+    if heads <= 0 or head_dim <= 0:
+        raise RuntimeError("heads and head_dim must be positive")
+    if not -2 ** 62 < offset < 2 ** 62 or rows_per_batch < 0:
+        raise RuntimeError("offset out of range or negative rows_per_batch")
+    rows, rot_dim = q.shape[0], 2 * inv_freq.numel()
+    ldq = _rows_view(q, None, heads * head_dim, "q", q.dtype)
+    if out is None:
+        out = torch.empty(rows, heads * head_dim, device=dev, dtype=q.dtype)
+    ldqo = _rows_view(out, rows, heads * head_dim, "out", q.dtype)
+    ldk = ldko = 0
+    if k is not None:
+        if kv_heads <= 0:
+            raise RuntimeError("k needs kv_heads")
+        ldk = _rows_view(k, rows, kv_heads * head_dim, "k", q.dtype)
+        if k_out is None:
+            k_out = torch.empty(rows, kv_heads * head_dim, device=dev, dtype=q.dtype)
+        ldko = _rows_view(k_out, rows, kv_heads * head_dim, "k_out", q.dtype)
+    elif k_out is not None:
+        raise RuntimeError("k_out without k")
+    pos = _index(row_pos, rows, "row_pos")
+    _count()
+    with torch.cuda.device(dev):
+        rc = _lib.load().sa3_rotary(q.data_ptr(), out.data_ptr(), _ptr(k), _ptr(k_out), _dt(q), rows, heads,
+                                    kv_heads if k is not None else 0, head_dim, rot_dim, ldq, ldqo, ldk, ldko,
+                                    inv_freq.data_ptr(), pos, rows_per_batch, offset, int(interleaved), int(inverse),
+                                    float(scale), _stream())
+    _lib.check(rc, "sa3_rotary")
+    return out if k is None else (out, k_out)
+
+
+def _cross_args(q, k, v, heads, kv_heads, head_dim, batch, max_seqlen_q, max_seqlen_k, cu_seqlens_q, cu_seqlens_k,
+                k_lens, key_mask, softmax_scale):
+    """Checks shared by the two passes; (kv_heads, strides of q k v, index pointers, batch, scale)."""
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError(f"cross_attention works on bf16 or fp16, got {q.dtype}")
+    kv_heads = heads if kv_heads is None else kv_heads
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
+        raise RuntimeError("heads must be a positive multiple of kv_heads")
+    if head_dim not in (64, 128):
+        raise RuntimeError("cross_attention implements head_dim 64 and 128")
+    ld = (_rows_view(q, None, heads * head_dim, "q", q.dtype), _rows_view(k, None, kv_heads * head_dim, "k", q.dtype),
+          _rows_view(v, k.shape[0], kv_heads * head_dim, "v", q.dtype))
+    n = [None if c is None else c.numel() - 1 for c in (cu_seqlens_q, cu_seqlens_k)]
+    for x in n:
+        if x is not None:
+            batch = x
+    if batch < 0 or any(x is not None and x != batch for x in n):
+        raise RuntimeError("cu_seqlens_q and cu_seqlens_k must describe the same number of sequences")
+    if cu_seqlens_q is None and q.shape[0] != batch * max_seqlen_q:
+        raise RuntimeError("uniform queries need rows = batch * max_seqlen_q")
+    if cu_seqlens_k is None and k.shape[0] != batch * max_seqlen_k:
+        raise RuntimeError("uniform keys need rows = batch * max_seqlen_k")
+    if key_mask is not None and (key_mask.dtype not in (torch.bool, torch.uint8) or not key_mask.is_contiguous()
+                                 or key_mask.numel() != k.shape[0]):
+        raise RuntimeError("key_mask must be a contiguous bool or uint8 tensor with one element a key row")
+    idx = (_index(cu_seqlens_q, batch + 1, "cu_seqlens_q"), _index(cu_seqlens_k, batch + 1, "cu_seqlens_k"),
+           _index(k_lens, batch, "k_lens"), _ptr(key_mask))
+    scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else float(softmax_scale)
+    if not 0.0 < scale < math.inf:
+        raise RuntimeError("softmax_scale must be positive and finite")
+    return kv_heads, ld, idx, batch, scale
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, heads: int, kv_heads: Optional[int] = None,
+                    head_dim: int = 64, batch: int = 1, max_seqlen_q: int = 0, max_seqlen_k: int = 0,
+                    cu_seqlens_q=None, cu_seqlens_k=None, k_lens=None, key_mask=None,
+                    softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    lse: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """softmax(scale * q k^T) v over the visible keys, on token rows q [rows, heads * head_dim], k and v
+    [key rows, kv_heads * head_dim]; query head h reads key head h // (heads // kv_heads).
+
+    Uniform sequences of max_seqlen_q / max_seqlen_k rows, or packed ones: cu_seqlens_q / cu_seqlens_k (int32
+    [batch + 1], each optional), with max_seqlen the longest. k_lens (int32 [batch]): how many keys of a sequence are
+    visible; key_mask (bool or uint8, one element a key row): zero hides a key. Rows that see no key give zeros and
+    lse = -inf. Returns out, or (out, lse) with return_lse (lse fp32 [heads, rows], which the backward pass takes).
+    """
+    dev = _one_device(q, k, v, cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, out, lse)
+    kv_heads, ld, idx, batch, scale = _cross_args(q, k, v, heads, kv_heads, head_dim, batch, max_seqlen_q, max_seqlen_k,
+                                                  cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, softmax_scale)
+    rows = q.shape[0]
+    if out is None:
+        out = torch.empty(rows, heads * head_dim, device=dev, dtype=q.dtype)
+    ldo = _rows_view(out, rows, heads * head_dim, "out", q.dtype)
+    if lse is None and return_lse:
+        lse = torch.empty(heads, rows, device=dev, dtype=torch.float32)
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (heads, rows) or not lse.is_contiguous()):
+        raise RuntimeError(f"lse must be a contiguous float32 tensor [{heads}, {rows}]")
+    _count()
+    with torch.cuda.device(dev):
+        rc = _lib.load().sa3_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), *idx,
+                                             batch, max_seqlen_q, max_seqlen_k, rows, k.shape[0], heads, kv_heads,
+                                             head_dim, *ld, ldo, scale, _dt(q), _stream())
+    _lib.check(rc, "sa3_cross_attention")
+    return (out, lse) if return_lse else out
+
+
+def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                             lse: torch.Tensor, *, heads: int, kv_heads: Optional[int] = None, head_dim: int = 64,
+                             batch: int = 1, max_seqlen_q: int = 0, max_seqlen_k: int = 0, cu_seqlens_q=None,
+                             cu_seqlens_k=None, k_lens=None, key_mask=None, softmax_scale: Optional[float] = None,
+                             dq: Optional[torch.Tensor] = None, dk: Optional[torch.Tensor] = None,
+                             dv: Optional[torch.Tensor] = None):
+    """(dq, dk, dv) of sum(out * dout), with out and lse from `cross_attention(..., return_lse=True)` of the same
+    arguments. The same bits in every run. Scratch comes from torch's allocator on the current stream."""
+    dev = _one_device(dout, q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, dq, dk, dv)
+    kv_heads, ld, idx, batch, scale = _cross_args(q, k, v, heads, kv_heads, head_dim, batch, max_seqlen_q, max_seqlen_k,
+                                                  cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, softmax_scale)
+    rows, krows, wq, wk = q.shape[0], k.shape[0], heads * head_dim, kv_heads * head_dim
+    lddo = _rows_view(dout, rows, wq, "dout", q.dtype)
+    ldo = _rows_view(out, rows, wq, "out", q.dtype)
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (heads, rows) or not lse.is_contiguous():
+        raise RuntimeError(f"lse must be a contiguous float32 tensor [{heads}, {rows}]")
+    dq = torch.empty(rows, wq, device=dev, dtype=q.dtype) if dq is None else dq
+    dk = torch.empty(krows, wk, device=dev, dtype=q.dtype) if dk is None else dk
+    dv = torch.empty(krows, wk, device=dev, dtype=q.dtype) if dv is None else dv
+    ldd = (_rows_view(dq, rows, wq, "dq", q.dtype), _rows_view(dk, krows, wk, "dk", q.dtype),
+           _rows_view(dv, krows, wk, "dv", q.dtype))
+    lib = _lib.load()
+    _count()
+    with torch.cuda.device(dev):
+        n = ctypes.c_longlong(0)
+        _lib.check(lib.sa3_cross_attention_bwd_workspace(batch, max_seqlen_q, max_seqlen_k, rows, krows, heads, kv_heads,
+                                                         head_dim, ctypes.byref(n)),
+                   "sa3_cross_attention_bwd_workspace")
+        ws = torch.empty(n.value, device=dev, dtype=torch.uint8)
+        rc = lib.sa3_cross_attention_bwd(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                         lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *idx, batch,
+                                         max_seqlen_q, max_seqlen_k, rows, krows, heads, kv_heads, head_dim, lddo, *ld,
+                                         ldo, *ldd, scale, _dt(q), ws.data_ptr(), n.value, _stream())
+    _lib.check(rc, "sa3_cross_attention_bwd")
+    return dq, dk, dv
+
+
 # ---------------------------------------------------------------------- GPTQ
 def gptq_gemm(a: torch.Tensor, qw: torch.Tensor, sz: torch.Tensor, n: int, out: Optional[torch.Tensor] = None, *,
               group_size: int = 128, bias=None, kind: int = _lib.EPI_STORE, residual=None, gate=None,

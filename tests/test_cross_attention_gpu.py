@@ -1,0 +1,210 @@
+"""Attention to an encoder's states, forward and backward, against the formulas in 64 bits.
+
+Tolerances, element by element. u is half a step of the 16-bit type (2^-8 bf16, 2^-11 fp16).
+  out   every probability is rounded once before P V: u * (P |V|); the result once: u * |out|.
+  dv    P rounded once: u * (P^T |dO|); the result: u * |dv|.
+  dS    rounded once, u * |dS|; delta = rowsum(dO * out) comes from the rounded out, P * (u * sum |dO| |out|
+        + its own P-rounding error u * sum |dO| (P |V|)).
+        dq and dk: scale * (those, times |K| or |Q|), and the result's rounding.
+  32-bit work (scores, exponentials, sums: relative 2^-20 or so of P) is taken in by a factor 1.25, and fp16's
+  subnormal steps (2^-25 a probability or dS) by their sum against |V|, |dO|, |K|, |Q|.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+FLOOR = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
+
+
+def reference(q, k, v, dout, seqs, heads, kv_heads, d, scale):
+    """seqs: (query rows, visible key rows) of each sequence, as index tensors. (values, tolerances) of out, lse, dq,
+    dk, dv in 64 bits; rows of no sequence stay NaN."""
+    u, fl = U[q.dtype], FLOOR[q.dtype]
+    q, k, v = q.double(), k.double(), v.double()
+    dout = None if dout is None else dout.double()
+    nan = float("nan")
+    out, dq = torch.full_like(q, nan), torch.full_like(q, nan)
+    dk, dv = torch.full_like(k, nan), torch.full_like(v, nan)
+    lse = torch.full((heads, q.shape[0]), nan, dtype=torch.float64, device=q.device)
+    tol = [torch.zeros_like(x) for x in (out, dq, dk, dv)]
+    for rq, rk, all_k in seqs:
+        dk[all_k] = 0.0
+        dv[all_k] = 0.0
+        for h in range(heads):
+            cq = slice(h * d, (h + 1) * d)
+            hk = h // (heads // kv_heads)
+            ck = slice(hk * d, (hk + 1) * d)
+            if len(rk) == 0 or len(rq) == 0:
+                out[rq, cq] = 0.0
+                dq[rq, cq] = 0.0
+                lse[h, rq] = -math.inf
+                continue
+            Q, K, V = q[rq, cq], k[rk, ck], v[rk, ck]
+            S = scale * Q @ K.T
+            P = torch.softmax(S, -1)
+            O = P @ V
+            out[rq, cq] = O
+            lse[h, rq] = torch.logsumexp(S, -1)
+            tol[0][rq, cq] = u * (P @ V.abs() + O.abs()) + fl * (1 + V.abs().sum(0))
+            if dout is None:
+                continue
+            G = dout[rq, cq]
+            dP = G @ V.T
+            delta = (G * O).sum(-1, keepdim=True)
+            dS = P * (dP - delta)
+            eS = u * dS.abs() + P * u * (G.abs() * (O.abs() + P @ V.abs())).sum(-1, keepdim=True) + fl
+            dq[rq, cq] = scale * dS @ K
+            dk[rk, ck] += scale * dS.T @ Q
+            dv[rk, ck] += P.T @ G
+            tol[1][rq, cq] = scale * eS @ K.abs()
+            tol[2][rk, ck] += scale * eS.T @ Q.abs()
+            tol[3][rk, ck] += (u * P + fl).T @ G.abs()
+    for i, x in enumerate((dq, dk, dv)):
+        tol[i + 1] += u * torch.nan_to_num(x).abs() + fl
+    return (out, lse, dq, dk, dv), tol
+
+
+def check(got, want, tol, what):
+    seen = ~want.isnan()
+    err = (got.double() - want)[seen].abs()
+    lim = 1.25 * tol[seen] + 1e-6
+    assert torch.isfinite(got[seen]).all(), what
+    over = err > lim
+    assert not bool(over.any()), f"{what}: {int(over.sum())} of {over.numel()} off, worst {float((err / lim).max()):.3g}x"
+
+
+def check_lse(got, want):
+    """fp32 scores and sums: 2^-20 of the largest score or so, 1e-5 absolute at these sizes."""
+    seen = ~want.isnan()
+    g, w = got.double()[seen], want[seen]
+    assert torch.equal(g == -math.inf, w == -math.inf)
+    fin = w != -math.inf
+    assert float((g[fin] - w[fin]).abs().max() if fin.any() else 0.0) <= 1e-5 * max(1.0, float(w[fin].abs().max()) if fin.any() else 1.0)
+
+
+def run_case(cuda, batch, lq, lk, heads, kv_heads, d, dtype, mask="none", packed=False, poison=True, backward=True,
+             scale=None, seed=0, spread=1.0):
+    from sa3_b200 import _lib, ops
+
+    g = torch.Generator(device=cuda).manual_seed(seed + 31 * lq + 7 * lk + batch)
+    dt = DT[dtype]
+    lqs = [max(0, lq - (5 * b) % (lq + 1)) for b in range(batch)] if packed else [lq] * batch
+    lks = [max(0, lk - (7 * (batch - 1 - b)) % (lk + 1)) for b in range(batch)] if packed else [lk] * batch
+    pad = 3 if packed else 0  # rows behind the last sequence
+    nq, nk = sum(lqs) + pad, sum(lks) + pad
+    q = (torch.randn(nq, heads * d, generator=g, device=cuda) * spread).to(dt)
+    k = torch.randn(nk, kv_heads * d, generator=g, device=cuda).to(dt)
+    v = torch.randn(nk, kv_heads * d, generator=g, device=cuda).to(dt)
+    dout = torch.randn(nq, heads * d, generator=g, device=cuda).to(dt)
+    how = dict(heads=heads, kv_heads=kv_heads, head_dim=d, batch=batch, max_seqlen_q=lq, max_seqlen_k=lk,
+               softmax_scale=scale)
+    q0 = [sum(lqs[:b]) for b in range(batch + 1)]
+    k0 = [sum(lks[:b]) for b in range(batch + 1)]
+    if packed:
+        how["cu_seqlens_q"] = torch.tensor(q0, dtype=torch.int32, device=cuda)
+        how["cu_seqlens_k"] = torch.tensor(k0, dtype=torch.int32, device=cuda)
+    vis = torch.ones(nk, dtype=torch.bool, device=cuda)
+    vis[k0[-1]:] = False
+    if mask in ("lengths", "both"):
+        lens = [x - (3 * b) % (x + 1) for b, x in enumerate(lks)]
+        how["k_lens"] = torch.tensor(lens, dtype=torch.int32, device=cuda)
+        for b in range(batch):
+            vis[k0[b] + lens[b]:k0[b + 1]] = False
+    if mask in ("keys", "both"):
+        m = torch.rand(nk, generator=g, device=cuda) < 0.6
+        if batch > 1:
+            m[k0[1]:k0[2]] = False  # nothing left for sequence 1
+        how["key_mask"] = m
+        vis &= m
+    seqs = [(torch.arange(q0[b], q0[b + 1], device=cuda),
+             torch.arange(k0[b], k0[b + 1], device=cuda)[vis[k0[b]:k0[b + 1]]],
+             torch.arange(k0[b], k0[b + 1], device=cuda)) for b in range(batch)]
+    (ro, rl, rdq, rdk, rdv), tol = reference(q, k, v, dout if backward else None, seqs, heads, kv_heads, d,
+                                             scale or 1.0 / math.sqrt(d))
+    if poison:  # hidden keys and rows of no sequence may hold anything
+        k[~vis], v[~vis] = float("nan"), float("inf")
+        q[q0[-1]:], dout[q0[-1]:] = float("nan"), float("nan")
+    mark = 7.0
+    out = torch.full((nq, heads * d), mark, device=cuda, dtype=dt)
+    lse = torch.full((heads, nq), mark, device=cuda)
+    got = ops.cross_attention(q, k, v, out=out, lse=lse, return_lse=True, **how)
+    assert got[0] is out and got[1] is lse
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+    check(out, ro, tol[0], "out")
+    check_lse(lse, rl)
+    assert bool((out[q0[-1]:] == mark).all()) and bool((lse[:, q0[-1]:] == mark).all())
+    if not backward:
+        return
+    dq = torch.full_like(q, mark)
+    dk, dv = torch.full_like(k, mark), torch.full_like(v, mark)
+    ops.cross_attention_backward(dout, q, k, v, out, lse, dq=dq, dk=dk, dv=dv, **how)
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+    for name, a, w, e in (("dq", dq, rdq, tol[1]), ("dk", dk, rdk, tol[2]), ("dv", dv, rdv, tol[3])):
+        check(a, w, e, name)
+    assert bool((dq[q0[-1]:] == mark).all())
+    assert bool((dk[k0[-1]:] == mark).all()) and bool((dv[k0[-1]:] == mark).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("batch,lq,lk,heads,kv_heads", [
+    (1, 128, 64, 1, 1),
+    (1, 17, 1, 1, 1),
+    (2, 129, 65, 4, 2),
+    (1, 300, 257, 3, 3),
+    (1, 64, 1000, 8, 1),
+])
+def test_forward(cuda, dtype, d, batch, lq, lk, heads, kv_heads):
+    run_case(cuda, batch, lq, lk, heads, kv_heads, d, dtype, backward=False)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("batch,lq,lk,heads,kv_heads", [
+    (1, 1, 1, 1, 1),
+    (1, 1, 257, 20, 20),
+    (3, 1, 1000, 8, 1),
+    (2, 1, 333, 16, 1),
+    (5, 2, 40, 6, 2),
+    (1, 4, 5003, 8, 2),
+])
+def test_few_rows(cuda, dtype, d, batch, lq, lk, heads, kv_heads):
+    run_case(cuda, batch, lq, lk, heads, kv_heads, d, dtype, backward=False)
+
+
+@pytest.mark.parametrize("mask", ["lengths", "keys", "both"])
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,lk", [(1, 100), (3, 1), (150, 70), (40, 200)])
+def test_masks_forward(cuda, mask, packed, d, lq, lk):
+    run_case(cuda, 4, lq, lk, 4, 2, d, "bf16", mask=mask, packed=packed, backward=False)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("batch,lq,lk,heads,kv_heads", [
+    (1, 64, 128, 1, 1),
+    (1, 128, 64, 1, 1),
+    (1, 1, 1, 1, 1),
+    (2, 77, 33, 8, 2),
+    (1, 300, 257, 3, 3),
+    (2, 1000, 130, 2, 1),
+    (1, 33, 700, 4, 4),
+])
+def test_backward(cuda, dtype, d, batch, lq, lk, heads, kv_heads):
+    run_case(cuda, batch, lq, lk, heads, kv_heads, d, dtype)
+
+
+@pytest.mark.parametrize("mask", ["none", "lengths", "keys", "both"])
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,lk", [(2, 5), (150, 70), (70, 300)])
+def test_masks_backward(cuda, mask, packed, d, lq, lk):
+    run_case(cuda, 4, lq, lk, 4, 2, d, "bf16", mask=mask, packed=packed)
