@@ -295,18 +295,22 @@ int sa3_rotary(const void* q, void* q_out, const void* k, void* k_out, int dtype
  * lse (fp32 [heads, total_q], or NULL): natural log of the sum of the exponentials.
  * softmax_scale > 0. Zero lengths and batches are valid.
  * At most 16 query rows a key head (max_seqlen_q * heads / kv_heads, e.g. one decoded token) take a kernel that
- * splits the keys over a cluster; the rest take a tcgen05 kernel.
+ * splits the keys over a cluster; the rest take a tcgen05 kernel. With few query rows and long keys either splits the
+ * keys over CTAs that a second launch joins (in a fixed order). That needs a workspace: 16-byte aligned device memory
+ * of the bytes that sa3_cross_attention_workspace reports for the current device (0: NULL will do), used by this call
+ * alone until it has run.
  *
  * sa3_cross_attention_bwd: dq, dk, dv of the sum of out * dout, from the forward's out and lse. dk and dv are summed
- * over the query heads of a group, in a fixed order (the same bits in every run). workspace: 16-byte aligned device
- * memory of at least the bytes that sa3_cross_attention_bwd_workspace reports for the current device, used by this
- * call alone until it has run.
+ * over the query heads of a group, in a fixed order (the same bits in every run). Its workspace likewise, from
+ * sa3_cross_attention_bwd_workspace.
  */
 int sa3_cross_attention(const void* q, const void* k, const void* v, void* out, float* lse, const int* cu_seqlens_q,
                         const int* cu_seqlens_k, const int* k_lens, const unsigned char* key_mask, int batch,
                         int max_seqlen_q, int max_seqlen_k, int total_q, int total_k, int heads, int kv_heads,
                         int head_dim, long long ldq, long long ldk, long long ldv, long long ldo, float softmax_scale,
-                        int dtype, void* stream);
+                        int dtype, void* workspace, long long workspace_bytes, void* stream);
+int sa3_cross_attention_workspace(int batch, int max_seqlen_q, int max_seqlen_k, int total_q, int heads, int kv_heads,
+                                  int head_dim, long long* bytes);
 int sa3_cross_attention_bwd_workspace(int batch, int max_seqlen_q, int max_seqlen_k, int total_q, int total_k,
                                       int heads, int kv_heads, int head_dim, long long* bytes);
 int sa3_cross_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,

@@ -15,7 +15,7 @@
 // type of the matrix instructions.
 #include "attn_tile.cuh"
 #include "common.cuh"
-#include "cross_attention.h"
+#include "cross_attention.cuh"
 #include "host_util.h"
 
 namespace sa3 {
@@ -27,33 +27,6 @@ constexpr float XA_LOG2E = 1.4426950408889634f;
 constexpr float XA_RESCALE_LOG2 = 8.f;  // move the reference maximum only when it grows by more than this
 constexpr int XA_SUB_M = XA_BM * 128;   // bytes of a 64-column sub-tile of the wide side
 constexpr int XA_SUB_N = XA_BN * 128;   // ... of the walked side
-
-// One sequence: row offsets and lengths, clamped to the buffers so that no offset reaches outside them.
-struct XSeq {
-  int qs, lq, ks, lk, seen;  // seen: keys before the sequence's key length (a key mask may hide more)
-};
-
-__device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
-
-__device__ __forceinline__ XSeq make_seq(const XParams& p, int b) {
-  XSeq s;
-  if (p.cu_q) {
-    s.qs = clampi(__ldg(p.cu_q + b), 0, p.total_q);
-    s.lq = clampi(__ldg(p.cu_q + b + 1) - s.qs, 0, min(p.total_q - s.qs, p.Lq));
-  } else {
-    s.qs = b * p.Lq;
-    s.lq = p.Lq;
-  }
-  if (p.cu_k) {
-    s.ks = clampi(__ldg(p.cu_k + b), 0, p.total_k);
-    s.lk = clampi(__ldg(p.cu_k + b + 1) - s.ks, 0, min(p.total_k - s.ks, p.Lk));
-  } else {
-    s.ks = b * p.Lk;
-    s.lk = p.Lk;
-  }
-  s.seen = p.k_lens ? clampi(__ldg(p.k_lens + b), 0, s.lk) : s.lk;
-  return s;
-}
 
 // Bit i: key j0 + i of the sequence is visible (i < 64). All lanes of a warp call it and get the same word.
 __device__ __forceinline__ uint64_t visible64(const XParams& p, const XSeq& s, int j0, int lane) {
@@ -116,6 +89,43 @@ template <int D>
 __device__ __forceinline__ void zero_row16(void* dst) {
 #pragma unroll
   for (int e = 0; e < D / 8; ++e) reinterpret_cast<uint4*>(dst)[e] = make_uint4(0, 0, 0, 0);
+}
+
+// the same in fp32
+template <int D>
+__device__ __forceinline__ void store_row32(uint32_t t_o, float f, bool store, float* dst) {
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld32_async(t_o + 32 * c, o);
+    tmem_wait_ld();
+    if (store)
+#pragma unroll
+      for (int e = 0; e < 32; e += 4)
+        *reinterpret_cast<float4*>(dst + 32 * c + e) =
+            make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 2]) * f,
+                        __uint_as_float(o[e + 3]) * f);
+  }
+}
+
+// Work item of the forward: query tile (fastest), head, part of the keys, sequence. Keys j0 .. of the part in T tiles.
+struct XItem {
+  XSeq s;
+  int tile, h, part, j0, T;
+};
+__device__ __forceinline__ XItem make_item(const XParams& p, int item, int qtiles) {
+  XItem it;
+  it.tile = item % qtiles;
+  int rest = item / qtiles;
+  it.h = rest % p.heads;
+  rest /= p.heads;
+  it.part = rest % p.parts;
+  it.s = make_seq(p, rest / p.parts);
+  const int all = it.tile * XA_BM < it.s.lq ? (it.s.seen + XA_BN - 1) / XA_BN : 0;
+  const int t0 = (int)((long long)all * it.part / p.parts);
+  it.T = (int)((long long)all * (it.part + 1) / p.parts) - t0;
+  it.j0 = t0 * XA_BN;
+  return it;
 }
 
 constexpr int XA_THREADS = 192;  // warps 0..3 softmax (TMEM lane quarters), 4 TMA, 5 MMA
@@ -188,10 +198,9 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
       int g = 0, qc = 0;
       bool ok = true, v_out = true;  // v_out: V of the last counted tile was issued
       for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
-        const int tile = item % qtiles, rest = item / qtiles;
-        const int h = rest % p.heads, b = rest / p.heads;
-        const XSeq s = make_seq(p, b);
-        const int T = tile * XA_BM < s.lq ? (s.seen + XA_BN - 1) / XA_BN : 0;
+        const XItem it = make_item(p, item, qtiles);
+        const XSeq& s = it.s;
+        const int tile = it.tile, h = it.h, T = it.T;
         if (T == 0) continue;
         const int cq = h * D, ck = (h / p.group) * D;
         const int qs = qc % C::QS;
@@ -208,7 +217,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
           }
           mbar_arrive_expect_tx(&k_full[ks], C::T_BYTES);
           for (int c = 0; c < C::SUBS; ++c)
-            tma_load_2d(sK(ks) + c * XA_SUB_N, &tmK, &k_full[ks], ck + 64 * c, s.ks + t * XA_BN);
+            tma_load_2d(sK(ks) + c * XA_SUB_N, &tmK, &k_full[ks], ck + 64 * c, s.ks + it.j0 + t * XA_BN);
           if (g >= C::VS && !mbar_wait(&v_empty[ks], ((g / C::VS) - 1) & 1, abort_flag, 102)) {
             g++;
             ok = v_out = false;
@@ -216,7 +225,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
           }
           mbar_arrive_expect_tx(&v_full[ks], C::T_BYTES);
           for (int c = 0; c < C::SUBS; ++c)
-            tma_load_2d(sV(ks) + c * XA_SUB_N, &tmV, &v_full[ks], ck + 64 * c, s.ks + t * XA_BN);
+            tma_load_2d(sV(ks) + c * XA_SUB_N, &tmV, &v_full[ks], ck + 64 * c, s.ks + it.j0 + t * XA_BN);
         }
       }
       if (*abort_flag) {
@@ -241,17 +250,16 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     int g = 0, qc = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
-      const int tile = item % qtiles, rest = item / qtiles;
-      const int b = rest / p.heads;
-      const XSeq s = make_seq(p, b);
-      const int T = tile * XA_BM < s.lq ? (s.seen + XA_BN - 1) / XA_BN : 0;
+      const XItem it = make_item(p, item, qtiles);
+      const XSeq& s = it.s;
+      const int T = it.T;
       if (T == 0) continue;
       ok = warp_wait(&q_full[qc % C::QS], (qc / C::QS) & 1, abort_flag, 104);
       auto scores = [&](int t) {
         const int n = g + (t > 0 ? 1 : 0), ks = n % C::KS;
         if (!warp_wait(&k_full[ks], (n / C::KS) & 1, abort_flag, 105)) return false;
         tc_fence_after();
-        const int cols = (min(XA_BN, s.seen - t * XA_BN) + 15) & ~15;
+        const int cols = (min(XA_BN, s.seen - it.j0 - t * XA_BN) + 15) & ~15;
         const uint32_t idesc = make_idesc(128, cols, fmt, fmt, 0, 0);
         const uint32_t qlo = k_lo + off16(sQ(qc % C::QS)), klo = k_lo + off16(sK(ks));
         const uint32_t t_s = tmem + 64 * (n & 1);
@@ -271,8 +279,8 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
           break;
         }
         const int vs = g % C::VS;
-        const int keys = min(XA_BN, s.seen - t * XA_BN), steps = (keys + 15) >> 4;
-        const uint64_t vis = visible64(p, s, t * XA_BN, lane);
+        const int keys = min(XA_BN, s.seen - it.j0 - t * XA_BN), steps = (keys + 15) >> 4;
+        const uint64_t vis = visible64(p, s, it.j0 + t * XA_BN, lane);
         ok = warp_wait(&v_full[vs], (g / C::VS) & 1, abort_flag, 106);
         if (!ok) break;
         const uint64_t all = steps == 4 ? ~0ull : (1ull << (16 * steps)) - 1;
@@ -300,19 +308,19 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
     int g = 0;
     for (int item = blockIdx.x; item < num_items; item += gridDim.x) {
-      const int tile = item % qtiles, rest = item / qtiles;
-      const int h = rest % p.heads, b = rest / p.heads;
-      const XSeq s = make_seq(p, b);
-      if (tile * XA_BM >= s.lq) continue;
-      const int T = (s.seen + XA_BN - 1) / XA_BN;
-      const int i = tile * XA_BM + r;
+      const XItem it = make_item(p, item, qtiles);
+      const XSeq& s = it.s;
+      const int h = it.h, T = it.T;
+      if (it.tile * XA_BM >= s.lq) continue;
+      const int i = it.tile * XA_BM + r;
       const bool row_ok = i < s.lq;
       const long long row = s.qs + i;
       uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + h * D;
-      float* lse = p.lse ? p.lse + (long long)h * p.total_q + row : nullptr;
+      const long long at = ((long long)it.part * p.heads + h) * p.total_q + row;  // one part: of lse itself
+      float* lse = p.parts > 1 ? p.part_lse + at : p.lse ? p.lse + at : nullptr;
       if (T == 0) {
         if (row_ok) {
-          zero_row16<D>(dst);
+          if (p.parts == 1) zero_row16<D>(dst);  // else a part of weight zero, whose output is not read
           if (lse) *lse = NEG_INF;
         }
         continue;
@@ -320,7 +328,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
       bool bad = false;
       float m = NEG_INF, l = 0.f;
       for (int t = 0; t < T; ++t, ++g) {
-        const uint64_t vis = visible64(p, s, t * XA_BN, lane);
+        const uint64_t vis = visible64(p, s, it.j0 + t * XA_BN, lane);
         const uint32_t t_s = tmem + lane_off + 64 * (g & 1);
         if (!mbar_wait(&s_full[g & 1], (g >> 1) & 1, abort_flag, 110)) bad = true;
         tc_fence_after();
@@ -379,7 +387,11 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
       if (!mbar_wait(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 112)) bad = true;
       tc_fence_after();
       const bool store = row_ok && !bad && !*abort_flag;
-      store_row16<D>(t_o, l > 0.f ? 1.f / l : 0.f, p.f16, store, dst);
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      if (p.parts > 1)
+        store_row32<D>(t_o, inv, store, p.part_o + at * D);
+      else
+        store_row16<D>(t_o, inv, p.f16, store, dst);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_empty);
@@ -901,23 +913,11 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
     } else {
       const long long width = (long long)p.kv_heads * D;
       float* dst = gr.partial + ((long long)(part * 2 + grp) * p.total_k + row) * width + hk * D;
+      if (T > 0)
+        store_row32<D>(t_g, f, store, dst);
+      else if (store)
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        if (T > 0) {
-          tmem_ld32_async(t_g + 32 * c, o);
-          tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
-        }
-        if (store)
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(dst + 32 * c + e) =
-                make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 2]) * f,
-                            __uint_as_float(o[e + 3]) * f);
-      }
+        for (int e = 0; e < D; e += 4) *reinterpret_cast<float4*>(dst + e) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
   }
   tc_fence_before();
@@ -925,19 +925,16 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
-// dK and dV from the parts of the walk, in part order. Rows that belong to no sequence are left alone: a row is
-// written when some sequence of the batch covers it (uniform batches cover every row).
+// dK and dV from the parts of the walk, in part order: grid (rows of a sequence x vectors, sequence).
 __global__ void __launch_bounds__(256) cross_join_kernel(const XParams p, const XGrad gr, int splits, int width) {
   grid_dep_wait();
+  const XSeq s = make_seq(p, blockIdx.y);
   const int vecs = width / 4;
-  const long long n = (long long)p.total_k * vecs;
-  const long long first = p.cu_k ? clampi(__ldg(p.cu_k), 0, p.total_k) : 0;
-  const long long last = p.cu_k ? clampi(__ldg(p.cu_k + p.batch), 0, p.total_k) : p.total_k;
+  const long long n = (long long)s.lk * vecs;
   for (long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x; at < 2 * n;
        at += (long long)gridDim.x * blockDim.x) {
     const int w = at >= n;
-    const long long i = at - w * n, row = i / vecs, c = (i - row * vecs) * 4;
-    if (row < first || row >= last) continue;
+    const long long i = at - w * n, row = s.ks + i / vecs, c = (i % vecs) * 4;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int sp = 0; sp < splits; ++sp) {
       const float4 v = *reinterpret_cast<const float4*>(gr.partial + ((long long)(sp * 2 + w) * p.total_k + row) * width + c);
@@ -951,15 +948,41 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const XParams p, const 
   }
 }
 
-// ------------------------------------------------------------------------------------------------ host
-static int sm_count() {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 0;
-  return sms;
+// The forward's output from the parts of the keys: out = sum_s exp(lse_s - lse) out_s, lse = log sum_s exp(lse_s).
+// grid (rows of a sequence x heads x vectors, sequence).
+template <int D>
+__global__ void __launch_bounds__(256) cross_merge_kernel(const XParams p) {
+  grid_dep_wait();
+  const XSeq s = make_seq(p, blockIdx.y);
+  const long long n = (long long)s.lq * p.heads * (D / 4);
+  for (long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x; at < n; at += (long long)gridDim.x * blockDim.x) {
+    const int d = 4 * (int)(at % (D / 4)), h = (int)(at / (D / 4) % p.heads);
+    const long long row = s.qs + at / (D / 4) / p.heads;
+    const long long one = (long long)p.heads * p.total_q, src = (long long)h * p.total_q + row;
+    float top = -INFINITY;
+    for (int sp = 0; sp < p.parts; ++sp) top = fmaxf(top, p.part_lse[sp * one + src]);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    if (top != -INFINITY)
+      for (int sp = 0; sp < p.parts; ++sp) {
+        const float e = p.part_lse[sp * one + src];
+        if (e == -INFINITY) continue;
+        const float f = fast_exp2((e - top) * XA_LOG2E);
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + (sp * one + src) * D + d);
+        l += f;
+        a.x = fmaf(v.x, f, a.x);
+        a.y = fmaf(v.y, f, a.y);
+        a.z = fmaf(v.z, f, a.z);
+        a.w = fmaf(v.w, f, a.w);
+      }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + h * D + d;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_2(a.x * inv, a.y * inv, p.f16), pack_2(a.z * inv, a.w * inv, p.f16));
+    if (d == 0 && p.lse) p.lse[src] = l > 0.f ? top + __log2f(l) * 0.6931471805599453f : -INFINITY;
+  }
 }
 
+// ------------------------------------------------------------------------------------------------ host
 // Parts of the dK / dV walk: the number that ends soonest when every wave of CTAs costs its longest walk plus the
 // set-up, epilogue and joining of a part (about 6 tiles). One part writes its result at once.
 static int dkv_splits(long long ctas, long long tiles, int sms) {
@@ -996,7 +1019,7 @@ static int check_common(const void* q, const void* k, const void* v, const void*
   // grid and item counts stay in 32 bits
   const long long items = ((long long)max_q / XA_BM + 1) * heads * (batch > 0 ? batch : 1);
   const long long kitems = ((long long)max_k / XA_BM + 1) * kv_heads * (batch > 0 ? batch : 1);
-  if (heads > 65535 || items > (1LL << 30) || kitems > (1LL << 25)) return SA3_ERR_UNSUPPORTED;
+  if (heads > 65535 || batch > 65535 || items > (1LL << 30) || kitems > (1LL << 25)) return SA3_ERR_UNSUPPORTED;
   return SA3_OK;
 }
 
@@ -1022,6 +1045,7 @@ static XParams make_params(void* out, float* lse, const int* cu_q, const int* cu
   p.out = out;
   p.ldo = ldo;
   p.lse = lse;
+  p.parts = 1;
   return p;
 }
 
@@ -1033,19 +1057,23 @@ static int token_map(CUtensorMap* m, const void* x, const void* other, int f16, 
   return make_tmap_2d(m, rows > 0 ? x : other, dt, 2, width, rows > 0 ? rows : 1, ld, 64, box);
 }
 
+// Grid of the joining kernels: enough blocks of 256 threads for `n` elements of a sequence, about 8 an SM in all.
+static dim3 rows_grid(long long n, int batch, int sms) {
+  const long long need = (n + 255) / 256, most = (8LL * sms + batch - 1) / batch;
+  return dim3((unsigned)(need < most ? need : most), (unsigned)batch);
+}
+
 template <int D>
 static int launch_fwd(const XParams& p, const void* q, const void* k, const void* v, long long ldq, long long ldk,
-                      long long ldv, cudaStream_t st) {
+                      long long ldv, int sms, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
   int rc;
   const long long wq = (long long)p.heads * D, wk = (long long)p.kv_heads * D;
   if ((rc = token_map(&mq, q, q, p.f16, wq, p.total_q, ldq, XA_BM))) return rc;
   if ((rc = token_map(&mk, k, q, p.f16, wk, p.total_k, ldk, XA_BN))) return rc;
   if ((rc = token_map(&mv, v, q, p.f16, wk, p.total_k, ldv, XA_BN))) return rc;
-  const int sms = sm_count();
-  if (sms <= 0) return SA3_ERR_LAUNCH;
   const int qtiles = (p.Lq + XA_BM - 1) / XA_BM;
-  const int items = qtiles * p.heads * p.batch;
+  const int items = qtiles * p.heads * p.batch * p.parts;
   if ((rc = ensure_smem(cross_fwd_kernel<D>, XFwd<D>::SMEM))) return rc;
   launch_ex(cross_fwd_kernel<D>, dim3(items < 2 * sms ? items : 2 * sms), dim3(XA_THREADS), XFwd<D>::SMEM, st, 1, mq,
             mk, mv, p, items, qtiles);
@@ -1082,9 +1110,7 @@ static int launch_bwd(const XParams& p, const XGrad& g, const void* q, const voi
               XDkv<D>::SMEM, st, 1, q64, do64, k128, v128, p, g, ktiles, splits);
     if ((rc = launch_status())) return rc;
     if (splits > 1) {
-      const long long vecs = 2LL * p.total_k * p.kv_heads * D / 4;
-      const long long blocks = (vecs + 255) / 256;
-      launch_ex(cross_join_kernel, dim3((unsigned)(blocks < 8LL * sms ? blocks : 8LL * sms)), dim3(256), 0, st, 1, p, g,
+      launch_ex(cross_join_kernel, rows_grid(2LL * p.Lk * p.kv_heads * D / 4, p.batch, sms), dim3(256), 0, st, 1, p, g,
                 splits, p.kv_heads * D);
       if ((rc = launch_status())) return rc;
     }
@@ -1092,8 +1118,24 @@ static int launch_bwd(const XParams& p, const XGrad& g, const void* q, const voi
   return SA3_OK;
 }
 
+// the parts' lse first, their outputs behind it at a 16-byte boundary
+static long long fwd_bytes(int parts, int heads, int total_q, int head_dim) {
+  const long long rows = (long long)parts * heads * total_q;
+  return 4 * (((rows + 3) & ~3LL) + rows * head_dim);
+}
+
 // delta first, the parts of dK and dV behind it at a 16-byte boundary
 static long long delta_bytes(int heads, int total_q) { return (((long long)heads * total_q * 4) + 15) & ~15LL; }
+
+// Parts of the keys in the forward (one CTA each, joined by a second launch): when the query tiles alone leave half of
+// the CTA slots empty and every part still has 8 key tiles or more.
+static int fwd_parts(int batch, int max_q, int max_k, int heads, int kv_heads, int sms) {
+  if (batch <= 0 || max_q <= 0) return 1;
+  if ((long long)max_q * (heads / kv_heads) <= XT_MAX_ROWS) return cross_token_parts(batch, kv_heads, max_k, sms);
+  const long long items = (long long)((max_q + XA_BM - 1) / XA_BM) * heads * batch;
+  const long long fill = 2LL * sms / items, most = max_k / (8 * XA_BN), n = fill < most ? fill : most;
+  return n >= 2 ? (int)n : 1;
+}
 
 static int bwd_splits(int batch, int max_q, int max_k, int heads, int kv_heads, int sms) {
   const long long ctas = (long long)((max_k + XA_BM - 1) / XA_BM) * kv_heads * batch;
@@ -1110,20 +1152,47 @@ extern "C" int sa3_cross_attention(const void* q, const void* k, const void* v, 
                                    const unsigned char* key_mask, int batch, int max_seqlen_q, int max_seqlen_k,
                                    int total_q, int total_k, int heads, int kv_heads, int head_dim, long long ldq,
                                    long long ldk, long long ldv, long long ldo, float softmax_scale, int dtype,
-                                   void* stream) {
+                                   void* workspace, long long workspace_bytes, void* stream) {
   int rc = check_common(q, k, v, out, cu_seqlens_q, cu_seqlens_k, batch, max_seqlen_q, max_seqlen_k, total_q, total_k,
                         heads, kv_heads, head_dim, ldq, ldk, ldv, ldo, softmax_scale, dtype);
   if (rc) return rc;
   if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(k_lens)) & 3) return SA3_ERR_ALIGN;
   if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return SA3_OK;
-  const XParams p = make_params(out, lse, cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, batch, max_seqlen_q,
-                                max_seqlen_k, total_q, total_k, heads, kv_heads, ldo, softmax_scale, dtype);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int sms = sm_count();
   if (sms <= 0) return SA3_ERR_LAUNCH;
+  XParams p = make_params(out, lse, cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, batch, max_seqlen_q, max_seqlen_k,
+                          total_q, total_k, heads, kv_heads, ldo, softmax_scale, dtype);
+  p.parts = fwd_parts(batch, max_seqlen_q, max_seqlen_k, heads, kv_heads, sms);
+  if (p.parts > 1) {
+    if (!workspace || workspace_bytes < fwd_bytes(p.parts, heads, total_q, head_dim)) return SA3_ERR_ARG;
+    if (!aligned16(workspace)) return SA3_ERR_ALIGN;
+    p.part_lse = static_cast<float*>(workspace);
+    p.part_o = p.part_lse + (((long long)p.parts * heads * total_q + 3) & ~3LL);
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if ((long long)max_seqlen_q * p.group <= XT_MAX_ROWS)
-    return cross_token(p, q, k, v, ldq, ldk, ldv, head_dim, sms, st);
-  return head_dim == 64 ? launch_fwd<64>(p, q, k, v, ldq, ldk, ldv, st) : launch_fwd<128>(p, q, k, v, ldq, ldk, ldv, st);
+    rc = cross_token(p, q, k, v, ldq, ldk, ldv, head_dim, sms, st);
+  else if (head_dim == 64)
+    rc = launch_fwd<64>(p, q, k, v, ldq, ldk, ldv, sms, st);
+  else
+    rc = launch_fwd<128>(p, q, k, v, ldq, ldk, ldv, sms, st);
+  if (rc || p.parts == 1) return rc;
+  const dim3 grid = rows_grid((long long)max_seqlen_q * heads * head_dim / 4, batch, sms);
+  launch_ex(head_dim == 64 ? cross_merge_kernel<64> : cross_merge_kernel<128>, grid, dim3(256), 0, st, 1, p);
+  return launch_status();
+}
+
+extern "C" int sa3_cross_attention_workspace(int batch, int max_seqlen_q, int max_seqlen_k, int total_q, int heads,
+                                             int kv_heads, int head_dim, long long* bytes) {
+  if (!bytes || batch < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || total_q < 0 || heads <= 0 || kv_heads <= 0 ||
+      heads % kv_heads != 0)
+    return SA3_ERR_ARG;
+  if (head_dim != 64 && head_dim != 128) return SA3_ERR_UNSUPPORTED;
+  const int sms = sm_count();
+  if (sms <= 0) return SA3_ERR_LAUNCH;
+  const int n = fwd_parts(batch, max_seqlen_q, max_seqlen_k, heads, kv_heads, sms);
+  *bytes = n > 1 ? fwd_bytes(n, heads, total_q, head_dim) : 0;
+  return SA3_OK;
 }
 
 extern "C" int sa3_cross_attention_bwd_workspace(int batch, int max_seqlen_q, int max_seqlen_k, int total_q, int total_k,

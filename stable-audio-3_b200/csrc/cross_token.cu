@@ -1,32 +1,37 @@
 // Attention of a few query rows (one decoded token of every sequence, times the query heads that share a key head)
 // to an encoder's states: out = softmax(scale * q K^T) V over the visible keys.
 //
-// Bound by reading K and V once. All query rows of a key head (at most 16: query tokens x heads of the group) form
-// one 16-row A operand, so K and V of the head are read once for the whole group. The keys are split over the warps
-// of a cluster of CTAs, 16 keys a step; K and V go from global memory straight into the B fragments of the warp
-// matrix instructions (the tensor cores' tcgen05 form would leave 112 of its 128 rows empty, and it needs the tiles
-// in shared memory first), 16 bytes a lane:
-//   K: lane (g, t) = (lane / 4, lane % 4) reads columns 32 c + 8 t .. + 7 of key g. They serve as the k indices
-//      {2t, 2t+1, 2t+8, 2t+9} of two steps; the sum over a head's columns may run in any order, so Q's fragments are
-//      read in the same order.
-//   V: lane (g, t) reads columns 64 c + 8 g .. + 7 of keys 2t, 2t+1, 2t+8, 2t+9; column e of the eight belongs to
-//      the n-tile e, whose column g is thus d = 64 c + 8 g + e.
-// Hidden keys are not read: their registers are zero and their scores -inf.
-// Each warp keeps its own running maximum, sum and fp32 accumulators; the warps of a CTA join through shared memory
-// and the CTAs of the cluster through distributed shared memory, in a fixed order: one launch, no workspace.
+// Bound by reading K and V once. All query rows of a key head (at most 16: query tokens x heads of the group) are the
+// N side of warp matrix instructions m16n8k16, so K and V of the head are read once for the whole group and no row of
+// the instruction is wasted up to 8 (tcgen05 would leave 112 of its 128 rows empty):
+//   S^T (16 keys x rows) = K Q^T          A = K by ldmatrix, B = Q^T, kept in registers
+//   O^T (16 columns x rows) += V^T P^T    A = V^T by ldmatrix.trans, B = P^T: the S^T fragment, transposed by movmatrix
+// The keys are split over the warps of a cluster of CTAs, 16 keys a step. Each warp copies its steps asynchronously
+// into a ring of its own in shared memory (16-byte chunk c of key j at chunk c ^ (j & 7): no bank conflicts on either
+// side), several steps ahead, so the bytes in flight take no registers and no warp waits for another. Hidden keys are
+// not read: their rows are filled with zeros and their scores are -inf.
+// The reference maximum of a row moves only when a score exceeds it by more than 2^8; one vote a step finds out, and
+// the usual step has no reduction over lanes. The warps of a CTA join through shared memory and the CTAs of the
+// cluster through distributed shared memory, in a fixed order: one launch, no workspace.
 #include <cooperative_groups.h>
 
 #include "attn_tile.cuh"
 #include "common.cuh"
-#include "cross_attention.h"
+#include "cross_attention.cuh"
 #include "host_util.h"
 
 namespace sa3 {
 namespace cg = cooperative_groups;
 
-constexpr int XT_WARPS = 8;
+constexpr int XT_WARPS = 4;
 constexpr int XT_THREADS = XT_WARPS * 32;
-constexpr int XT_KEYS = 16;  // keys of a step of a warp
+constexpr int XT_KEYS = 16;          // keys of a step of a warp
+constexpr int XT_MAX_CLUSTER = 8;
+constexpr int XT_PART_KEYS = 512;    // least keys of a part of the split without clusters: 8 steps of a warp
+constexpr float XT_RESCALE_LOG2 = 8.f;
+// Steps in flight: 96 KB a CTA at either width, two CTAs an SM.
+template <int D>
+constexpr int XT_STAGES = D == 64 ? 6 : 3;
 
 struct XTokenParams {
   XParams p;
@@ -34,202 +39,222 @@ struct XTokenParams {
   long long ldq, ldk, ldv;
 };
 
-__device__ __forceinline__ int clamp_to(int v, int lo, int hi) { return min(max(v, lo), hi); }
-
 template <bool F16>
-__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                          uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (F16)
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// 16 bytes from global to shared memory, or zeros
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
 
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-
-// R16: 9..16 query rows, else at most 8 (the upper half of every fragment is zero and is not kept).
-template <int D, bool F16, bool R16>
-__global__ void __launch_bounds__(XT_THREADS, R16 ? 1 : 2) cross_token_kernel(const XTokenParams a, int csize) {
-  constexpr int ROWS = R16 ? 16 : 8;
-  constexpr int KC = D / 32, VC = D / 64;  // 16-byte column chunks of a lane
-  extern __shared__ float sh[];            // [warps][ROWS][D] partial outputs, then [warps][ROWS] maxima and sums
+// NT: tiles of 8 query rows (1 or 2).
+template <int D, bool F16, int NT>
+__global__ void __launch_bounds__(XT_THREADS, 2) cross_token_kernel(const XTokenParams a, int csize) {
+  constexpr int ROWS = 8 * NT;
+  constexpr int CH = D / 8;                 // 16-byte chunks of a key
+  constexpr int KPI = 32 / CH;              // keys that one copy instruction of a warp covers
+  constexpr int ST = XT_STAGES<D>, HALF = XT_KEYS * D * 2, STEP = 2 * HALF;  // K, then V, of a step
+  // the warps' rings; afterwards [warps][ROWS][D] partial outputs and their [warps][ROWS] maxima and sums
+  extern __shared__ __align__(128) float sh[];
   float* sh_m = sh + XT_WARPS * ROWS * D;
   float* sh_l = sh_m + XT_WARPS * ROWS;
   const XParams& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int rank = blockIdx.x % csize, unit = blockIdx.x / csize;
+  const int rank = blockIdx.x % csize, part = blockIdx.x / csize % p.parts, unit = blockIdx.x / csize / p.parts;
   const int hk = unit % p.kv_heads, b = unit / p.kv_heads;
   grid_dep_wait();
-  int qs = b * p.Lq, lq = p.Lq, ks = b * p.Lk, lk = p.Lk;
-  if (p.cu_q) {
-    qs = clamp_to(__ldg(p.cu_q + b), 0, p.total_q);
-    lq = clamp_to(__ldg(p.cu_q + b + 1) - qs, 0, min(p.total_q - qs, p.Lq));
-  }
-  if (p.cu_k) {
-    ks = clamp_to(__ldg(p.cu_k + b), 0, p.total_k);
-    lk = clamp_to(__ldg(p.cu_k + b + 1) - ks, 0, min(p.total_k - ks, p.Lk));
-  }
-  const int seen = p.k_lens ? clamp_to(__ldg(p.k_lens + b), 0, lk) : lk;
+  const XSeq sq = make_seq(p, b);
+  const int qs = sq.qs, lq = sq.lq, ks = sq.ks, seen = sq.seen;
   const int rows = lq * p.group;  // row m: token m / group, head hk * group + m % group
 
-  // Q fragments in the column order of the K loads
-  uint32_t qa[KC][2][2], qb[KC][2][2];  // [chunk][step][a0, a2] of row g, [a1, a3] of row g + 8
-  auto q_row = [&](int m) {
-    return reinterpret_cast<const uint16_t*>(a.q) + (long long)(qs + m / p.group) * a.ldq +
-           (hk * p.group + m % p.group) * D;
+  const int first = ((part * csize + rank) * XT_WARPS + warp) * XT_KEYS, stride = p.parts * csize * XT_WARPS * XT_KEYS;
+  const int steps = first < seen ? (seen - first - 1) / stride + 1 : 0;
+  const uint32_t ring = smem_u32(sh) + warp * ST * STEP;
+  // copies: lane -> key lane / CH of a group of KPI keys, chunk lane % CH
+  const int ck = lane / CH, cc = lane % CH;
+  const long long row0 = (long long)ks + first + ck;
+  const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.k) + row0 * a.ldk + hk * D + 8 * cc;
+  const uint16_t* vp = reinterpret_cast<const uint16_t*>(a.v) + row0 * a.ldv + hk * D + 8 * cc;
+  const long long k_step = (long long)stride * a.ldk, v_step = (long long)stride * a.ldv;
+  // issue the copies of step c, at which kp and vp stand, into its slot; the mask of its visible keys
+  auto fetch = [&](int c) -> uint32_t {
+    uint32_t vis = 0;
+    if (c < steps) {
+      const int j0 = first + c * stride;
+      vis = seen - j0 >= XT_KEYS ? 0xffffu : (1u << (seen - j0)) - 1u;
+      if (p.key_mask) {
+        const bool on = lane < XT_KEYS && ((vis >> lane) & 1u) && __ldg(p.key_mask + (long long)ks + j0 + lane) != 0;
+        vis = __ballot_sync(0xffffffffu, on);
+      }
+      const uint32_t slot = ring + (c % ST) * STEP;
+#pragma unroll
+      for (int i = 0; i < XT_KEYS / KPI; ++i) {
+        const int j = i * KPI + ck;
+        const bool on = (vis >> j) & 1u;
+        const uint32_t dst = slot + j * (D * 2) + ((cc ^ (j & 7)) << 4);
+        // a hidden key's address is not formed: it may lie behind the buffer
+        copy16(dst, on ? kp + i * KPI * a.ldk : a.k, on);
+        copy16(dst + HALF, on ? vp + i * KPI * a.ldv : a.v, on);
+      }
+      kp += k_step;
+      vp += v_step;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    return vis;
   };
+  uint32_t ahead[ST];
 #pragma unroll
-  for (int c = 0; c < KC; ++c) {
-    uint4 x = make_uint4(0, 0, 0, 0), y = x;
-    if (g < rows) x = __ldg(reinterpret_cast<const uint4*>(q_row(g) + 32 * c + 8 * t));
-    if (R16 && g + 8 < rows) y = __ldg(reinterpret_cast<const uint4*>(q_row(g + 8) + 32 * c + 8 * t));
-    qa[c][0][0] = x.x, qa[c][0][1] = x.y, qa[c][1][0] = x.z, qa[c][1][1] = x.w;
-    qb[c][0][0] = y.x, qb[c][0][1] = y.y, qb[c][1][0] = y.z, qb[c][1][1] = y.w;
+  for (int c = 0; c < ST; ++c) ahead[c] = fetch(c);
+
+  // B fragments of Q^T: columns 16 i + 2 t, + 1 (first), + 8 (second) of row 8 n + g
+  uint32_t qf[NT][D / 16][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int m = 8 * n + g;
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) +
+                          (m < rows ? (long long)(qs + m / p.group) * a.ldq + (hk * p.group + m % p.group) * D : 0);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      qf[n][i][0] = m < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * i + 2 * t)) : 0u;
+      qf[n][i][1] = m < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * i + 2 * t + 8)) : 0u;
+    }
   }
+  // O^T tiles: (column 16 i + g, rows 8 n + 2t and + 1), (column + 8, the same)
+  float o[NT][D / 16][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
+  float mr[NT][2], lr[NT][2];  // rows 8 n + 2t, + 1: reference maximum (uniform over g) and this lane's part of the sum
+#pragma unroll
+  for (int n = 0; n < NT; ++n) mr[n][0] = mr[n][1] = -INFINITY, lr[n][0] = lr[n][1] = 0.f;
 
-  float o[VC * 8][R16 ? 4 : 2];
+  // ldmatrix: lane l gives the row address of matrix l / 8. K: keys (l & 15), chunk 2 i + (l >> 4).
+  // V^T: keys (l & 7) + 8 * (l >> 4), chunk 2 i + ((l >> 3) & 1).
+  const int kj = lane & 15, kc = lane >> 4, vj = (lane & 7) + 8 * (lane >> 4), vc = (lane >> 3) & 1;
+  for (int step = 0; step < steps; ++step) {
+    const uint32_t vis = ahead[0];
+    asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+    __syncwarp();
+    const uint32_t slot = ring + (step % ST) * STEP;
+    float s[NT][2][4];  // two chains of the sum over a head's columns
 #pragma unroll
-  for (int n = 0; n < VC * 8; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int e = 0; e < (R16 ? 4 : 2); ++e) o[n][e] = 0.f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-
-  const uint16_t* kb = reinterpret_cast<const uint16_t*>(a.k) + hk * D + 8 * t;
-  const uint16_t* vb = reinterpret_cast<const uint16_t*>(a.v) + hk * D + 8 * g;
-  const int stride = csize * XT_WARPS * XT_KEYS;
-  for (int j0 = (rank * XT_WARPS + warp) * XT_KEYS; j0 < seen; j0 += stride) {
-    uint32_t vis = seen - j0 >= XT_KEYS ? 0xffffu : (1u << (seen - j0)) - 1u;
-    if (p.key_mask) {
-      const bool on = lane < XT_KEYS && ((vis >> lane) & 1u) && __ldg(p.key_mask + ks + j0 + lane) != 0;
-      vis = __ballot_sync(0xffffffffu, on);
+      for (int e = 0; e < 4; ++e) s[n][0][e] = s[n][1][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      uint32_t ka[4];
+      ldmatrix4(ka, slot + kj * (D * 2) + (((2 * i + kc) ^ (kj & 7)) << 4));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_16816<F16>(s[n][i & 1], ka, qf[n][i][0], qf[n][i][1]);
     }
-    uint4 kf[2][KC], vf[4][VC];
+    // lane (g, t): keys g and g + 8 of rows 8 n + 2 t, + 1
+    const bool on0 = (vis >> g) & 1u, on1 = (vis >> (g + 8)) & 1u;
+    bool move = false;
+    float x[NT][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const bool on = (vis >> (8 * n + g)) & 1u;
-      const uint16_t* src = kb + (long long)(ks + j0 + 8 * n + g) * a.ldk;
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int c = 0; c < KC; ++c) kf[n][c] = on ? ld_stream(src + 32 * c) : make_uint4(0, 0, 0, 0);
+      for (int e = 0; e < 4; ++e)
+        x[n][e] = (e < 2 ? on0 : on1) ? (s[n][0][e] + s[n][1][e]) * p.scale_log2 : -INFINITY;
+      move = move || fmaxf(x[n][0], x[n][2]) > mr[n][0] + XT_RESCALE_LOG2 ||
+             fmaxf(x[n][1], x[n][3]) > mr[n][1] + XT_RESCALE_LOG2;
     }
+    if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int j = 2 * t + (r & 1) + 8 * (r >> 1);
-      const bool on = (vis >> j) & 1u;
-      const uint16_t* src = vb + (long long)(ks + j0 + j) * a.ldv;
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int c = 0; c < VC; ++c) vf[r][c] = on ? ld_stream(src + 64 * c) : make_uint4(0, 0, 0, 0);
-    }
-    float s[2][4];
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(x[n][e], x[n][e + 2]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float top = fmaxf(mr[n][e], mx);
+          const float f = top > mr[n][e] ? fast_exp2(mr[n][e] - top) : 1.f;
+          mr[n][e] = top;
+          lr[n][e] *= f;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        mma_16816<F16>(s[n], qa[c][0][0], R16 ? qb[c][0][0] : 0u, qa[c][0][1], R16 ? qb[c][0][1] : 0u, kf[n][c].x,
-                       kf[n][c].y);
-        mma_16816<F16>(s[n], qa[c][1][0], R16 ? qb[c][1][0] : 0u, qa[c][1][1], R16 ? qb[c][1][1] : 0u, kf[n][c].z,
-                       kf[n][c].w);
-      }
-      // lane (g, t) holds keys 8 n + 2 t, + 1 of rows g and g + 8
-      const bool on0 = (vis >> (8 * n + 2 * t)) & 1u, on1 = (vis >> (8 * n + 2 * t + 1)) & 1u;
-      s[n][0] = on0 ? s[n][0] * p.scale_log2 : -INFINITY;
-      s[n][1] = on1 ? s[n][1] * p.scale_log2 : -INFINITY;
-      s[n][2] = on0 ? s[n][2] * p.scale_log2 : -INFINITY;
-      s[n][3] = on1 ? s[n][3] * p.scale_log2 : -INFINITY;
-    }
-    auto quad_max = [](float x) {
-      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-      return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-    };
-    const float n0 = fmaxf(m0, quad_max(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]))));
-    const float n1 = R16 ? fmaxf(m1, quad_max(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])))) : 0.f;
-    if (__any_sync(0xffffffffu, n0 > m0 || (R16 && n1 > m1))) {
-      const float f0 = n0 > m0 ? fast_exp2(m0 - n0) : 1.f, f1 = R16 && n1 > m1 ? fast_exp2(m1 - n1) : 1.f;
-      l0 *= f0;
-      l1 *= f1;
-#pragma unroll
-      for (int n = 0; n < VC * 8; ++n) {
-        o[n][0] *= f0;
-        o[n][1] *= f0;
-        if (R16) {
-          o[n][2] *= f1;
-          o[n][3] *= f1;
-        }
-      }
-      m0 = n0;
-      m1 = n1;
-    }
-    const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
-    uint32_t pa[2], pb[2];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const float e0 = fast_exp2(s[n][0] - u0), e1 = fast_exp2(s[n][1] - u0);
-      l0 += e0 + e1;
-      pa[n] = pack_2(e0, e1, F16);
-      pb[n] = 0u;
-      if (R16) {
-        const float e2 = fast_exp2(s[n][2] - u1), e3 = fast_exp2(s[n][3] - u1);
-        l1 += e2 + e3;
-        pb[n] = pack_2(e2, e3, F16);
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < VC; ++c) {
-      const uint32_t w0[4] = {vf[0][c].x, vf[0][c].y, vf[0][c].z, vf[0][c].w};
-      const uint32_t w1[4] = {vf[1][c].x, vf[1][c].y, vf[1][c].z, vf[1][c].w};
-      const uint32_t w2[4] = {vf[2][c].x, vf[2][c].y, vf[2][c].z, vf[2][c].w};
-      const uint32_t w3[4] = {vf[3][c].x, vf[3][c].y, vf[3][c].z, vf[3][c].w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t sel = e & 1 ? 0x7632u : 0x5410u;
-        const uint32_t b0 = __byte_perm(w0[e >> 1], w1[e >> 1], sel), b1 = __byte_perm(w2[e >> 1], w3[e >> 1], sel);
-        float x[4] = {o[8 * c + e][0], o[8 * c + e][1], R16 ? o[8 * c + e][R16 ? 2 : 0] : 0.f,
-                      R16 ? o[8 * c + e][R16 ? 3 : 0] : 0.f};
-        mma_16816<F16>(x, pa[0], pb[0], pa[1], pb[1], b0, b1);
-        o[8 * c + e][0] = x[0];
-        o[8 * c + e][1] = x[1];
-        if (R16) {
-          o[8 * c + e][R16 ? 2 : 0] = x[2];
-          o[8 * c + e][R16 ? 3 : 0] = x[3];
+          for (int i = 0; i < D / 16; ++i) {
+            o[n][i][e] *= f;
+            o[n][i][e + 2] *= f;
+          }
         }
       }
     }
-  }
-
-  // the warp's partial result: lane (g, t) has d = 64 c + 16 t + e (first of a pair) and + 8 (second)
-  auto quad_sum = [](float x) {
-    x += __shfl_xor_sync(0xffffffffu, x, 1);
-    return x + __shfl_xor_sync(0xffffffffu, x, 2);
-  };
-  l0 = quad_sum(l0);
-  l1 = quad_sum(l1);
+    uint32_t pb[NT][2];
 #pragma unroll
-  for (int hh = 0; hh < (R16 ? 2 : 1); ++hh) {
-    float* dst = sh + (warp * ROWS + g + 8 * hh) * D + 16 * t;
-#pragma unroll
-    for (int c = 0; c < VC; ++c)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int n = 8 * c + (e & 7), x = 2 * hh + (e >> 3);
-        *reinterpret_cast<float4*>(dst + 64 * c + e) = make_float4(o[n][x], o[n + 1][x], o[n + 2][x], o[n + 3][x]);
-      }
-    if (t == 0) {
-      sh_m[warp * ROWS + g + 8 * hh] = hh ? m1 : m0;
-      sh_l[warp * ROWS + g + 8 * hh] = hh ? l1 : l0;
+    for (int n = 0; n < NT; ++n) {
+      const float u0 = mr[n][0] == -INFINITY ? 0.f : mr[n][0], u1 = mr[n][1] == -INFINITY ? 0.f : mr[n][1];
+      const float p0 = fast_exp2(x[n][0] - u0), p1 = fast_exp2(x[n][1] - u1);
+      const float p2 = fast_exp2(x[n][2] - u0), p3 = fast_exp2(x[n][3] - u1);
+      lr[n][0] += p0 + p2;
+      lr[n][1] += p1 + p3;
+      pb[n][0] = transpose8(pack_2(p0, p1, F16));
+      pb[n][1] = transpose8(pack_2(p2, p3, F16));
     }
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      uint32_t va[4];
+      ldmatrix4_trans(va, slot + HALF + vj * (D * 2) + (((2 * i + vc) ^ (vj & 7)) << 4));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_16816<F16>(o[n][i], va, pb[n][0], pb[n][1]);
+    }
+    __syncwarp();  // every lane has read the slot
+#pragma unroll
+    for (int c = 0; c + 1 < ST; ++c) ahead[c] = ahead[c + 1];
+    ahead[ST - 1] = fetch(step + ST);
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();  // the rings become the joining buffers
+
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      lr[n][e] += __shfl_xor_sync(0xffffffffu, lr[n][e], 4);
+      lr[n][e] += __shfl_xor_sync(0xffffffffu, lr[n][e], 8);
+      lr[n][e] += __shfl_xor_sync(0xffffffffu, lr[n][e], 16);
+      const int r = warp * ROWS + 8 * n + 2 * t + e;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        sh[r * D + 16 * i + g] = o[n][i][e];
+        sh[r * D + 16 * i + g + 8] = o[n][i][e + 2];
+      }
+      if (g == 0) {
+        sh_m[r] = mr[n][e];
+        sh_l[r] = lr[n][e];
+      }
+    }
   __syncthreads();
   // the CTA's, in warp 0's place: an element is read and written by the same thread
   float keep_m = -INFINITY, keep_l = 0.f;
@@ -287,24 +312,38 @@ __global__ void __launch_bounds__(XT_THREADS, R16 ? 1 : 2) cross_token_kernel(co
     const float inv = l > 0.f ? 1.f / l : 0.f;
     const long long row = qs + r / p.group;
     const int h = hk * p.group + r % p.group;
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + h * D + d;
-    *reinterpret_cast<uint2*>(dst) =
-        make_uint2(pack_2(acc.x * inv, acc.y * inv, F16), pack_2(acc.z * inv, acc.w * inv, F16));
-    if (d == 0 && p.lse)
-      p.lse[(long long)h * p.total_q + row] = l > 0.f ? (mx + __log2f(l)) * 0.6931471805599453f : -INFINITY;
+    acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    const float lse = l > 0.f ? (mx + __log2f(l)) * 0.6931471805599453f : -INFINITY;
+    if (p.parts > 1) {
+      const long long at = ((long long)part * p.heads + h) * p.total_q + row;
+      *reinterpret_cast<float4*>(p.part_o + at * D + d) = acc;
+      if (d == 0) p.part_lse[at] = lse;
+    } else {
+      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + h * D + d;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_2(acc.x, acc.y, F16), pack_2(acc.z, acc.w, F16));
+      if (d == 0 && p.lse) p.lse[(long long)h * p.total_q + row] = lse;
+    }
   }
   cl.sync();  // no CTA leaves while another reads its shared memory
 }
 
-template <int D, bool F16, bool R16>
-static int launch_token(const XTokenParams& a, int csize, cudaStream_t st) {
-  constexpr int ROWS = R16 ? 16 : 8;
-  constexpr int SMEM = (XT_WARPS * ROWS * D + 2 * XT_WARPS * ROWS) * 4;
-  auto kern = cross_token_kernel<D, F16, R16>;
+template <int D, bool F16, int NT>
+static int launch_token(const XTokenParams& a, int csize, int sms, cudaStream_t st) {
+  constexpr int ROWS = 8 * NT;
+  constexpr int RING = XT_WARPS * XT_STAGES<D> * 2 * XT_KEYS * D * 2;
+  constexpr int JOIN = (XT_WARPS * ROWS * D + 2 * XT_WARPS * ROWS) * 4;
+  constexpr int NEED = RING > JOIN ? RING : JOIN;
+  constexpr int ALONE = 120 * 1024;  // no second CTA fits beside it
+  static_assert(NEED <= ALONE && 2 * (NEED + 1024) <= 228 * 1024, "two CTAs an SM");
+  const long long ctas = (long long)a.p.batch * a.p.kv_heads * a.p.parts * csize;
+  // The CTAs of a cluster are packed two to an SM where two fit, even when SMs are left empty. A launch that has an
+  // SM for every CTA asks for so much shared memory that they spread.
+  const int SMEM = ctas <= sms ? ALONE : NEED;
+  auto kern = cross_token_kernel<D, F16, NT>;
   int rc;
-  if ((rc = ensure_smem(kern, SMEM))) return rc;
+  if ((rc = ensure_smem(kern, ALONE))) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((long long)a.p.batch * a.p.kv_heads * csize));
+  cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(XT_THREADS);
   cfg.dynamicSmemBytes = SMEM;
   cfg.stream = st;
@@ -328,16 +367,27 @@ static int launch_token(const XTokenParams& a, int csize, cudaStream_t st) {
   return launch_status();
 }
 
-// Cluster size: more CTAs to a key head while the launch leaves SMs idle and every warp still has a step of keys.
+// Parts of the keys that are joined by a second launch: when even clusters of 8 leave SMs empty and the keys are
+// long enough to pay for that launch. Two CTAs an SM.
+int cross_token_parts(int batch, int kv_heads, int max_k, int sms) {
+  const long long units = (long long)batch * kv_heads;
+  if (units * XT_MAX_CLUSTER >= sms || max_k < 2 * XT_MAX_CLUSTER * XT_PART_KEYS) return 1;
+  const long long fill = 2LL * sms / units, most = max_k / XT_PART_KEYS;
+  return (int)(fill < most ? fill : most);
+}
+
+// Cluster size: more CTAs to a key head while the launch leaves room for them and every warp still has a step of keys.
 int cross_token(const XParams& p, const void* q, const void* k, const void* v, long long ldq, long long ldk,
                 long long ldv, int head_dim, int sms, cudaStream_t st) {
   XTokenParams a = {p, q, k, v, ldq, ldk, ldv};
   const long long units = (long long)p.batch * p.kv_heads;
   int csize = 1;
-  while (csize < 8 && units * csize < 2LL * sms && (long long)csize * 2 * XT_WARPS * XT_KEYS <= p.Lk) csize *= 2;
-  const bool r16 = (long long)p.Lq * p.group > 8;
-#define SA3_TOKEN(D, F)                                                              \
-  return r16 ? launch_token<D, F, true>(a, csize, st) : launch_token<D, F, false>(a, csize, st)
+  while (p.parts == 1 && csize < XT_MAX_CLUSTER && units * csize * 2 <= 2LL * sms &&
+         (long long)csize * 2 * XT_WARPS * XT_KEYS <= p.Lk)
+    csize *= 2;
+  const bool two = (long long)p.Lq * p.group > 8;
+#define SA3_TOKEN(D, F) \
+  return two ? launch_token<D, F, 2>(a, csize, sms, st) : launch_token<D, F, 1>(a, csize, sms, st)
   if (head_dim == 64) {
     if (p.f16) {
       SA3_TOKEN(64, true);

@@ -8,6 +8,7 @@
 #include <stdint.h>
 #include <stdlib.h>
 
+#include <atomic>
 #include <mutex>
 #include <set>
 #include <utility>
@@ -119,6 +120,17 @@ inline int ensure_smem(F func, int bytes) {
     return SA3_ERR_LAUNCH;
   done.insert(key);
   return SA3_OK;
+}
+
+// SM count of the current device, asked once per device; 0 on failure.
+inline int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 0;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 }  // namespace sa3

@@ -86,7 +86,8 @@ SIGNATURES = {
     "sa3_rotary": [c_vp, c_vp, c_vp, c_vp, c_int, c_ll, c_int, c_int, c_int, c_int, c_ll, c_ll, c_ll, c_ll, c_vp, c_vp,
                    c_ll, c_ll, c_int, c_int, c_float, c_vp],
     "sa3_cross_attention": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int,
-                            c_int, c_int, c_int, c_ll, c_ll, c_ll, c_ll, c_float, c_int, c_vp],
+                            c_int, c_int, c_int, c_ll, c_ll, c_ll, c_ll, c_float, c_int, c_vp, c_ll, c_vp],
+    "sa3_cross_attention_workspace": [c_int, c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(c_ll)],
     "sa3_cross_attention_bwd_workspace": [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                           ctypes.POINTER(c_ll)],
     "sa3_cross_attention_bwd": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int,
@@ -114,6 +115,8 @@ def library_path() -> str:
 def load(build_if_missing: bool = True) -> ctypes.CDLL:
     """Load libsa3b200.so (building it in-tree first if it is absent)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

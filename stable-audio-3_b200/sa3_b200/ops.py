@@ -7,6 +7,7 @@ non-zero status. Nothing here computes on the CPU: a CPU tensor is an error.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional, Sequence
 
@@ -302,37 +303,46 @@ def diff_attn_swa(q_bat: torch.Tensor, k_bat: torch.Tensor, v_bat: torch.Tensor,
 
 
 # ---------------------------------------------------------------------- rotary positions, cross-attention
-def _one_device(*ts: Optional[torch.Tensor]) -> torch.device:
-    """The device of the tensors, which must be CUDA tensors of one device."""
-    dev = None
+def _device_of(*ts: Optional[torch.Tensor]) -> int:
+    """The device index of the tensors, which must be CUDA tensors of one device."""
+    dev = ts[0].get_device()
+    if dev < 0:
+        raise RuntimeError("sa3_b200 ops run on CUDA tensors only (no CPU path)")
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("sa3_b200 ops run on CUDA tensors only (no CPU path)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"tensors on {dev} and {t.device}: one call works on one device")
+        if t is not None and t.get_device() != dev:
+            if not t.is_cuda:
+                raise RuntimeError("sa3_b200 ops run on CUDA tensors only (no CPU path)")
+            raise RuntimeError(f"tensors on {ts[0].device} and {t.device}: one call works on one device")
     return dev
 
 
-def _rows_view(t: torch.Tensor, rows: Optional[int], cols: int, name: str, dtype: torch.dtype) -> int:
+def _on_device(dev: int, fn, *args) -> int:
+    """fn(*args, the current stream of device `dev`), with that device current (the library launches on it)."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)  # torch.cuda.current_stream(dev).cuda_stream takes 3 us
+    if torch._C._cuda_getDevice() == dev:
+        return fn(*args, stream)
+    with torch.cuda.device(dev):
+        return fn(*args, stream)
+
+
+def _rows_view(t: torch.Tensor, rows: int, cols: int, name: str, dtype: torch.dtype) -> int:
     """Row stride of a token-row view [rows, cols]; refuses other shapes, types and strides."""
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != 2 or t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
-        raise RuntimeError(f"{name} must be [{'rows' if rows is None else rows}, {cols}], got {tuple(t.shape)}")
-    if t.stride(1) != 1 and t.shape[1] > 1 and t.numel() > 0:
+    if tuple(t.shape) != (rows, cols):
+        raise RuntimeError(f"{name} must be [{rows}, {cols}], got {tuple(t.shape)}")
+    ld, inner = t.stride()
+    if rows <= 1:
+        ld = cols  # one row has no stride of its own: torch may report anything there
+    if inner != 1 and cols > 1 and rows > 0:
         raise RuntimeError(f"{name} must be a row-major view, got strides {t.stride()}")
-    # a single row has no stride of its own: torch may report anything there
-    return t.stride(0) if t.shape[0] > 1 else cols
+    return ld
 
 
 def _index(t: Optional[torch.Tensor], n: int, name: str) -> Optional[int]:
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not torch.int32 or tuple(t.shape) != (n,) or not t.is_contiguous():
         raise RuntimeError(f"{name} must be a contiguous int32 tensor of {n} elements")
     return t.data_ptr()
 
@@ -383,72 +393,91 @@ def rotary(q: torch.Tensor, inv_freq: torch.Tensor, *, heads: int, head_dim: int
     position row_pos[r] (int32), or offset + r % rows_per_batch (0: one sequence). inverse=True rotates back, with the
     same scale: the gradient. out / k_out may be q / k themselves. Returns out, or (out, k_out) when k is given.
     """
-    dev = _one_device(q, inv_freq, k, row_pos, out, k_out)
-    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise RuntimeError(f"rotary works on bf16, fp16 or fp32, got {q.dtype}")
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+    dev = _device_of(q, inv_freq, k, row_pos, out, k_out)
+    dtype = q.dtype
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise RuntimeError(f"rotary works on bf16, fp16 or fp32, got {dtype}")
+    if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise RuntimeError("inv_freq must be a contiguous float64 tensor [rot_dim / 2]")
     if heads <= 0 or head_dim <= 0:
         raise RuntimeError("heads and head_dim must be positive")
-    if not -2 ** 62 < offset < 2 ** 62 or rows_per_batch < 0:
-        raise RuntimeError("offset out of range or negative rows_per_batch")
-    rows, rot_dim = q.shape[0], 2 * inv_freq.numel()
-    ldq = _rows_view(q, None, heads * head_dim, "q", q.dtype)
+    if not -2 ** 62 < offset < 2 ** 62 or not 0 <= rows_per_batch < 2 ** 62:
+        raise RuntimeError("offset or rows_per_batch out of range")
+    rows, wq, wk = q.shape[0], heads * head_dim, kv_heads * head_dim
+    ldq = _rows_view(q, rows, wq, "q", dtype)
+    ldqo, ldk, ldko = wq, 0, 0
     if out is None:
-        out = torch.empty(rows, heads * head_dim, device=dev, dtype=q.dtype)
-    ldqo = _rows_view(out, rows, heads * head_dim, "out", q.dtype)
-    ldk = ldko = 0
+        out = q.new_empty(rows, wq)
+    else:
+        ldqo = _rows_view(out, rows, wq, "out", dtype)
     if k is not None:
         if kv_heads <= 0:
             raise RuntimeError("k needs kv_heads")
-        ldk = _rows_view(k, rows, kv_heads * head_dim, "k", q.dtype)
+        ldk, ldko = _rows_view(k, rows, wk, "k", dtype), wk
         if k_out is None:
-            k_out = torch.empty(rows, kv_heads * head_dim, device=dev, dtype=q.dtype)
-        ldko = _rows_view(k_out, rows, kv_heads * head_dim, "k_out", q.dtype)
-    elif k_out is not None:
-        raise RuntimeError("k_out without k")
+            k_out = k.new_empty(rows, wk)
+        else:
+            ldko = _rows_view(k_out, rows, wk, "k_out", dtype)
+    elif k_out is not None or kv_heads:
+        raise RuntimeError("k_out or kv_heads without k")
     pos = _index(row_pos, rows, "row_pos")
     _count()
-    with torch.cuda.device(dev):
-        rc = _lib.load().sa3_rotary(q.data_ptr(), out.data_ptr(), _ptr(k), _ptr(k_out), _dt(q), rows, heads,
-                                    kv_heads if k is not None else 0, head_dim, rot_dim, ldq, ldqo, ldk, ldko,
-                                    inv_freq.data_ptr(), pos, rows_per_batch, offset, int(interleaved), int(inverse),
-                                    float(scale), _stream())
-    _lib.check(rc, "sa3_rotary")
+    rc = _on_device(dev, _lib.load().sa3_rotary, q.data_ptr(), out.data_ptr(), _ptr(k), _ptr(k_out), _dt(q), rows,
+                    heads, kv_heads, head_dim, 2 * inv_freq.numel(), ldq, ldqo, ldk, ldko, inv_freq.data_ptr(), pos,
+                    rows_per_batch, offset, interleaved, inverse, scale)
+    if rc:
+        _lib.check(rc, "sa3_rotary")
     return out if k is None else (out, k_out)
 
 
 def _cross_args(q, k, v, heads, kv_heads, head_dim, batch, max_seqlen_q, max_seqlen_k, cu_seqlens_q, cu_seqlens_k,
                 k_lens, key_mask, softmax_scale):
     """Checks shared by the two passes; (kv_heads, strides of q k v, index pointers, batch, scale)."""
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise RuntimeError(f"cross_attention works on bf16 or fp16, got {q.dtype}")
-    kv_heads = heads if kv_heads is None else kv_heads
+    dtype = q.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise RuntimeError(f"cross_attention works on bf16 or fp16, got {dtype}")
+    if kv_heads is None:
+        kv_heads = heads
     if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
         raise RuntimeError("heads must be a positive multiple of kv_heads")
     if head_dim not in (64, 128):
         raise RuntimeError("cross_attention implements head_dim 64 and 128")
-    ld = (_rows_view(q, None, heads * head_dim, "q", q.dtype), _rows_view(k, None, kv_heads * head_dim, "k", q.dtype),
-          _rows_view(v, k.shape[0], kv_heads * head_dim, "v", q.dtype))
-    n = [None if c is None else c.numel() - 1 for c in (cu_seqlens_q, cu_seqlens_k)]
-    for x in n:
-        if x is not None:
-            batch = x
-    if batch < 0 or any(x is not None and x != batch for x in n):
-        raise RuntimeError("cu_seqlens_q and cu_seqlens_k must describe the same number of sequences")
-    if cu_seqlens_q is None and q.shape[0] != batch * max_seqlen_q:
+    rows, krows, wk = q.shape[0], k.shape[0], kv_heads * head_dim
+    ld = (_rows_view(q, rows, heads * head_dim, "q", dtype), _rows_view(k, krows, wk, "k", dtype),
+          _rows_view(v, krows, wk, "v", dtype))
+    if cu_seqlens_q is not None:
+        batch = cu_seqlens_q.numel() - 1
+    elif cu_seqlens_k is not None:
+        batch = cu_seqlens_k.numel() - 1
+    if batch < 0 or max_seqlen_q < 0 or max_seqlen_k < 0:
+        raise RuntimeError("batch and lengths must not be negative")
+    if cu_seqlens_q is None and rows != batch * max_seqlen_q:
         raise RuntimeError("uniform queries need rows = batch * max_seqlen_q")
-    if cu_seqlens_k is None and k.shape[0] != batch * max_seqlen_k:
+    if cu_seqlens_k is None and krows != batch * max_seqlen_k:
         raise RuntimeError("uniform keys need rows = batch * max_seqlen_k")
     if key_mask is not None and (key_mask.dtype not in (torch.bool, torch.uint8) or not key_mask.is_contiguous()
-                                 or key_mask.numel() != k.shape[0]):
+                                 or key_mask.numel() != krows):
         raise RuntimeError("key_mask must be a contiguous bool or uint8 tensor with one element a key row")
     idx = (_index(cu_seqlens_q, batch + 1, "cu_seqlens_q"), _index(cu_seqlens_k, batch + 1, "cu_seqlens_k"),
            _index(k_lens, batch, "k_lens"), _ptr(key_mask))
-    scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else float(softmax_scale)
+    scale = head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not 0.0 < scale < math.inf:
         raise RuntimeError("softmax_scale must be positive and finite")
     return kv_heads, ld, idx, batch, scale
+
+
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(name: str, dev: int, *sizes) -> int:
+    """Scratch of a pass: a function of the device's SM count and the sizes alone."""
+    n = ctypes.c_longlong(0)
+    with torch.cuda.device(dev):
+        _lib.check(getattr(_lib.load(), name)(*sizes, ctypes.byref(n)), name)
+    return n.value
+
+
+def _check_lse(lse, heads, rows):
+    if lse.dtype is not torch.float32 or tuple(lse.shape) != (heads, rows) or not lse.is_contiguous():
+        raise RuntimeError(f"lse must be a contiguous float32 tensor [{heads}, {rows}]")
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, heads: int, kv_heads: Optional[int] = None,
@@ -462,25 +491,29 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, heads:
     Uniform sequences of max_seqlen_q / max_seqlen_k rows, or packed ones: cu_seqlens_q / cu_seqlens_k (int32
     [batch + 1], each optional), with max_seqlen the longest. k_lens (int32 [batch]): how many keys of a sequence are
     visible; key_mask (bool or uint8, one element a key row): zero hides a key. Rows that see no key give zeros and
-    lse = -inf. Returns out, or (out, lse) with return_lse (lse fp32 [heads, rows], which the backward pass takes).
+    lse = -inf. Scratch, where it is needed, comes from torch's allocator on the current stream. Returns out, or (out, lse) with return_lse (lse fp32 [heads, rows], which the backward pass takes).
     """
-    dev = _one_device(q, k, v, cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, out, lse)
+    dev = _device_of(q, k, v, cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, out, lse)
     kv_heads, ld, idx, batch, scale = _cross_args(q, k, v, heads, kv_heads, head_dim, batch, max_seqlen_q, max_seqlen_k,
                                                   cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, softmax_scale)
-    rows = q.shape[0]
+    rows, width = q.shape[0], heads * head_dim
     if out is None:
-        out = torch.empty(rows, heads * head_dim, device=dev, dtype=q.dtype)
-    ldo = _rows_view(out, rows, heads * head_dim, "out", q.dtype)
-    if lse is None and return_lse:
-        lse = torch.empty(heads, rows, device=dev, dtype=torch.float32)
-    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (heads, rows) or not lse.is_contiguous()):
-        raise RuntimeError(f"lse must be a contiguous float32 tensor [{heads}, {rows}]")
+        out, ldo = q.new_empty(rows, width), width
+    else:
+        ldo = _rows_view(out, rows, width, "out", q.dtype)
+    if lse is not None:
+        _check_lse(lse, heads, rows)
+    elif return_lse:
+        lse = q.new_empty(heads, rows, dtype=torch.float32)
+    n = _scratch_bytes("sa3_cross_attention_workspace", dev, batch, max_seqlen_q, max_seqlen_k, rows, heads, kv_heads,
+                       head_dim)
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
     _count()
-    with torch.cuda.device(dev):
-        rc = _lib.load().sa3_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), *idx,
-                                             batch, max_seqlen_q, max_seqlen_k, rows, k.shape[0], heads, kv_heads,
-                                             head_dim, *ld, ldo, scale, _dt(q), _stream())
-    _lib.check(rc, "sa3_cross_attention")
+    rc = _on_device(dev, _lib.load().sa3_cross_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                    _ptr(lse), *idx, batch, max_seqlen_q, max_seqlen_k, rows, k.shape[0], heads, kv_heads, head_dim,
+                    *ld, ldo, scale, _dt(q), _ptr(ws), n)
+    if rc:
+        _lib.check(rc, "sa3_cross_attention")
     return (out, lse) if return_lse else out
 
 
@@ -492,32 +525,36 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
                              dv: Optional[torch.Tensor] = None):
     """(dq, dk, dv) of sum(out * dout), with out and lse from `cross_attention(..., return_lse=True)` of the same
     arguments. The same bits in every run. Scratch comes from torch's allocator on the current stream."""
-    dev = _one_device(dout, q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, dq, dk, dv)
+    dev = _device_of(q, dout, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, dq, dk, dv)
     kv_heads, ld, idx, batch, scale = _cross_args(q, k, v, heads, kv_heads, head_dim, batch, max_seqlen_q, max_seqlen_k,
                                                   cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, softmax_scale)
-    rows, krows, wq, wk = q.shape[0], k.shape[0], heads * head_dim, kv_heads * head_dim
-    lddo = _rows_view(dout, rows, wq, "dout", q.dtype)
-    ldo = _rows_view(out, rows, wq, "out", q.dtype)
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (heads, rows) or not lse.is_contiguous():
-        raise RuntimeError(f"lse must be a contiguous float32 tensor [{heads}, {rows}]")
-    dq = torch.empty(rows, wq, device=dev, dtype=q.dtype) if dq is None else dq
-    dk = torch.empty(krows, wk, device=dev, dtype=q.dtype) if dk is None else dk
-    dv = torch.empty(krows, wk, device=dev, dtype=q.dtype) if dv is None else dv
-    ldd = (_rows_view(dq, rows, wq, "dq", q.dtype), _rows_view(dk, krows, wk, "dk", q.dtype),
-           _rows_view(dv, krows, wk, "dv", q.dtype))
-    lib = _lib.load()
+    rows, krows, wq, wk, dtype = q.shape[0], k.shape[0], heads * head_dim, kv_heads * head_dim, q.dtype
+    lddo = _rows_view(dout, rows, wq, "dout", dtype)
+    ldo = _rows_view(out, rows, wq, "out", dtype)
+    _check_lse(lse, heads, rows)
+    lddq, lddk, lddv = wq, wk, wk
+    if dq is None:
+        dq = q.new_empty(rows, wq)
+    else:
+        lddq = _rows_view(dq, rows, wq, "dq", dtype)
+    if dk is None:
+        dk = k.new_empty(krows, wk)
+    else:
+        lddk = _rows_view(dk, krows, wk, "dk", dtype)
+    if dv is None:
+        dv = v.new_empty(krows, wk)
+    else:
+        lddv = _rows_view(dv, krows, wk, "dv", dtype)
+    n = _scratch_bytes("sa3_cross_attention_bwd_workspace", dev, batch, max_seqlen_q, max_seqlen_k, rows, krows, heads,
+                       kv_heads, head_dim)
+    ws = q.new_empty(n, dtype=torch.uint8)
     _count()
-    with torch.cuda.device(dev):
-        n = ctypes.c_longlong(0)
-        _lib.check(lib.sa3_cross_attention_bwd_workspace(batch, max_seqlen_q, max_seqlen_k, rows, krows, heads, kv_heads,
-                                                         head_dim, ctypes.byref(n)),
-                   "sa3_cross_attention_bwd_workspace")
-        ws = torch.empty(n.value, device=dev, dtype=torch.uint8)
-        rc = lib.sa3_cross_attention_bwd(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                         lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *idx, batch,
-                                         max_seqlen_q, max_seqlen_k, rows, krows, heads, kv_heads, head_dim, lddo, *ld,
-                                         ldo, *ldd, scale, _dt(q), ws.data_ptr(), n.value, _stream())
-    _lib.check(rc, "sa3_cross_attention_bwd")
+    rc = _on_device(dev, _lib.load().sa3_cross_attention_bwd, dout.data_ptr(), q.data_ptr(), k.data_ptr(),
+                    v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *idx,
+                    batch, max_seqlen_q, max_seqlen_k, rows, krows, heads, kv_heads, head_dim, lddo, *ld, ldo, lddq,
+                    lddk, lddv, scale, _dt(q), ws.data_ptr(), n)
+    if rc:
+        _lib.check(rc, "sa3_cross_attention_bwd")
     return dq, dk, dv
 
 

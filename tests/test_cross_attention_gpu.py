@@ -208,3 +208,22 @@ def test_backward(cuda, dtype, d, batch, lq, lk, heads, kv_heads):
 @pytest.mark.parametrize("lq,lk", [(2, 5), (150, 70), (70, 300)])
 def test_masks_backward(cuda, mask, packed, d, lq, lk):
     run_case(cuda, 4, lq, lk, 4, 2, d, "bf16", mask=mask, packed=packed)
+
+
+@pytest.mark.parametrize("mask", ["none", "lengths", "keys", "both"])
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("batch,lq,lk,heads,kv_heads,d,dtype", [
+    (1, 40, 5003, 4, 2, 64, "bf16"),    # query tiles that leave CTA slots empty
+    (3, 33, 1500, 2, 1, 128, "fp16"),
+    (1, 1, 9001, 2, 1, 128, "bf16"),    # single tokens over long keys
+    (3, 2, 8300, 6, 2, 64, "fp16"),
+])
+def test_split_keys(cuda, mask, packed, batch, lq, lk, heads, kv_heads, d, dtype):
+    run_case(cuda, batch, lq, lk, heads, kv_heads, d, dtype, mask=mask, packed=packed, backward=mask == "both")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_scores_move_the_reference_maximum(cuda, d):
+    """Scores spread over hundreds: the running maximum moves in most tiles."""
+    run_case(cuda, 1, 200, 700, 2, 1, d, "bf16", spread=30.0, backward=False)
+    run_case(cuda, 1, 1, 700, 2, 1, d, "fp16", spread=30.0, backward=False)
