@@ -107,6 +107,65 @@ __device__ __forceinline__ void commit_elect(uint64_t* bar) {
       "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
       : "memory");
 }
+// 16 columns of this thread's TMEM lane, complete on return
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+  tmem_wait_ld();
+}
+
+// Four K = 16 steps under one election: SS operands K-major in 128-byte rows (+32 bytes a step on both sides), TS with
+// A in TMEM (+8 columns a step) and an MN-major B (+16 rows of 128 bytes a step).
+__device__ __forceinline__ void mma4_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 r, x, y;\n\t.reg .b64 da, db;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t"
+      "setp.eq.b32 p, %4, %4;\n\t"
+      "add.u32 x, %1, 2;\n\tadd.u32 y, %2, 2;\n\tmov.b64 da, {x, %3};\n\tmov.b64 db, {y, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t"
+      "add.u32 x, %1, 4;\n\tadd.u32 y, %2, 4;\n\tmov.b64 da, {x, %3};\n\tmov.b64 db, {y, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t"
+      "add.u32 x, %1, 6;\n\tadd.u32 y, %2, 6;\n\tmov.b64 da, {x, %3};\n\tmov.b64 db, {y, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma4_ts(uint32_t d_tmem, uint32_t a0, uint32_t a1, uint32_t b_lo, uint32_t b_hi,
+                                        uint32_t idesc, uint32_t accumulate) {
+  // a0: columns of steps 0 and 1, a1: of steps 2 and 3
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 r, x, y;\n\t.reg .b64 db;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %5, p;\n\t"
+      "setp.eq.b32 p, %5, %5;\n\t"
+      "add.u32 x, %1, 8;\n\tadd.u32 y, %3, 128;\n\tmov.b64 db, {y, %4};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %5, p;\n\t"
+      "add.u32 y, %3, 256;\n\tmov.b64 db, {y, %4};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%2], db, %5, p;\n\t"
+      "add.u32 x, %2, 8;\n\tadd.u32 y, %3, 384;\n\tmov.b64 db, {y, %4};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %5, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a0), "r"(a1), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit2_elect(uint64_t* a, uint64_t* b) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}\n" ::"r"(smem_u32(a)),
+      "r"(smem_u32(b))
+      : "memory");
+}
 // mbar_wait on every lane of a converged warp; the warp agrees on the outcome.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int site) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, site));

@@ -28,15 +28,15 @@ constexpr float XA_RESCALE_LOG2 = 8.f;  // move the reference maximum only when 
 constexpr int XA_SUB_M = XA_BM * 128;   // bytes of a 64-column sub-tile of the wide side
 constexpr int XA_SUB_N = XA_BN * 128;   // ... of the walked side
 
+// the lowest min(n, 64) bits
+__device__ __forceinline__ uint64_t low_bits64(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+
 // Bit i: key j0 + i of the sequence is visible (i < 64). All lanes of a warp call it and get the same word.
 __device__ __forceinline__ uint64_t visible64(const XParams& p, const XSeq& s, int j0, int lane) {
   const int n = s.seen - j0;
-  bool a = lane < n, b = lane + 32 < n;
-  if (p.key_mask) {
-    const uint8_t* m = p.key_mask + s.ks + j0;
-    a = a && __ldg(m + lane) != 0;
-    b = b && __ldg(m + lane + 32) != 0;
-  }
+  if (!p.key_mask) return low_bits64(n);
+  const uint8_t* m = p.key_mask + s.ks + j0;
+  const bool a = lane < n && __ldg(m + lane) != 0, b = lane + 32 < n && __ldg(m + lane + 32) != 0;
   const uint32_t lo = __ballot_sync(0xffffffffu, a), hi = __ballot_sync(0xffffffffu, b);
   return ((uint64_t)hi << 32) | lo;
 }
@@ -60,21 +60,57 @@ __device__ __forceinline__ float unpack_hi(uint32_t w, bool f16) {
   return f16 ? __half2float(__ushort_as_half((unsigned short)(w >> 16))) : __uint_as_float(w & 0xffff0000u);
 }
 
+__device__ __forceinline__ float max32(const uint32_t (&s)[32]) {
+  float m[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m[e] = -INFINITY;
+  max_chunk(s, m);
+  return fmaxf(fmax3(fmax3(m[0], m[1], m[2]), m[3], m[4]), fmax3(m[5], m[6], m[7]));
+}
+
 // scores of hidden columns become -inf
 __device__ __forceinline__ void hide32(uint32_t (&s)[32], uint32_t vis) {
 #pragma unroll
   for (int e = 0; e < 32; ++e) s[e] = (vis >> e) & 1u ? s[e] : NEG_INF_BITS;
 }
 
-// D columns of one TMEM lane times f, rounded to 16 bits, to a row in memory
-template <int D>
-__device__ __forceinline__ void store_row16(uint32_t t_o, float f, bool f16, bool store, void* dst) {
+// A softmax warp's 32 TMEM lanes x NC columns, times f (0 where !keep), rounded to 16 bits, to the first `rows` of 32
+// rows at dst. A lane holds one row: 16 columns at a time go through shared memory (chunk c of row r at c ^ (r / 4 & 1):
+// no bank conflicts either way), so that a store instruction fills whole 32-byte sectors, two lanes to a row.
+constexpr int XA_STAGE = 32 * 32;
+template <int NC>
+__device__ __forceinline__ void store_rows16(uint32_t t_src, float f, bool keep, bool f16, uint8_t* stage, int lane,
+                                             int rows, uint16_t* dst, long long ld) {
+  uint16_t* out = dst + (lane >> 1) * ld + (lane & 1) * 8;
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) {
-    uint32_t o[32];
-    tmem_ld32_async(t_o + 32 * c, o);
+  for (int c = 0; c < NC / 16; ++c) {
+    uint32_t o[16], w[8];
+    tmem_ld16(t_src + 16 * c, o);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      w[e] = keep ? pack_2(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f, f16) : 0u;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<uint4*>(stage + lane * 32 + ((e ^ ((lane >> 2) & 1)) << 4)) =
+          make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 16 * e + (lane >> 1);
+      const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 32 + (((lane & 1) ^ ((r >> 2) & 1)) << 4));
+      if (r < rows) *reinterpret_cast<uint4*>(out + 16 * e * ld + 16 * c) = v;
+    }
+    __syncwarp();
+  }
+}
+// one lane's row, directly
+template <int NC>
+__device__ __forceinline__ void store_row16(uint32_t t_src, float f, bool f16, bool store, uint16_t* dst) {
+#pragma unroll
+  for (int c = 0; c < NC / 32; ++c) {
+    uint32_t o[32], w[16];
+    tmem_ld32_async(t_src + 32 * c, o);
     tmem_wait_ld();
-    uint32_t w[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e)
       w[e] = pack_2(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f, f16);
@@ -91,44 +127,87 @@ __device__ __forceinline__ void zero_row16(void* dst) {
   for (int e = 0; e < D / 8; ++e) reinterpret_cast<uint4*>(dst)[e] = make_uint4(0, 0, 0, 0);
 }
 
-// the same in fp32
-template <int D>
-__device__ __forceinline__ void store_row32(uint32_t t_o, float f, bool store, float* dst) {
+// one lane's NC columns in fp32
+template <int NC>
+__device__ __forceinline__ void store_rows32(uint32_t t_src, float f, bool keep, bool store, float* dst) {
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) {
+  for (int c = 0; c < NC / 32; ++c) {
     uint32_t o[32];
-    tmem_ld32_async(t_o + 32 * c, o);
+    tmem_ld32_async(t_src + 32 * c, o);
     tmem_wait_ld();
     if (store)
 #pragma unroll
       for (int e = 0; e < 32; e += 4)
         *reinterpret_cast<float4*>(dst + 32 * c + e) =
-            make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 2]) * f,
-                        __uint_as_float(o[e + 3]) * f);
+            keep ? make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 2]) * f,
+                               __uint_as_float(o[e + 3]) * f)
+                 : make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
 
-// Work item of the forward: query tile (fastest), head, part of the keys, sequence. Keys j0 .. of the part in T tiles.
-struct XItem {
+// The walk of a persistent CTA over work items: query tile (fastest), head, part of the keys, sequence. Steps by the
+// grid without divisions: every role of the CTA walks by itself, and a division there delays each item's first product.
+struct XWalk {
   XSeq s;
-  int tile, h, part, j0, T;
+  int tile, h, part, b;  // the item
+  int j0, T;             // its keys: from j0, in T tiles; T = 0 also for a tile behind the end of its sequence
+  int item, dt, dh, dp, db, qtiles;
+  __device__ __forceinline__ void load(const XParams& p) {
+    const int all = tile * XA_BM < s.lq ? (s.seen + XA_BN - 1) / XA_BN : 0;
+    T = all;
+    j0 = 0;
+    if (p.parts > 1) {
+      const int t0 = (int)((long long)all * part / p.parts);
+      T = (int)((long long)all * (part + 1) / p.parts) - t0;
+      j0 = t0 * XA_BN;
+    }
+  }
+  __device__ __forceinline__ XWalk(const XParams& p, int qt, int num_items) {
+    qtiles = qt;
+    int x = item = blockIdx.x;
+    tile = x % qt, x /= qt, h = x % p.heads, x /= p.heads, part = x % p.parts, b = x / p.parts;
+    x = gridDim.x;
+    dt = x % qt, x /= qt, dh = x % p.heads, x /= p.heads, dp = x % p.parts, db = x / p.parts;
+    if (item < num_items) {
+      s = make_seq(p, b);
+      load(p);
+    }
+  }
+  __device__ __forceinline__ void next(const XParams& p, int num_items) {
+    item += gridDim.x;
+    if (item >= num_items) return;
+    tile += dt;
+    int c = tile >= qtiles;
+    tile -= c ? qtiles : 0;
+    h += dh + c;
+    c = h >= p.heads;
+    h -= c ? p.heads : 0;
+    part += dp + c;
+    c = part >= p.parts;
+    part -= c ? p.parts : 0;
+    const int was = b;
+    b += db + c;
+    if (b != was) s = make_seq(p, b);
+    load(p);
+  }
 };
-__device__ __forceinline__ XItem make_item(const XParams& p, int item, int qtiles) {
-  XItem it;
-  it.tile = item % qtiles;
-  int rest = item / qtiles;
-  it.h = rest % p.heads;
-  rest /= p.heads;
-  it.part = rest % p.parts;
-  it.s = make_seq(p, rest / p.parts);
-  const int all = it.tile * XA_BM < it.s.lq ? (it.s.seen + XA_BN - 1) / XA_BN : 0;
-  const int t0 = (int)((long long)all * it.part / p.parts);
-  it.T = (int)((long long)all * (it.part + 1) / p.parts) - t0;
-  it.j0 = t0 * XA_BN;
-  return it;
-}
 
-constexpr int XA_THREADS = 192;  // warps 0..3 softmax (TMEM lane quarters), 4 TMA, 5 MMA
+// Forward and dQ: warps 0..7 softmax, 8 TMA, 9 and 10 MMA (11 idles). Softmax warp w has TMEM lane quarter w % 4 and
+// columns 32 (w / 4) .. + 31 of every score tile: two warps share a row. The score products and the products with the
+// probabilities are issued by warps of their own: a warp alone takes some ten cycles an instruction, and with one
+// issuer for both, its loop set the time of a tile. A score tile's packed results lie over the scores of the same warp:
+// k-step k at column 32 (k / 2) + 8 (k % 2).
+constexpr int XA_THREADS = 384;
+constexpr int XA_SOFTMAX = 8;      // softmax warps of a CTA: arrivals on the barriers that they release
+constexpr int XA_REGS_LAUNCH = 80;  // two CTAs an SM
+constexpr int XA_REGS_LOW = 48;     // loads and MMA after the split
+constexpr int XA_REGS_HIGH = 96;    // softmax after the split
+static_assert(XA_REGS_LOW * 128 + XA_REGS_HIGH * 256 <= XA_REGS_LAUNCH * XA_THREADS,
+              "register split exceeds the block's launch allocation");
+__device__ __forceinline__ void regs_low() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XA_REGS_LOW)); }
+__device__ __forceinline__ void regs_high() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(XA_REGS_HIGH)); }
+// the two softmax warps that share a lane quarter (64 threads)
+__device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); }
 
 // ------------------------------------------------------------------------------------------------ forward
 // Persistent, two CTAs an SM: while one CTA's softmax warps exponentiate, the other's tensor core and loads run.
@@ -143,10 +222,12 @@ struct XFwd {
   static constexpr int QS = D == 64 ? 2 : 1, KS = D == 64 ? 4 : 2, VS = KS;
   static constexpr int Q_BYTES = SUBS * XA_SUB_M, T_BYTES = SUBS * XA_SUB_N;
   static constexpr int TILES = QS * Q_BYTES + (KS + VS) * T_BYTES;
-  static constexpr int SMEM = TILES + 1024 + 512;
+  static constexpr int PAIRS = 6 * XA_BM * 4;  // maxima [2][2][rows] and sums [2][rows] of the warp pairs
+  static constexpr int SMEM = TILES + XA_SOFTMAX * XA_STAGE + PAIRS + 1024 + 256;
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
-template <int D>
+template <int D, bool F16>
 __global__ void __launch_bounds__(XA_THREADS, 2)
     cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const XParams p, int num_items, int qtiles) {
@@ -156,7 +237,10 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
   auto sQ = [&](int s) { return smem + s * C::Q_BYTES; };
   auto sK = [&](int s) { return smem + C::QS * C::Q_BYTES + s * C::T_BYTES; };
   auto sV = [&](int s) { return smem + C::QS * C::Q_BYTES + (C::KS + s) * C::T_BYTES; };
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::TILES);
+  uint8_t* stage = smem + C::TILES;  // XA_STAGE bytes a softmax warp
+  float* sh_m = reinterpret_cast<float*>(stage + XA_SOFTMAX * XA_STAGE);
+  float* sh_l = sh_m + 4 * XA_BM;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sh_m + 6 * XA_BM);
   uint64_t* q_full = bars;        // [QS]
   uint64_t* q_empty = bars + 2;   // [QS]
   uint64_t* k_full = bars + 4;    // [KS]
@@ -164,19 +248,19 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
   uint64_t* v_full = bars + 12;   // [VS]
   uint64_t* v_empty = bars + 16;  // [VS]
   uint64_t* s_full = bars + 20;   // [2] scores of a tile are in TMEM
-  uint64_t* p_full = bars + 22;   // [2] its probabilities are (4 arrivals)
+  uint64_t* p_full = bars + 22;   // [2] its probabilities are (XA_SOFTMAX arrivals)
   // [2] P V of a tile is done. Two, since the softmax skips most of these phases: when it waits for tile g's it
   // knows that tile g - 2's is over, so the parity on the tile's own barrier cannot be that of an older phase.
   uint64_t* o_full = bars + 24;
-  uint64_t* o_empty = bars + 26;  // the softmax has read an item's O (4 arrivals)
-  uint64_t* done = bars + 27;
-  constexpr int NBARS = 28;
+  uint64_t* o_empty = bars + 26;  // the softmax has read an item's O (XA_SOFTMAX arrivals)
+  uint64_t* done = bars + 27;     // [2]
+  constexpr int NBARS = 29;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < NBARS; ++i) mbar_init(&bars[i], (i == 22 || i == 23 || i == 26) ? 4 : 1);
+    for (int i = 0; i < NBARS; ++i) mbar_init(&bars[i], (i == 22 || i == 23 || i == 26) ? XA_SOFTMAX : 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -193,39 +277,36 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
   const uint32_t tmem = *tmem_slot;
   grid_dep_wait();
 
-  if (warp == 4) {
+  if (warp >= XA_SOFTMAX) regs_low();
+  if (warp == 8) {
     if (lane == 0) {
       int g = 0, qc = 0;
       bool ok = true, v_out = true;  // v_out: V of the last counted tile was issued
-      for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
-        const XItem it = make_item(p, item, qtiles);
+      for (XWalk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+        if (it.T == 0) continue;
         const XSeq& s = it.s;
-        const int tile = it.tile, h = it.h, T = it.T;
-        if (T == 0) continue;
-        const int cq = h * D, ck = (h / p.group) * D;
+        const int cq = it.h * D, ck = (it.h / p.group) * D;
         const int qs = qc % C::QS;
         if (qc >= C::QS && !mbar_wait(&q_empty[qs], ((qc / C::QS) - 1) & 1, abort_flag, 100)) break;
         mbar_arrive_expect_tx(&q_full[qs], C::Q_BYTES);
         for (int c = 0; c < C::SUBS; ++c)
-          tma_load_2d(sQ(qs) + c * XA_SUB_M, &tmQ, &q_full[qs], cq + 64 * c, s.qs + tile * XA_BM);
+          tma_load_2d(sQ(qs) + c * XA_SUB_M, &tmQ, &q_full[qs], cq + 64 * c, s.qs + it.tile * XA_BM);
         qc++;
-        for (int t = 0; t < T; ++t, ++g) {
-          const int ks = g % C::KS;
+        for (int t = 0; t < it.T; ++t, ++g) {
+          const int ks = g % C::KS, row = s.ks + it.j0 + t * XA_BN;
           if (g >= C::KS && !mbar_wait(&k_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 101)) {
             ok = false;
             break;
           }
           mbar_arrive_expect_tx(&k_full[ks], C::T_BYTES);
-          for (int c = 0; c < C::SUBS; ++c)
-            tma_load_2d(sK(ks) + c * XA_SUB_N, &tmK, &k_full[ks], ck + 64 * c, s.ks + it.j0 + t * XA_BN);
+          for (int c = 0; c < C::SUBS; ++c) tma_load_2d(sK(ks) + c * XA_SUB_N, &tmK, &k_full[ks], ck + 64 * c, row);
           if (g >= C::VS && !mbar_wait(&v_empty[ks], ((g / C::VS) - 1) & 1, abort_flag, 102)) {
             g++;
             ok = v_out = false;
             break;
           }
           mbar_arrive_expect_tx(&v_full[ks], C::T_BYTES);
-          for (int c = 0; c < C::SUBS; ++c)
-            tma_load_2d(sV(ks) + c * XA_SUB_N, &tmV, &v_full[ks], ck + 64 * c, s.ks + it.j0 + t * XA_BN);
+          for (int c = 0; c < C::SUBS; ++c) tma_load_2d(sV(ks) + c * XA_SUB_N, &tmV, &v_full[ks], ck + 64 * c, row);
         }
       }
       if (*abort_flag) {
@@ -238,164 +319,186 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
         }
       }
     }
-  } else if (warp == 5) {
-    const int fmt = p.f16 ? 0 : 1;
+  } else if (warp == 9) {
+    // S of every tile: the buffer of tile g held the probabilities of tile g - 2
+    const int fmt = F16 ? 0 : 1;
     const uint32_t base = smem_u32(smem);
-    const uint64_t dk = sdesc_kmajor_sw128(base), dv = sdesc_mnmajor_sw128(base, XA_SUB_N);
+    const uint64_t dk = sdesc_kmajor_sw128(base);
     const uint32_t k_hi = (uint32_t)(dk >> 32), k_lo = (uint32_t)dk;
-    const uint32_t v_hi = (uint32_t)(dv >> 32), v_lo = (uint32_t)dv;
-    const uint32_t idesc_o = make_idesc(128, D, fmt, fmt, 0, 1);
-    const uint32_t t_o = tmem + 128;
-    auto off16 = [&](const uint8_t* x) { return (smem_u32(x) - base) >> 4; };
+    const uint32_t idesc_full = make_idesc(128, XA_BN, fmt, fmt, 0, 0);
     int g = 0, qc = 0;
     bool ok = true;
-    for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
-      const XItem it = make_item(p, item, qtiles);
-      const XSeq& s = it.s;
-      const int T = it.T;
-      if (T == 0) continue;
-      ok = warp_wait(&q_full[qc % C::QS], (qc / C::QS) & 1, abort_flag, 104);
-      auto scores = [&](int t) {
-        const int n = g + (t > 0 ? 1 : 0), ks = n % C::KS;
-        if (!warp_wait(&k_full[ks], (n / C::KS) & 1, abort_flag, 105)) return false;
+    for (XWalk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+      if (it.T == 0) continue;
+      const int qs = qc % C::QS;
+      const uint32_t qlo = k_lo + ((qs * C::Q_BYTES) >> 4);
+      int left = it.s.seen - it.j0;
+      ok = warp_wait(&q_full[qs], (qc / C::QS) & 1, abort_flag, 104);
+      for (int t = 0; t < it.T && ok; ++t, ++g, left -= XA_BN) {
+        const int ks = g % C::KS;
+        ok = warp_wait(&k_full[ks], (g / C::KS) & 1, abort_flag, 105) &&
+             (g < 2 || warp_wait(&o_full[g & 1], ((g - 2) >> 1) & 1, abort_flag, 105));
+        if (!ok) break;
         tc_fence_after();
-        const int cols = (min(XA_BN, s.seen - it.j0 - t * XA_BN) + 15) & ~15;
-        const uint32_t idesc = make_idesc(128, cols, fmt, fmt, 0, 0);
-        const uint32_t qlo = k_lo + off16(sQ(qc % C::QS)), klo = k_lo + off16(sK(ks));
-        const uint32_t t_s = tmem + 64 * (n & 1);
+        const uint32_t idesc = left >= XA_BN ? idesc_full : make_idesc(128, (left + 15) & ~15, fmt, fmt, 0, 0);
+        const uint32_t klo = k_lo + ((C::QS * C::Q_BYTES + ks * C::T_BYTES) >> 4);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          mma_ss_lo(t_s, qlo + (k >> 2) * (XA_SUB_M >> 4) + 2 * (k & 3), klo + (k >> 2) * (XA_SUB_N >> 4) + 2 * (k & 3),
-                    k_hi, idesc, k != 0);
-        commit_elect(&s_full[n & 1]);
-        commit_elect(&k_empty[ks]);
-        if (t == T - 1) commit_elect(&q_empty[qc % C::QS]);
-        return true;
-      };
-      ok = ok && scores(0);
-      for (int t = 0; t < T && ok; ++t, ++g) {
-        if (t + 1 < T && !scores(t + 1)) {
-          ok = false;
-          break;
-        }
-        const int vs = g % C::VS;
-        const int keys = min(XA_BN, s.seen - it.j0 - t * XA_BN), steps = (keys + 15) >> 4;
-        const uint64_t vis = visible64(p, s, it.j0 + t * XA_BN, lane);
-        ok = warp_wait(&v_full[vs], (g / C::VS) & 1, abort_flag, 106);
-        if (!ok) break;
-        const uint64_t all = steps == 4 ? ~0ull : (1ull << (16 * steps)) - 1;
-        if ((vis & all) != all) zero_rows(sV(vs), C::SUBS, 16 * steps, vis, lane);
-        ok = warp_wait(&p_full[g & 1], (g >> 1) & 1, abort_flag, 107) &&
-             (t > 0 || qc == 0 || warp_wait(o_empty, (qc - 1) & 1, abort_flag, 108));
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t vlo = v_lo + off16(sV(vs)), t_p = tmem + 64 * (g & 1);
-        for (int k = 0; k < steps; ++k)
-          mma_ts_lo(t_o, t_p + 8 * k, vlo + k * (2048 >> 4), v_hi, idesc_o, (t > 0 || k > 0) ? 1u : 0u);
-        commit_elect(&o_full[g & 1]);
-        commit_elect(&v_empty[vs]);
+        for (int c = 0; c < C::SUBS; ++c)
+          mma4_ss(tmem + 64 * (g & 1), qlo + c * (XA_SUB_M >> 4), klo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
+        commit2_elect(&s_full[g & 1], &k_empty[ks]);
+        if (t == it.T - 1) commit_elect(&q_empty[qs]);
       }
       qc++;
     }
-    commit_elect(done);
+    commit_elect(&done[0]);
     volatile int never = 0;
-    warp_wait(done, 0, &never, 109);
-  } else {
-    const int r = warp * 32 + lane;
-    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
-    const uint32_t t_o = tmem + lane_off + 128;
+    warp_wait(&done[0], 0, &never, 109);
+  } else if (warp == 10) {
+    // O (+)= P V
+    const int fmt = F16 ? 0 : 1;
+    const uint64_t dv = sdesc_mnmajor_sw128(smem_u32(sV(0)), XA_SUB_N);
+    const uint32_t v_hi = (uint32_t)(dv >> 32), v_lo = (uint32_t)dv;
+    const uint32_t idesc_o = make_idesc(128, D, fmt, fmt, 0, 1);
+    const uint32_t t_o = tmem + 128;
+    int g = 0, qc = 0;
+    bool ok = true;
+    for (XWalk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+      if (it.T == 0) continue;
+      ok = qc == 0 || warp_wait(o_empty, (qc - 1) & 1, abort_flag, 108);
+      for (int t = 0; t < it.T && ok; ++t, ++g) {
+        const int vs = g % C::VS, j0 = it.j0 + t * XA_BN;
+        ok = warp_wait(&v_full[vs], (g / C::VS) & 1, abort_flag, 106);
+        if (!ok) break;
+        const int steps = min(XA_BN / 16, (it.s.seen - j0 + 15) >> 4);
+        if (p.key_mask || it.s.seen - j0 < XA_BN) {
+          const uint64_t vis = visible64(p, it.s, j0, lane), all = low_bits64(16 * steps);
+          if ((vis & all) != all) zero_rows(sV(vs), C::SUBS, 16 * steps, vis, lane);
+        }
+        ok = warp_wait(&p_full[g & 1], (g >> 1) & 1, abort_flag, 107);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t vlo = v_lo + ((vs * C::T_BYTES) >> 4), t_p = tmem + 64 * (g & 1);
+        if (steps == XA_BN / 16) {
+          mma4_ts(t_o, t_p, t_p + 32, vlo, v_hi, idesc_o, t > 0);
+        } else {
+          for (int k = 0; k < steps; ++k)
+            mma_ts_lo(t_o, t_p + 32 * (k >> 1) + 8 * (k & 1), vlo + k * (2048 >> 4), v_hi, idesc_o, (t > 0 || k > 0) ? 1u : 0u);
+        }
+        commit2_elect(&o_full[g & 1], &v_empty[vs]);
+      }
+      qc++;
+    }
+    commit_elect(&done[1]);
+    volatile int never = 0;
+    warp_wait(&done[1], 0, &never, 109);
+  } else if (warp < XA_SOFTMAX) {
+    regs_high();
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t t_o = tmem + lane_off + 128 + half * (D / 2);  // this warp's half of O's columns
+    float* own_m = sh_m + half * XA_BM + quarter * 32 + lane;     // + 2 * XA_BM for odd tiles
+    const float* other_m = sh_m + (1 - half) * XA_BM + quarter * 32 + lane;
     const float NEG_INF = -INFINITY;
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
     int g = 0;
-    for (int item = blockIdx.x; item < num_items; item += gridDim.x) {
-      const XItem it = make_item(p, item, qtiles);
+    for (XWalk it(p, qtiles, num_items); it.item < num_items; it.next(p, num_items)) {
       const XSeq& s = it.s;
-      const int h = it.h, T = it.T;
+      const int T = it.T;
       if (it.tile * XA_BM >= s.lq) continue;
-      const int i = it.tile * XA_BM + r;
-      const bool row_ok = i < s.lq;
-      const long long row = s.qs + i;
-      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + h * D;
-      const long long at = ((long long)it.part * p.heads + h) * p.total_q + row;  // one part: of lse itself
-      float* lse = p.parts > 1 ? p.part_lse + at : p.lse ? p.lse + at : nullptr;
-      if (T == 0) {
-        if (row_ok) {
-          if (p.parts == 1) zero_row16<D>(dst);  // else a part of weight zero, whose output is not read
-          if (lse) *lse = NEG_INF;
-        }
-        continue;
-      }
+      const int rows = min(32, s.lq - it.tile * XA_BM - quarter * 32);  // of this warp that exist
       bool bad = false;
       float m = NEG_INF, l = 0.f;
-      for (int t = 0; t < T; ++t, ++g) {
-        const uint64_t vis = visible64(p, s, it.j0 + t * XA_BN, lane);
-        const uint32_t t_s = tmem + lane_off + 64 * (g & 1);
+      int left = s.seen - it.j0;  // keys of this tile and the following ones
+      for (int t = 0; t < T; ++t, ++g, left -= XA_BN) {
+        uint32_t vis = (uint32_t)(low_bits64(left) >> (32 * half));
+        if (p.key_mask) vis = (uint32_t)(visible64(p, s, it.j0 + t * XA_BN, lane) >> (32 * half));
+        const uint32_t t_s = tmem + lane_off + 64 * (g & 1) + 32 * half;
         if (!mbar_wait(&s_full[g & 1], (g >> 1) & 1, abort_flag, 110)) bad = true;
         tc_fence_after();
-        uint32_t sa[32], sb[32];
-        tmem_ld32_async(t_s, sa);
-        tmem_ld32_async(t_s + 32, sb);
-        tmem_wait_ld();
-        if (vis != ~0ull) {
-          hide32(sa, (uint32_t)vis);
-          hide32(sb, (uint32_t)(vis >> 32));
-        }
-        float mx8[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) mx8[e] = NEG_INF;
-        max_chunk(sa, mx8);
-        max_chunk(sb, mx8);
-        const float mx =
-            fmaxf(fmax3(fmax3(mx8[0], mx8[1], mx8[2]), mx8[3], mx8[4]), fmax3(mx8[5], mx8[6], mx8[7]));
-        const float m_tile = mx * p.scale_log2;  // scale > 0; -inf when the row sees none of these keys
-        const bool move = m_tile > m + XA_RESCALE_LOG2;
-        const float alpha = move ? fast_exp2(m - m_tile) : 1.f;
-        l *= alpha;
-        if (__any_sync(0xffffffffu, move && m != NEG_INF)) {
-          // some row of this warp moves a finite maximum: rescale O once P V of the last tile is done
-          if (!mbar_wait(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 111)) bad = true;
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32], w[16];
-            tmem_ld32_async(t_o + 32 * c, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(o[16 * hh + e]) * alpha);
-              tmem_st16(t_o + 32 * c + 16 * hh, w);
-            }
+        if (rows > 0) {  // else no row of this warp exists: what P holds there is multiplied and never stored
+          uint32_t sa[32];
+          tmem_ld32_async(t_s, sa);
+          tmem_wait_ld();
+          float mx;
+          if (vis == 0xffffffffu) {
+            mx = max32(sa);
+          } else {
+            hide32(sa, vis);
+            mx = max32(sa);
           }
+          // the other half of the row
+          own_m[(g & 1) * 2 * XA_BM] = mx;
+          pair_sync(quarter);
+          mx = fmaxf(mx, other_m[(g & 1) * 2 * XA_BM]);
+          const float m_tile = mx * p.scale_log2;  // scale > 0; -inf when the row sees none of these keys
+          const bool move = m_tile > m + XA_RESCALE_LOG2;
+          if (__any_sync(0xffffffffu, move)) {
+            const float alpha = move ? fast_exp2(m - m_tile) : 1.f;
+            l *= alpha;
+            if (t > 0) {
+              // rescale this warp's half of O once P V of the last tile is done
+              if (!mbar_wait(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 111)) bad = true;
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < D / 64; ++c) {
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                  uint32_t o[16];
+                  tmem_ld16(t_o + 32 * c + 16 * hh, o);
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                  tmem_st16(t_o + 32 * c + 16 * hh, o);
+                }
+              }
+            }
+            if (move) m = m_tile;
+          }
+          if (left > 32 * half) {  // columns behind the last key are not multiplied
+            const float mu = m == NEG_INF ? 0.f : m;
+            uint64_t acc[4] = {0, 0, 0, 0};
+            uint32_t w[16];
+            exp_chunk(sa, scale2, f2(-mu, -mu), acc, w, F16);
+            tmem_st16(t_s, w);
+            const float2 sum = f2_split(fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3])));
+            l += sum.x + sum.y;
+          }
+          tmem_wait_st();
         }
-        if (move) m = m_tile;
-        const float mu = m == NEG_INF ? 0.f : m;
-        const uint64_t negm2 = f2(-mu, -mu);
-        uint64_t acc[4] = {0, 0, 0, 0};
-        uint32_t w[16];
-        exp_chunk(sa, scale2, negm2, acc, w, p.f16);
-        tmem_st16(t_s, w);
-        exp_chunk(sb, scale2, negm2, acc, w, p.f16);
-        tmem_st16(t_s + 16, w);
-        const float2 sum = f2_split(fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3])));
-        l += sum.x + sum.y;
-        tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[g & 1]);
       }
+      const long long row0 = s.qs + it.tile * XA_BM + quarter * 32;
+      const long long at = ((long long)it.part * p.heads + it.h) * p.total_q + row0;  // one part: of lse itself
+      float* lse = half ? nullptr : p.parts > 1 ? p.part_lse + at : p.lse ? p.lse + at : nullptr;
+      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + row0 * p.ldo + it.h * D + half * (D / 2);
+      if (T == 0) {
+        if (lane < rows) {
+          if (p.parts == 1) zero_row16<D / 2>(dst + lane * p.ldo);  // else a part of weight zero: its output is not read
+          if (lse) lse[lane] = NEG_INF;
+        }
+        continue;
+      }
+      if (rows > 0) {
+        float* x = sh_l + quarter * 32 + lane;
+        x[half * XA_BM] = l;
+        pair_sync(quarter);
+        l += x[(1 - half) * XA_BM];
+      }
       if (!mbar_wait(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 112)) bad = true;
       tc_fence_after();
-      const bool store = row_ok && !bad && !*abort_flag;
+      const int put = bad || *abort_flag ? 0 : rows;
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      if (p.parts > 1)
-        store_row32<D>(t_o, inv, store, p.part_o + at * D);
-      else
-        store_row16<D>(t_o, inv, p.f16, store, dst);
+      if (rows > 0) {
+        if (p.parts > 1)
+          store_rows32<D / 2>(t_o, inv, true, lane < put, p.part_o + (at + lane) * D + half * (D / 2));
+        else
+          store_rows16<D / 2>(t_o, inv, true, F16, stage + warp * XA_STAGE, lane, put, dst, p.ldo);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_empty);
-      if (store && lse) *lse = l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : NEG_INF;
+      if (lane < put && lse) lse[lane] = l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : NEG_INF;
     }
   }
   tc_fence_before();
@@ -406,52 +509,63 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
 // ------------------------------------------------------------------------------------------------ dQ
 // The forward's walk again: a CTA holds Q and dO of a query tile, walks the keys, recomputes P from the stored lse
 // and accumulates dQ in TMEM. It also forms delta = rowsum(dO * O), which the dK / dV kernel reads, so O and dO are
-// read once here and delta needs no launch of its own. TMEM (256 columns): S, dP, dQ; dS (packed pairs) gets columns
-// of its own where they fit (D = 64), so that S and dP of the next tile are multiplied while this one's dS is
-// formed; at D = 128 it lies over S.
+// read once here and delta needs no launch of its own. TMEM (256 columns): S, dP, dQ, and dS (packed pairs) in two
+// buffers of its own where they fit (D = 64); at D = 128 dS lies over dP. S of the next tile is multiplied as soon as
+// the softmax has read this one's, dP with it at D = 64, and after this tile's dS K at D = 128.
 template <int D>
 struct XDq {
   static constexpr int SUBS = D / 64;
   static constexpr bool SEP = D == 64;
-  static constexpr int QS = SEP ? 2 : 1, KS = SEP ? 2 : 1;
+  static constexpr int QS = SEP ? 2 : 1, KS = 2, VS = SEP ? 2 : 1;
   static constexpr int Q_BYTES = SUBS * XA_SUB_M, T_BYTES = SUBS * XA_SUB_N;
-  static constexpr int TILES = 2 * QS * Q_BYTES + 2 * KS * T_BYTES;
-  static constexpr int SMEM = TILES + 1024 + 512;
-  static constexpr int COL_DQ = 128, COL_DS = SEP ? 192 : 0;
+  static constexpr int TILES = 2 * QS * Q_BYTES + (KS + VS) * T_BYTES;
+  // at D = 128 there is no room to stage the stores
+  static constexpr int STAGE = SEP ? XA_SOFTMAX * XA_STAGE : 0;
+  static constexpr int SMEM = TILES + STAGE + XA_BM * 4 + 256;
+  static constexpr int COL_DQ = 128, COL_DS = SEP ? 192 : 64;
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
-template <int D>
+template <int D, bool F16>
 __global__ void __launch_bounds__(XA_THREADS, 2)
     cross_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const XParams p,
                     const XGrad gr, int num_items, int qtiles) {
   using C = XDq<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw;
+  if (smem_u32(smem_raw) & 1023) {
+    // dynamic shared memory starts on a 1024-byte boundary when there is no static one; the swizzled tiles need that
+    if (threadIdx.x == 0) record_error(SA3_DEVERR_TIMEOUT, 119);
+    return;
+  }
   auto sQ = [&](int s) { return smem + s * C::Q_BYTES; };
   auto sDO = [&](int s) { return smem + (C::QS + s) * C::Q_BYTES; };
   auto sK = [&](int s) { return smem + 2 * C::QS * C::Q_BYTES + s * C::T_BYTES; };
   auto sV = [&](int s) { return smem + 2 * C::QS * C::Q_BYTES + (C::KS + s) * C::T_BYTES; };
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::TILES);
+  uint8_t* stage = smem + C::TILES;                                   // XA_STAGE bytes a softmax warp
+  float* sh_delta = reinterpret_cast<float*>(stage + C::STAGE);       // [rows] of the item
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sh_delta + XA_BM);
   uint64_t* q_full = bars;          // [QS] Q and dO
   uint64_t* q_empty = bars + 2;     // [QS]
   uint64_t* k_full = bars + 4;      // [KS]
   uint64_t* k_empty = bars + 6;     // [KS]
-  uint64_t* v_full = bars + 8;      // [KS]
-  uint64_t* v_empty = bars + 10;    // [KS]
+  uint64_t* v_full = bars + 8;      // [VS]
+  uint64_t* v_empty = bars + 10;    // [VS]
   uint64_t* sdp_full = bars + 12;   // S and dP of a tile are in TMEM
-  uint64_t* sdp_empty = bars + 13;  // the softmax holds them in registers (4 arrivals)
-  uint64_t* ds_full = bars + 14;    // dS is in TMEM (4 arrivals)
-  uint64_t* dq_full = bars + 15;    // one phase per dS K
-  uint64_t* dq_empty = bars + 16;   // the softmax has read an item's dQ (4 arrivals)
-  uint64_t* done = bars + 17;
-  constexpr int NBARS = 18;
+  uint64_t* sdp_empty = bars + 13;  // the softmax holds them in registers (XA_SOFTMAX arrivals)
+  uint64_t* ds_full = bars + 14;    // [2] dS is in TMEM (XA_SOFTMAX arrivals)
+  uint64_t* dq_full = bars + 16;    // [2] dS K of a tile is done
+  uint64_t* dq_empty = bars + 18;   // the softmax has read an item's dQ (XA_SOFTMAX arrivals)
+  uint64_t* done = bars + 19;       // [2]
+  constexpr int NBARS = 21;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert(NBARS * 8 + 8 <= 256, "barriers");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < NBARS; ++i) mbar_init(&bars[i], (i == 13 || i == 14 || i == 16) ? 4 : 1);
+    for (int i = 0; i < NBARS; ++i) mbar_init(&bars[i], (i == 13 || i == 14 || i == 15 || i == 18) ? XA_SOFTMAX : 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -469,203 +583,236 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
   const uint32_t tmem = *tmem_slot;
   grid_dep_wait();
 
-  if (warp == 4) {
+  if (warp >= XA_SOFTMAX) regs_low();
+  if (warp == 8) {
     if (lane == 0) {
       int g = 0, qc = 0;
       bool ok = true, v_out = true;  // v_out: V of the last counted tile was issued
-      for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
-        const int tile = item % qtiles, rest = item / qtiles;
-        const int h = rest % p.heads, b = rest / p.heads;
-        const XSeq s = make_seq(p, b);
-        const int T = tile * XA_BM < s.lq ? (s.seen + XA_BN - 1) / XA_BN : 0;
-        if (T == 0) continue;
-        const int cq = h * D, ck = (h / p.group) * D;
+      for (XWalk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+        if (it.T == 0) continue;
+        const XSeq& s = it.s;
+        const int cq = it.h * D, ck = (it.h / p.group) * D;
         const int qs = qc % C::QS;
         if (qc >= C::QS && !mbar_wait(&q_empty[qs], ((qc / C::QS) - 1) & 1, abort_flag, 120)) break;
         mbar_arrive_expect_tx(&q_full[qs], 2 * C::Q_BYTES);
         for (int c = 0; c < C::SUBS; ++c) {
-          tma_load_2d(sQ(qs) + c * XA_SUB_M, &tmQ, &q_full[qs], cq + 64 * c, s.qs + tile * XA_BM);
-          tma_load_2d(sDO(qs) + c * XA_SUB_M, &tmDO, &q_full[qs], cq + 64 * c, s.qs + tile * XA_BM);
+          tma_load_2d(sQ(qs) + c * XA_SUB_M, &tmQ, &q_full[qs], cq + 64 * c, s.qs + it.tile * XA_BM);
+          tma_load_2d(sDO(qs) + c * XA_SUB_M, &tmDO, &q_full[qs], cq + 64 * c, s.qs + it.tile * XA_BM);
         }
         qc++;
-        for (int t = 0; t < T; ++t, ++g) {
-          const int ks = g % C::KS;
-          if (g >= C::KS && !mbar_wait(&v_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 121)) {
+        for (int t = 0; t < it.T; ++t, ++g) {
+          const int ks = g % C::KS, vs = g % C::VS, row = s.ks + t * XA_BN;
+          if (g >= C::KS && !mbar_wait(&k_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 121)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&v_full[ks], C::T_BYTES);
-          for (int c = 0; c < C::SUBS; ++c)
-            tma_load_2d(sV(ks) + c * XA_SUB_N, &tmV, &v_full[ks], ck + 64 * c, s.ks + t * XA_BN);
-          if (g >= C::KS && !mbar_wait(&k_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 122)) {
+          mbar_arrive_expect_tx(&k_full[ks], C::T_BYTES);
+          for (int c = 0; c < C::SUBS; ++c) tma_load_2d(sK(ks) + c * XA_SUB_N, &tmK, &k_full[ks], ck + 64 * c, row);
+          if (g >= C::VS && !mbar_wait(&v_empty[vs], ((g / C::VS) - 1) & 1, abort_flag, 122)) {
             g++;
             ok = v_out = false;
             break;
           }
-          mbar_arrive_expect_tx(&k_full[ks], C::T_BYTES);
-          for (int c = 0; c < C::SUBS; ++c)
-            tma_load_2d(sK(ks) + c * XA_SUB_N, &tmK, &k_full[ks], ck + 64 * c, s.ks + t * XA_BN);
+          mbar_arrive_expect_tx(&v_full[vs], C::T_BYTES);
+          for (int c = 0; c < C::SUBS; ++c) tma_load_2d(sV(vs) + c * XA_SUB_N, &tmV, &v_full[vs], ck + 64 * c, row);
         }
       }
       if (*abort_flag) {
         volatile int never = 0;
         for (int c = max(qc - C::QS, 0); c < qc; ++c) mbar_wait(&q_full[c % C::QS], (c / C::QS) & 1, &never, 123);
-        for (int c = max(g - C::KS, 0); c < g; ++c) {
-          mbar_wait(&v_full[c % C::KS], (c / C::KS) & 1, &never, 123);
-          if (c + 1 < g || v_out) mbar_wait(&k_full[c % C::KS], (c / C::KS) & 1, &never, 123);
-        }
+        for (int c = max(g - C::KS, 0); c < g; ++c) mbar_wait(&k_full[c % C::KS], (c / C::KS) & 1, &never, 123);
+        const int gv = v_out ? g : g - 1;
+        for (int c = max(gv - C::VS, 0); c < gv; ++c) mbar_wait(&v_full[c % C::VS], (c / C::VS) & 1, &never, 123);
       }
     }
-  } else if (warp == 5) {
-    const int fmt = p.f16 ? 0 : 1;
+  } else if (warp == 9) {
+    // S = Q K^T and dP = dO V^T
+    const int fmt = F16 ? 0 : 1;
     const uint32_t base = smem_u32(smem);
-    const uint64_t dk = sdesc_kmajor_sw128(base), dm = sdesc_mnmajor_sw128(base, XA_SUB_N);
+    const uint64_t dk = sdesc_kmajor_sw128(base);
     const uint32_t k_hi = (uint32_t)(dk >> 32), k_lo = (uint32_t)dk;
-    const uint32_t m_hi = (uint32_t)(dm >> 32), m_lo = (uint32_t)dm;
-    const uint32_t idesc_q = make_idesc(128, D, fmt, fmt, 0, 1);
-    auto off16 = [&](const uint8_t* x) { return (smem_u32(x) - base) >> 4; };
+    const uint32_t idesc_full = make_idesc(128, XA_BN, fmt, fmt, 0, 0);
     int g = 0, qc = 0;
     bool ok = true;
-    for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
-      const int tile = item % qtiles, rest = item / qtiles;
-      const int b = rest / p.heads;
-      const XSeq s = make_seq(p, b);
-      const int T = tile * XA_BM < s.lq ? (s.seen + XA_BN - 1) / XA_BN : 0;
-      if (T == 0) continue;
+    for (XWalk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+      if (it.T == 0) continue;
       const int qs = qc % C::QS;
+      const uint32_t qlo = k_lo + ((qs * C::Q_BYTES) >> 4), dlo = k_lo + (((C::QS + qs) * C::Q_BYTES) >> 4);
       ok = warp_wait(&q_full[qs], (qc / C::QS) & 1, abort_flag, 124);
-      // S = Q K^T and dP = dO V^T of tile t, which is tile n of the walk
-      auto products = [&](int t, int n) {
-        const int ks = n % C::KS;
-        const int keys = min(XA_BN, s.seen - t * XA_BN), cols = (keys + 15) & ~15;
-        const uint64_t vis = visible64(p, s, t * XA_BN, lane);
-        if (!warp_wait(&k_full[ks], (n / C::KS) & 1, abort_flag, 125) ||
-            !warp_wait(&v_full[ks], (n / C::KS) & 1, abort_flag, 125))
-          return false;
-        const uint64_t all = cols == 64 ? ~0ull : (1ull << cols) - 1;
-        if ((vis & all) != all) zero_rows(sK(ks), C::SUBS, cols, vis, lane);  // dS K multiplies them by zero
-        tc_fence_after();
-        const uint32_t idesc = make_idesc(128, cols, fmt, fmt, 0, 0);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t alo = k_lo + off16(half ? sDO(qs) : sQ(qs)), blo = k_lo + off16(half ? sV(ks) : sK(ks));
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            mma_ss_lo(tmem + 64 * half, alo + (k >> 2) * (XA_SUB_M >> 4) + 2 * (k & 3),
-                      blo + (k >> 2) * (XA_SUB_N >> 4) + 2 * (k & 3), k_hi, idesc, k != 0);
+      for (int t = 0; t < it.T && ok; ++t, ++g) {
+        const int ks = g % C::KS, vs = g % C::VS, left = it.s.seen - t * XA_BN;
+        ok = warp_wait(&k_full[ks], (g / C::KS) & 1, abort_flag, 125);
+        if (!ok) break;
+        const int cols = min(XA_BN, (left + 15) & ~15);
+        if (p.key_mask || left < XA_BN) {
+          const uint64_t vis = visible64(p, it.s, t * XA_BN, lane), all = low_bits64(cols);
+          if ((vis & all) != all) zero_rows(sK(ks), C::SUBS, cols, vis, lane);  // dS K multiplies them by zero
         }
-        commit_elect(sdp_full);
-        commit_elect(&v_empty[ks]);
-        if (t == T - 1) commit_elect(&q_empty[qs]);
-        return true;
-      };
-      // S and dP of the last item's last tile: their readers are done once its dS was written
-      ok = ok && products(0, g);
-      for (int t = 0; t < T && ok; ++t, ++g) {
-        if (C::SEP && t + 1 < T)
-          ok = warp_wait(sdp_empty, g & 1, abort_flag, 126) && products(t + 1, g + 1);
-        ok = ok && warp_wait(ds_full, g & 1, abort_flag, 127) &&
-             (t > 0 || qc == 0 || warp_wait(dq_empty, (qc - 1) & 1, abort_flag, 128));
+        ok = g == 0 || warp_wait(sdp_empty, (g - 1) & 1, abort_flag, 126);
         if (!ok) break;
         tc_fence_after();
-        const int ks = g % C::KS, steps = (min(XA_BN, s.seen - t * XA_BN) + 15) >> 4;
-        const uint32_t mlo = m_lo + off16(sK(ks));
-        for (int k = 0; k < steps; ++k)
-          mma_ts_lo(tmem + C::COL_DQ, tmem + C::COL_DS + 8 * k, mlo + k * (2048 >> 4), m_hi, idesc_q,
-                    (t > 0 || k > 0) ? 1u : 0u);
-        commit_elect(dq_full);
-        commit_elect(&k_empty[ks]);
-        if (!C::SEP && t + 1 < T) ok = products(t + 1, g + 1);
+        const uint32_t idesc = left >= XA_BN ? idesc_full : make_idesc(128, cols, fmt, fmt, 0, 0);
+        const uint32_t klo = k_lo + ((2 * C::QS * C::Q_BYTES + ks * C::T_BYTES) >> 4);
+        const uint32_t vlo = k_lo + ((2 * C::QS * C::Q_BYTES + (C::KS + vs) * C::T_BYTES) >> 4);
+#pragma unroll
+        for (int c = 0; c < C::SUBS; ++c)
+          mma4_ss(tmem, qlo + c * (XA_SUB_M >> 4), klo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
+        ok = warp_wait(&v_full[vs], (g / C::VS) & 1, abort_flag, 125) &&
+             (C::SEP || g == 0 || warp_wait(&dq_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 125));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < C::SUBS; ++c)
+          mma4_ss(tmem + 64, dlo + c * (XA_SUB_M >> 4), vlo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
+        commit2_elect(sdp_full, &v_empty[vs]);
+        if (t == it.T - 1) commit_elect(&q_empty[qs]);
       }
       qc++;
     }
-    commit_elect(done);
+    commit_elect(&done[0]);
     volatile int never = 0;
-    warp_wait(done, 0, &never, 129);
-  } else {
-    const int r = warp * 32 + lane;
-    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
-    const uint32_t t_s = tmem + lane_off, t_ds = t_s + C::COL_DS, t_dq = t_s + C::COL_DQ;
+    warp_wait(&done[0], 0, &never, 129);
+  } else if (warp == 10) {
+    // dQ (+)= dS K
+    const int fmt = F16 ? 0 : 1;
+    const uint64_t dm = sdesc_mnmajor_sw128(smem_u32(sK(0)), XA_SUB_N);
+    const uint32_t m_hi = (uint32_t)(dm >> 32), m_lo = (uint32_t)dm;
+    const uint32_t idesc = make_idesc(128, D, fmt, fmt, 0, 1);
+    const uint32_t t_dq = tmem + C::COL_DQ;
+    int g = 0, qc = 0;
+    bool ok = true;
+    for (XWalk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+      if (it.T == 0) continue;
+      ok = qc == 0 || warp_wait(dq_empty, (qc - 1) & 1, abort_flag, 128);
+      for (int t = 0; t < it.T && ok; ++t, ++g) {
+        const int ks = g % C::KS;
+        ok = warp_wait(&ds_full[g & 1], (g >> 1) & 1, abort_flag, 127);
+        if (!ok) break;
+        tc_fence_after();
+        const int steps = min(XA_BN / 16, (it.s.seen - t * XA_BN + 15) >> 4);
+        const uint32_t mlo = m_lo + ((ks * C::T_BYTES) >> 4);
+        const uint32_t t_ds = tmem + C::COL_DS + (C::SEP ? 32 * (g & 1) : 0);
+        if (steps == XA_BN / 16) {
+          mma4_ts(t_dq, t_ds, t_ds + (C::SEP ? 16 : 32), mlo, m_hi, idesc, t > 0);
+        } else {
+          for (int k = 0; k < steps; ++k)
+            mma_ts_lo(t_dq, t_ds + (C::SEP ? 16 : 32) * (k >> 1) + 8 * (k & 1), mlo + k * (2048 >> 4), m_hi, idesc, (t > 0 || k > 0) ? 1u : 0u);
+        }
+        commit2_elect(&dq_full[g & 1], &k_empty[ks]);
+      }
+      qc++;
+    }
+    commit_elect(&done[1]);
+    volatile int never = 0;
+    warp_wait(&done[1], 0, &never, 129);
+  } else if (warp < XA_SOFTMAX) {
+    regs_high();
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t t_s = tmem + lane_off + 32 * half, t_dq = tmem + lane_off + C::COL_DQ + half * (D / 2);
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
     int g = 0;
-    for (int item = blockIdx.x; item < num_items; item += gridDim.x) {
-      const int tile = item % qtiles, rest = item / qtiles;
-      const int h = rest % p.heads, b = rest / p.heads;
-      const XSeq s = make_seq(p, b);
-      if (tile * XA_BM >= s.lq) continue;
-      const int T = (s.seen + XA_BN - 1) / XA_BN;
-      const int i = tile * XA_BM + r;
-      const bool row_ok = i < s.lq;
-      const long long row = s.qs + i;
-      float delta = 0.f, lse = -INFINITY;
-      if (row_ok) {
-        const uint4* po = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.out) + row * p.ldo + h * D);
-        const uint4* pd =
-            reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(gr.dout) + row * gr.lddo + h * D);
-        lse = __ldg(p.lse + (long long)h * p.total_q + row);
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (XWalk it(p, qtiles, num_items); it.item < num_items; it.next(p, num_items)) {
+      const XSeq& s = it.s;
+      if (it.tile * XA_BM >= s.lq) continue;
+      const int h = it.h, T = it.T;
+      const int rows = min(32, s.lq - it.tile * XA_BM - quarter * 32);  // of this warp that exist
+      const long long row0 = s.qs + it.tile * XA_BM + quarter * 32;
+      const long long stat = (long long)h * p.total_q + row0;
+      float lse = -INFINITY;
+      if (lane < rows) lse = __ldg(p.lse + stat + lane);
+      {
+        // delta: this warp's 16 of the pair's 32 rows, D / 8 lanes a row, 16 bytes each
+        constexpr int LPR = D / 8, RPI = 32 / LPR;
+        const int c = lane % LPR, first = 16 * half + lane / LPR;
+        const uint16_t* po = reinterpret_cast<const uint16_t*>(p.out) + (row0 + first) * p.ldo + h * D + 8 * c;
+        const uint16_t* pd = reinterpret_cast<const uint16_t*>(gr.dout) + (row0 + first) * gr.lddo + h * D + 8 * c;
+#pragma unroll 1
+        for (int n = 0; n < 16; n += 4 * RPI) {
+          uint4 o4[4], d4[4];
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 a = __ldg(po + c), d = __ldg(pd + c);
-          const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, dw[4] = {d.x, d.y, d.z, d.w};
+          for (int e = 0; e < 4; ++e) {
+            const int r = n + e * RPI;
+            o4[e] = d4[e] = make_uint4(0, 0, 0, 0);
+            if (first + r < rows) {
+              o4[e] = __ldg(reinterpret_cast<const uint4*>(po + r * p.ldo));
+              d4[e] = __ldg(reinterpret_cast<const uint4*>(pd + r * gr.lddo));
+            }
+          }
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            acc[e] = fmaf(unpack_hi(aw[e], p.f16), unpack_hi(dw[e], p.f16),
-                          fmaf(unpack_lo(aw[e], p.f16), unpack_lo(dw[e], p.f16), acc[e]));
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t ow[4] = {o4[e].x, o4[e].y, o4[e].z, o4[e].w}, dw[4] = {d4[e].x, d4[e].y, d4[e].z, d4[e].w};
+            float sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              sum = fmaf(unpack_hi(ow[x], F16), unpack_hi(dw[x], F16),
+                         fmaf(unpack_lo(ow[x], F16), unpack_lo(dw[x], F16), sum));
+#pragma unroll
+            for (int x = LPR / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            if (c == 0) sh_delta[quarter * 32 + n + e * RPI + first] = sum;
+          }
         }
-        delta = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-        gr.delta[(long long)h * p.total_q + row] = delta;
       }
-      uint16_t* dst = reinterpret_cast<uint16_t*>(gr.dq) + row * gr.lddq + h * D;
+      pair_sync(quarter);
+      const float delta = sh_delta[quarter * 32 + lane];
+      pair_sync(quarter);  // both have read it before the next item's is written
+      if (half == 0 && lane < rows) gr.delta[stat + lane] = delta;
+      uint16_t* dst = reinterpret_cast<uint16_t*>(gr.dq) + row0 * gr.lddq + h * D + half * (D / 2);
       if (T == 0) {
-        if (row_ok) zero_row16<D>(dst);
+        if (lane < rows) zero_row16<D / 2>(dst + lane * gr.lddq);
         continue;
       }
       // a row that saw no key has lse = -inf: with +inf instead its probabilities come out as zero
       const float l2 = lse == -INFINITY ? INFINITY : lse * XA_LOG2E;
       const uint64_t negl2 = f2(-l2, -l2), negd2 = f2(-delta, -delta);
       bool bad = false;
-      for (int t = 0; t < T; ++t, ++g) {
-        const uint64_t vis = visible64(p, s, t * XA_BN, lane);
+      int left = s.seen;
+      for (int t = 0; t < T; ++t, ++g, left -= XA_BN) {
+        uint32_t vis = (uint32_t)(low_bits64(left) >> (32 * half));
+        if (p.key_mask) vis = (uint32_t)(visible64(p, s, t * XA_BN, lane) >> (32 * half));
+        const uint32_t t_ds = tmem + lane_off + C::COL_DS + (C::SEP ? 32 * (g & 1) + 16 * half : 32 * half);
         if (!mbar_wait(sdp_full, g & 1, abort_flag, 130)) bad = true;
+        // the dS that last lay in this tile's columns has been multiplied (D = 128: dP was multiplied after it)
+        if (C::SEP && g > 1 && !mbar_wait(&dq_full[g & 1], ((g - 2) >> 1) & 1, abort_flag, 131)) bad = true;
         tc_fence_after();
-        uint32_t w[2][16];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t sc[32], dp[32];
-          tmem_ld32_async(t_s + 32 * c, sc);
-          tmem_ld32_async(t_s + 64 + 32 * c, dp);
+        if (rows > 0 && left > 32 * half) {  // else no row of this warp exists, or no column: nothing of it is used
+          uint32_t sc[32], dp[32], w[16];
+          tmem_ld32_async(t_s, sc);
+          tmem_ld32_async(t_s + 64, dp);
           tmem_wait_ld();
-          if (c == 1 && C::SEP) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(sdp_empty);
-          }
-          const uint32_t v = (uint32_t)(vis >> (32 * c));
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sdp_empty);
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float2 x = f2_split(ffma2(f2(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), scale2, negl2));
             const uint64_t pr = f2(fast_exp2(x.x), fast_exp2(x.y));
-            float2 d = f2_split(fmul2(pr, fadd2(f2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), negd2)));
-            if (v != 0xffffffffu) {
-              d.x = (v >> e) & 1u ? d.x : 0.f;
-              d.y = (v >> (e + 1)) & 1u ? d.y : 0.f;
-            }
-            w[c][e >> 1] = pack_2(d.x, d.y, p.f16);
+            const float2 d = f2_split(fmul2(pr, fadd2(f2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), negd2)));
+            w[e >> 1] = pack_2(d.x, d.y, F16);
           }
+          if (vis != 0xffffffffu) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              w[e] &= ((vis >> (2 * e)) & 1u ? 0x0000ffffu : 0u) | ((vis >> (2 * e + 1)) & 1u ? 0xffff0000u : 0u);
+          }
+          tmem_st16(t_ds, w);
+          tmem_wait_st();
+        } else if (lane == 0) {
+          mbar_arrive(sdp_empty);
         }
-        // dS of the last tile must have been multiplied before its columns are written again
-        if (C::SEP && g > 0 && !mbar_wait(dq_full, (g - 1) & 1, abort_flag, 131)) bad = true;
-        tmem_st16(t_ds, w[0]);
-        tmem_st16(t_ds + 16, w[1]);
-        tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(ds_full);
+        if (lane == 0) mbar_arrive(&ds_full[g & 1]);
       }
-      if (!mbar_wait(dq_full, (g - 1) & 1, abort_flag, 132)) bad = true;
+      if (!mbar_wait(&dq_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 132)) bad = true;
       tc_fence_after();
-      store_row16<D>(t_dq, p.scale, p.f16, row_ok && !bad && !*abort_flag, dst);
+      const int put = bad || *abort_flag ? 0 : rows;
+      if (rows > 0) {
+        if (C::SEP)
+          store_rows16<D / 2>(t_dq, p.scale, true, F16, stage + warp * XA_STAGE, lane, put, dst, gr.lddq);
+        else
+          store_row16<D / 2>(t_dq, p.scale, F16, lane < put, dst + lane * gr.lddq);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dq_empty);
@@ -684,7 +831,8 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
 // dV += P^T dO and dK += dS^T Q, with dO and Q read as they lie. Two score buffers, each with a softmax warpgroup of
 // its own: one forms P and dS while the tensor core works on the other. TMEM (512 columns): 2 x (S^T 64, dP^T 64),
 // dV, dK.
-constexpr int XB_THREADS = 320;  // warps 0..7 softmax, 8 loads, 9 MMA
+constexpr int XB_THREADS = 608;  // warps 0..15 softmax (8 to a score buffer, two to a row), 16 loads, 17 and 18 MMA
+constexpr int XB_SOFTMAX = 8;
 template <int D>
 struct XDkv {
   static constexpr int SUBS = D / 64;
@@ -692,11 +840,11 @@ struct XDkv {
   static constexpr int K_BYTES = SUBS * XA_SUB_M, T_BYTES = SUBS * XA_SUB_N;
   static constexpr int TILES = 2 * K_BYTES + STAGES * 2 * T_BYTES;
   static constexpr int STATS = STAGES * 2 * XA_BN * 4;
-  static constexpr int SMEM = TILES + STATS + 1024 + 512;
+  static constexpr int SMEM = TILES + STATS + 1024 + 512;  // the stores go through the tiles of Q and dO
   static constexpr int COL_DV = 256, COL_DK = 256 + D;
 };
 
-template <int D>
+template <int D, bool F16>
 __global__ void __launch_bounds__(XB_THREADS, 1)
     cross_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const XParams p,
@@ -714,15 +862,17 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
   uint64_t* full = bars + 1;      // [STAGES]
   uint64_t* empty = bars + 5;     // [STAGES]
   uint64_t* sdp_full = bars + 9;  // [2]
-  uint64_t* ds_full = bars + 11;  // [2] 4 arrivals
-  uint64_t* done = bars + 13;
-  constexpr int NBARS = 14;
+  uint64_t* ds_full = bars + 11;  // [2] XB_SOFTMAX arrivals
+  uint64_t* used = bars + 13;     // [2] P and dS of a buffer have been multiplied
+  uint64_t* done = bars + 15;     // [2]
+  constexpr int NBARS = 17;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+  static_assert(2 * XB_SOFTMAX * XA_STAGE <= C::STAGES * 2 * C::T_BYTES, "room for the stores");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < NBARS; ++i) mbar_init(&bars[i], (i == 11 || i == 12) ? 4 : 1);
+    for (int i = 0; i < NBARS; ++i) mbar_init(&bars[i], (i == 11 || i == 12) ? XB_SOFTMAX : 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -752,7 +902,7 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
   const int t1 = j0 < s.seen ? (int)(steps_all * (part + 1) / splits) : t0;  // hidden keys get zeros
   const int T = j0 < s.lk ? t1 - t0 : 0;
 
-  if (warp == 8) {
+  if (warp == 16) {
     if (T > 0) {
       if (lane == 0) {
         mbar_arrive_expect_tx(kv_full, 2 * C::K_BYTES);
@@ -801,83 +951,88 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
         for (int c = max(t - C::STAGES, 0); c < t; ++c) mbar_wait(&full[c % C::STAGES], (c / C::STAGES) & 1, &never, 141);
       }
     }
-  } else if (warp == 9) {
-    const int fmt = p.f16 ? 0 : 1;
-    const uint32_t base = smem_u32(smem);
-    const uint64_t dk = sdesc_kmajor_sw128(base), dm = sdesc_mnmajor_sw128(base, XA_SUB_N);
-    const uint32_t k_hi = (uint32_t)(dk >> 32), k_lo = (uint32_t)dk;
-    const uint32_t m_hi = (uint32_t)(dm >> 32), m_lo = (uint32_t)dm;
-    const uint32_t idesc_s = make_idesc(128, XA_BN, fmt, fmt, 0, 0), idesc_g = make_idesc(128, D, fmt, fmt, 0, 1);
-    auto off16 = [&](const uint8_t* x) { return (smem_u32(x) - base) >> 4; };
+  } else if (warp == 17) {
+    // S^T = K Q^T and dP^T = V dO^T
+    const int fmt = F16 ? 0 : 1;
+    const uint64_t dk = sdesc_kmajor_sw128(smem_u32(smem));
+    const uint32_t k_hi = (uint32_t)(dk >> 32), k_lo = (uint32_t)dk, v_lo = k_lo + (C::K_BYTES >> 4);
+    const uint32_t idesc = make_idesc(128, XA_BN, fmt, fmt, 0, 0);
     bool ok = T > 0 && warp_wait(kv_full, 0, abort_flag, 142);
-    auto products = [&](int t) {
+    int i0 = T > 0 ? (t0 % qtiles) * XA_BN : 0;  // first row of the tile in its sequence
+    for (int t = 0; t < T && ok; ++t) {
       const int st = t % C::STAGES;
-      if (!warp_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 143)) return false;
-      const int rows = s.lq - ((t0 + t) % qtiles) * XA_BN;
+      ok = warp_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 143) &&
+           (t < 2 || warp_wait(&used[t & 1], ((t - 2) >> 1) & 1, abort_flag, 143));
+      if (!ok) break;
+      const int rows = s.lq - i0;
       if (rows < XA_BN) {
         // rows behind the end: dV and dK multiply them by zero probabilities
-        zero_rows(sQ(st), C::SUBS, XA_BN, (1ull << rows) - 1, lane);
-        zero_rows(sDO(st), C::SUBS, XA_BN, (1ull << rows) - 1, lane);
+        zero_rows(sQ(st), C::SUBS, XA_BN, low_bits64(rows), lane);
+        zero_rows(sDO(st), C::SUBS, XA_BN, low_bits64(rows), lane);
       }
+      i0 = rows > XA_BN ? i0 + XA_BN : 0;
       tc_fence_after();
+      const uint32_t qlo = k_lo + ((2 * C::K_BYTES + 2 * st * C::T_BYTES) >> 4), dlo = qlo + (C::T_BYTES >> 4);
+      const uint32_t t_s = tmem + 128 * (t & 1);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t alo = k_lo + off16(half ? sV : sK), blo = k_lo + off16(half ? sDO(st) : sQ(st));
+      for (int c = 0; c < C::SUBS; ++c)
+        mma4_ss(t_s, k_lo + c * (XA_SUB_M >> 4), qlo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          mma_ss_lo(tmem + 128 * (t & 1) + 64 * half, alo + (k >> 2) * (XA_SUB_M >> 4) + 2 * (k & 3),
-                    blo + (k >> 2) * (XA_SUB_N >> 4) + 2 * (k & 3), k_hi, idesc_s, k != 0);
-      }
+      for (int c = 0; c < C::SUBS; ++c)
+        mma4_ss(t_s + 64, v_lo + c * (XA_SUB_M >> 4), dlo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
       commit_elect(&sdp_full[t & 1]);
-      return true;
-    };
-    ok = ok && products(0) && (T < 2 || products(1));
+    }
+    commit_elect(&done[0]);
+    volatile int never = 0;
+    warp_wait(&done[0], 0, &never, 145);
+  } else if (warp == 18) {
+    // dV += P^T dO, dK += dS^T Q
+    const int fmt = F16 ? 0 : 1;
+    const uint64_t dm = sdesc_mnmajor_sw128(smem_u32(sQ(0)), XA_SUB_N);
+    const uint32_t m_hi = (uint32_t)(dm >> 32), m_lo = (uint32_t)dm;
+    const uint32_t idesc = make_idesc(128, D, fmt, fmt, 0, 1);
+    bool ok = true;
     for (int t = 0; t < T && ok; ++t) {
       ok = warp_wait(&ds_full[t & 1], (t >> 1) & 1, abort_flag, 144);
       if (!ok) break;
       tc_fence_after();
       const int st = t % C::STAGES;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t mlo = m_lo + off16(half ? sQ(st) : sDO(st));
-#pragma unroll
-        for (int k = 0; k < XA_BN / 16; ++k)
-          mma_ts_lo(tmem + (half ? C::COL_DK : C::COL_DV), tmem + 128 * (t & 1) + 64 * half + 8 * k,
-                    mlo + k * (2048 >> 4), m_hi, idesc_g, (t > 0 || k > 0) ? 1u : 0u);
-      }
-      commit_elect(&empty[st]);
-      if (t + 2 < T) ok = products(t + 2);
+      const uint32_t qlo = m_lo + ((2 * st * C::T_BYTES) >> 4), dlo = qlo + (C::T_BYTES >> 4);
+      const uint32_t t_s = tmem + 128 * (t & 1);
+      mma4_ts(tmem + C::COL_DV, t_s, t_s + 32, dlo, m_hi, idesc, t > 0);
+      mma4_ts(tmem + C::COL_DK, t_s + 64, t_s + 96, qlo, m_hi, idesc, t > 0);
+      commit2_elect(&empty[st], &used[t & 1]);
     }
-    commit_elect(done);
+    commit_elect(&done[1]);
     volatile int never = 0;
-    warp_wait(done, 0, &never, 145);
+    warp_wait(&done[1], 0, &never, 145);
   } else {
-    const int grp = warp >> 2;
-    const int r = (warp & 3) * 32 + lane;
-    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lane_off + 128 * grp;
+    const int grp = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t t_s = tmem + lane_off + 128 * grp + 32 * half;
     const int j = j0 + r;
     const long long row = s.ks + j;
     bool vis = j < s.seen;
     if (vis && p.key_mask) vis = __ldg(p.key_mask + row) != 0;
+    const bool some = __any_sync(0xffffffffu, vis);  // else the rows of this warp are not stored, or stored as zeros
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
     bool bad = false;
     for (int t = grp; t < T; t += 2) {
       const int st = t % C::STAGES;
-      const float* sp = stats + st * 2 * XA_BN;
+      const float* sp = stats + st * 2 * XA_BN + 32 * half;
       if (!mbar_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 146)) bad = true;
       if (!mbar_wait(&sdp_full[grp], (t >> 1) & 1, abort_flag, 147)) bad = true;
       tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      if (some) {
         uint32_t sc[32], dp[32], wp[16], wd[16];
-        tmem_ld32_async(t_s + 32 * c, sc);
-        tmem_ld32_async(t_s + 64 + 32 * c, dp);
+        tmem_ld32_async(t_s, sc);
+        tmem_ld32_async(t_s + 64, dp);
         tmem_wait_ld();
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-          const float4 l4 = *reinterpret_cast<const float4*>(sp + 32 * c + e);
-          const float4 d4 = *reinterpret_cast<const float4*>(sp + XA_BN + 32 * c + e);
+          const float4 l4 = *reinterpret_cast<const float4*>(sp + e);
+          const float4 d4 = *reinterpret_cast<const float4*>(sp + XA_BN + e);
 #pragma unroll
           for (int f = 0; f < 4; f += 2) {
             const uint64_t nl = f ? f2(l4.z, l4.w) : f2(l4.x, l4.y), nd = f ? f2(d4.z, d4.w) : f2(d4.x, d4.y);
@@ -886,38 +1041,40 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
             const float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
             const float2 d = f2_split(
                 fmul2(f2(p0, p1), fadd2(f2(__uint_as_float(dp[e + f]), __uint_as_float(dp[e + f + 1])), nd)));
-            wp[(e + f) >> 1] = vis ? pack_2(p0, p1, p.f16) : 0u;
-            wd[(e + f) >> 1] = vis ? pack_2(d.x, d.y, p.f16) : 0u;
+            wp[(e + f) >> 1] = pack_2(p0, p1, F16);
+            wd[(e + f) >> 1] = pack_2(d.x, d.y, F16);
           }
         }
-        tmem_st16(t_s + 16 * c, wp);
-        tmem_st16(t_s + 64 + 16 * c, wd);
+        tmem_st16(t_s, wp);
+        tmem_st16(t_s + 64, wd);
+        tmem_wait_st();
       }
-      tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ds_full[grp]);
     }
-    // warpgroup 0 stores dV, warpgroup 1 dK
-    if (!mbar_wait(done, 0, abort_flag, 148)) bad = true;
+    // Warps 0..7 store dV, 8..15 dK, half of the columns each. The row of a hidden key has accumulated whatever its K
+    // and V gave (rows of the products do not mix): it is stored as zeros.
+    if (!mbar_wait(&done[1], 0, abort_flag, 148)) bad = true;
     tc_fence_after();
-    const bool store = j < s.lk && !bad && !*abort_flag;
-    const uint32_t t_g = tmem + lane_off + (grp ? C::COL_DK : C::COL_DV);
+    const int rows = bad || *abort_flag ? 0 : s.lk - j0 - quarter * 32;  // of this warp that exist, if positive
+    const uint32_t t_g = tmem + lane_off + (grp ? C::COL_DK : C::COL_DV) + half * (D / 2);
     const float f = grp ? p.scale : 1.f;
     if (splits == 1) {
-      uint16_t* dst = reinterpret_cast<uint16_t*>(grp ? gr.dk : gr.dv) + row * (grp ? gr.lddk : gr.lddv) + hk * D;
+      const long long ld = grp ? gr.lddk : gr.lddv;
+      uint16_t* dst = reinterpret_cast<uint16_t*>(grp ? gr.dk : gr.dv) + (row - lane) * ld + hk * D + half * (D / 2);
       if (T > 0)
-        store_row16<D>(t_g, f, p.f16, store, dst);
-      else if (store)
-        zero_row16<D>(dst);
+        store_rows16<D / 2>(t_g, f, vis, F16, sQ(0) + warp * XA_STAGE, lane, rows, dst, ld);
+      else if (lane < rows)
+        zero_row16<D / 2>(dst + lane * ld);
     } else {
       const long long width = (long long)p.kv_heads * D;
-      float* dst = gr.partial + ((long long)(part * 2 + grp) * p.total_k + row) * width + hk * D;
+      float* dst = gr.partial + ((long long)(part * 2 + grp) * p.total_k + row) * width + hk * D + half * (D / 2);
       if (T > 0)
-        store_row32<D>(t_g, f, store, dst);
-      else if (store)
+        store_rows32<D / 2>(t_g, f, vis, lane < rows, dst);
+      else if (lane < rows)
 #pragma unroll
-        for (int e = 0; e < D; e += 4) *reinterpret_cast<float4*>(dst + e) = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int e = 0; e < D / 2; e += 4) *reinterpret_cast<float4*>(dst + e) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
   }
   tc_fence_before();
@@ -1063,7 +1220,7 @@ static dim3 rows_grid(long long n, int batch, int sms) {
   return dim3((unsigned)(need < most ? need : most), (unsigned)batch);
 }
 
-template <int D>
+template <int D, bool F16>
 static int launch_fwd(const XParams& p, const void* q, const void* k, const void* v, long long ldq, long long ldk,
                       long long ldv, int sms, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
@@ -1074,13 +1231,13 @@ static int launch_fwd(const XParams& p, const void* q, const void* k, const void
   if ((rc = token_map(&mv, v, q, p.f16, wk, p.total_k, ldv, XA_BN))) return rc;
   const int qtiles = (p.Lq + XA_BM - 1) / XA_BM;
   const int items = qtiles * p.heads * p.batch * p.parts;
-  if ((rc = ensure_smem(cross_fwd_kernel<D>, XFwd<D>::SMEM))) return rc;
-  launch_ex(cross_fwd_kernel<D>, dim3(items < 2 * sms ? items : 2 * sms), dim3(XA_THREADS), XFwd<D>::SMEM, st, 1, mq,
+  if ((rc = ensure_smem(cross_fwd_kernel<D, F16>, XFwd<D>::SMEM))) return rc;
+  launch_ex(cross_fwd_kernel<D, F16>, dim3(items < 2 * sms ? items : 2 * sms), dim3(XA_THREADS), XFwd<D>::SMEM, st, 1, mq,
             mk, mv, p, items, qtiles);
   return launch_status();
 }
 
-template <int D>
+template <int D, bool F16>
 static int launch_bwd(const XParams& p, const XGrad& g, const void* q, const void* k, const void* v, long long ldq,
                       long long ldk, long long ldv, int splits, int sms, cudaStream_t st) {
   CUtensorMap q128, do128, q64, do64, k64, v64, k128, v128;
@@ -1098,15 +1255,15 @@ static int launch_bwd(const XParams& p, const XGrad& g, const void* q, const voi
   if (p.total_q > 0 && p.Lq > 0) {
     const int qtiles = (p.Lq + XA_BM - 1) / XA_BM;
     const int items = qtiles * p.heads * p.batch;
-    if ((rc = ensure_smem(cross_dq_kernel<D>, XDq<D>::SMEM))) return rc;
-    launch_ex(cross_dq_kernel<D>, dim3(items < 2 * sms ? items : 2 * sms), dim3(XA_THREADS), XDq<D>::SMEM, st, 1, q128,
+    if ((rc = ensure_smem(cross_dq_kernel<D, F16>, XDq<D>::SMEM))) return rc;
+    launch_ex(cross_dq_kernel<D, F16>, dim3(items < 2 * sms ? items : 2 * sms), dim3(XA_THREADS), XDq<D>::SMEM, st, 1, q128,
               do128, k64, v64, p, g, items, qtiles);
     if ((rc = launch_status())) return rc;
   }
   if (p.total_k > 0 && p.Lk > 0) {
     const int ktiles = (p.Lk + XA_BM - 1) / XA_BM;
-    if ((rc = ensure_smem(cross_dkv_kernel<D>, XDkv<D>::SMEM))) return rc;
-    launch_ex(cross_dkv_kernel<D>, dim3((unsigned)(ktiles * p.kv_heads * p.batch * splits)), dim3(XB_THREADS),
+    if ((rc = ensure_smem(cross_dkv_kernel<D, F16>, XDkv<D>::SMEM))) return rc;
+    launch_ex(cross_dkv_kernel<D, F16>, dim3((unsigned)(ktiles * p.kv_heads * p.batch * splits)), dim3(XB_THREADS),
               XDkv<D>::SMEM, st, 1, q64, do64, k128, v128, p, g, ktiles, splits);
     if ((rc = launch_status())) return rc;
     if (splits > 1) {
@@ -1172,10 +1329,9 @@ extern "C" int sa3_cross_attention(const void* q, const void* k, const void* v, 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if ((long long)max_seqlen_q * p.group <= XT_MAX_ROWS)
     rc = cross_token(p, q, k, v, ldq, ldk, ldv, head_dim, sms, st);
-  else if (head_dim == 64)
-    rc = launch_fwd<64>(p, q, k, v, ldq, ldk, ldv, sms, st);
   else
-    rc = launch_fwd<128>(p, q, k, v, ldq, ldk, ldv, sms, st);
+    rc = (head_dim == 64 ? p.f16 ? launch_fwd<64, true> : launch_fwd<64, false>
+                         : p.f16 ? launch_fwd<128, true> : launch_fwd<128, false>)(p, q, k, v, ldq, ldk, ldv, sms, st);
   if (rc || p.parts == 1) return rc;
   const dim3 grid = rows_grid((long long)max_seqlen_q * heads * head_dim / 4, batch, sms);
   launch_ex(head_dim == 64 ? cross_merge_kernel<64> : cross_merge_kernel<128>, grid, dim3(256), 0, st, 1, p);
@@ -1249,6 +1405,7 @@ extern "C" int sa3_cross_attention_bwd(const void* dout, const void* q, const vo
   g.delta = static_cast<float*>(workspace);
   g.partial = splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(workspace) + at) : nullptr;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return head_dim == 64 ? launch_bwd<64>(p, g, q, k, v, ldq, ldk, ldv, splits, sms, st)
-                        : launch_bwd<128>(p, g, q, k, v, ldq, ldk, ldv, splits, sms, st);
+  return (head_dim == 64 ? p.f16 ? launch_bwd<64, true> : launch_bwd<64, false>
+                         : p.f16 ? launch_bwd<128, true> : launch_bwd<128, false>)(p, g, q, k, v, ldq, ldk, ldv,
+                                                                                   splits, sms, st);
 }
