@@ -166,6 +166,10 @@ __device__ __forceinline__ void commit2_elect(uint64_t* a, uint64_t* b) {
       "r"(smem_u32(b))
       : "memory");
 }
+// A value that all lanes of a converged warp share, in a uniform register. What an issue loop computes from such values
+// stays there; operands of an MMA that the compiler cannot see to be uniform are moved there one by one before each
+// instruction, which made an issue loop several times as slow as the products it sent.
+__device__ __forceinline__ int uniform_int(int x) { return __reduce_max_sync(0xffffffffu, x); }
 // mbar_wait on every lane of a converged warp; the warp agrees on the outcome.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int site) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, site));

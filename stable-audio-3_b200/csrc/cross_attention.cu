@@ -24,7 +24,7 @@ SA3_DEFINE_ERROR_READER(read_error_cross)
 constexpr int XA_BM = 128;  // rows of the wide side of a tile: queries (forward, dQ) or keys (dK / dV)
 constexpr int XA_BN = 64;   // rows of the walked side: keys (forward, dQ) or queries (dK / dV)
 constexpr float XA_LOG2E = 1.4426950408889634f;
-constexpr float XA_RESCALE_LOG2 = 8.f;  // move the reference maximum only when it grows by more than this
+constexpr float XA_MOST = 32768.f;  // largest sum of a step's exponentials that keeps a row's reference maximum
 constexpr int XA_SUB_M = XA_BM * 128;   // bytes of a 64-column sub-tile of the wide side
 constexpr int XA_SUB_N = XA_BN * 128;   // ... of the walked side
 
@@ -41,14 +41,14 @@ __device__ __forceinline__ uint64_t visible64(const XParams& p, const XSeq& s, i
   return ((uint64_t)hi << 32) | lo;
 }
 
-// A whole warp zeroes the rows of an XA_BN-row tile (subs sub-tiles of 64 columns) whose bit in `keep` is clear. A row is
-// 128 contiguous bytes of a sub-tile: the 128-byte swizzle only permutes its 16-byte chunks.
-__device__ __forceinline__ void zero_rows(uint8_t* tile, int subs, int rows, uint64_t keep, int lane) {
+// A whole warp zeroes those of `rows` <= 64 rows of a tile (subs sub-tiles of 64 columns, `sub` bytes apart) whose bit in
+// `keep` is clear. A row is 128 contiguous bytes of a sub-tile: the 128-byte swizzle only permutes its 16-byte chunks.
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int subs, int sub, int rows, uint64_t keep, int lane) {
   const int chunk = lane & 7;
   for (int r = lane >> 3; r < rows; r += 4)
     if (!((keep >> r) & 1))
       for (int c = 0; c < subs; ++c)
-        *reinterpret_cast<uint4*>(tile + c * XA_SUB_N + r * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(tile + c * sub + r * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   __syncwarp();
 }
@@ -75,34 +75,42 @@ __device__ __forceinline__ void hide32(uint32_t (&s)[32], uint32_t vis) {
 }
 
 // A softmax warp's 32 TMEM lanes x NC columns, times f (0 where !keep), rounded to 16 bits, to the first `rows` of 32
-// rows at dst. A lane holds one row: 16 columns at a time go through shared memory (chunk c of row r at c ^ (r / 4 & 1):
-// no bank conflicts either way), so that a store instruction fills whole 32-byte sectors, two lanes to a row.
-constexpr int XA_STAGE = 32 * 32;
-template <int NC>
+// rows at dst. A lane holds one row: CW columns at a time go through 64 * CW bytes of shared memory (16-byte chunks
+// exchanged within a row so that neither side has bank conflicts), so that a store instruction writes CW consecutive
+// columns of several rows and not 8 of 32.
+template <int NC, int CW>
 __device__ __forceinline__ void store_rows16(uint32_t t_src, float f, bool keep, bool f16, uint8_t* stage, int lane,
                                              int rows, uint16_t* dst, long long ld) {
-  uint16_t* out = dst + (lane >> 1) * ld + (lane & 1) * 8;
+  constexpr int LPR = CW / 8, RPI = 32 / LPR;  // lanes a row, rows an instruction
+  auto slot = [](int r, int c) {
+    return r * (CW * 2) + ((c ^ (CW == 64 ? r & 7 : CW == 32 ? (r >> 1) & 3 : (r >> 2) & 1)) << 4);
+  };
+  uint16_t* out = dst + (lane / LPR) * ld + (lane % LPR) * 8;
 #pragma unroll
-  for (int c = 0; c < NC / 16; ++c) {
-    uint32_t o[16], w[8];
-    tmem_ld16(t_src + 16 * c, o);
+  for (int c = 0; c < NC / CW; ++c) {
+    uint32_t w[CW / 2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      w[e] = keep ? pack_2(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f, f16) : 0u;
+    for (int x = 0; x < CW / 16; ++x) {
+      uint32_t o[16];
+      tmem_ld16(t_src + CW * c + 16 * x, o);
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-      *reinterpret_cast<uint4*>(stage + lane * 32 + ((e ^ ((lane >> 2) & 1)) << 4)) =
-          make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+      for (int e = 0; e < 8; ++e)
+        w[8 * x + e] = keep ? pack_2(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f, f16) : 0u;
+    }
+#pragma unroll
+    for (int e = 0; e < LPR; ++e)
+      *reinterpret_cast<uint4*>(stage + slot(lane, e)) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
     __syncwarp();
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = 16 * e + (lane >> 1);
-      const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 32 + (((lane & 1) ^ ((r >> 2) & 1)) << 4));
-      if (r < rows) *reinterpret_cast<uint4*>(out + 16 * e * ld + 16 * c) = v;
+    for (int e = 0; e < LPR; ++e) {
+      const int r = RPI * e + lane / LPR;
+      const uint4 v = *reinterpret_cast<const uint4*>(stage + slot(r, lane % LPR));
+      if (r < rows) *reinterpret_cast<uint4*>(out + RPI * e * ld + CW * c) = v;
     }
     __syncwarp();
   }
 }
+constexpr int XA_STAGE = 32 * 32;  // bytes of a warp's pass of 16 columns
 // one lane's row, directly
 template <int NC>
 __device__ __forceinline__ void store_row16(uint32_t t_src, float f, bool f16, bool store, uint16_t* dst) {
@@ -120,6 +128,13 @@ __device__ __forceinline__ void store_row16(uint32_t t_src, float f, bool f16, b
       for (int e = 0; e < 4; ++e) d[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
     }
   }
+}
+// The swizzled tiles need a base on a 1024-byte boundary. Dynamic shared memory starts on one when a kernel has no
+// static shared memory; if it ever did not, the kernel would report that and do nothing.
+__device__ __forceinline__ bool aligned_base(const uint8_t* smem) {
+  if ((smem_u32(smem) & 1023) == 0) return true;
+  if (threadIdx.x == 0) record_error(SA3_DEVERR_TIMEOUT, 119);
+  return false;
 }
 template <int D>
 __device__ __forceinline__ void zero_row16(void* dst) {
@@ -145,21 +160,22 @@ __device__ __forceinline__ void store_rows32(uint32_t t_src, float f, bool keep,
   }
 }
 
-// The walk of a persistent CTA over work items: query tile (fastest), head, part of the keys, sequence. Steps by the
+// The walk of a persistent CTA over work items: query rows (fastest), head, part of the keys, sequence. Steps by the
 // grid without divisions: every role of the CTA walks by itself, and a division there delays each item's first product.
+template <int ROWS, int KEYS>  // query rows of an item, keys of a tile
 struct XWalk {
   XSeq s;
   int tile, h, part, b;  // the item
   int j0, T;             // its keys: from j0, in T tiles; T = 0 also for a tile behind the end of its sequence
   int item, dt, dh, dp, db, qtiles;
   __device__ __forceinline__ void load(const XParams& p) {
-    const int all = tile * XA_BM < s.lq ? (s.seen + XA_BN - 1) / XA_BN : 0;
+    const int all = tile * ROWS < s.lq ? (s.seen + KEYS - 1) / KEYS : 0;
     T = all;
     j0 = 0;
     if (p.parts > 1) {
       const int t0 = (int)((long long)all * part / p.parts);
       T = (int)((long long)all * (part + 1) / p.parts) - t0;
-      j0 = t0 * XA_BN;
+      j0 = t0 * KEYS;
     }
   }
   __device__ __forceinline__ XWalk(const XParams& p, int qt, int num_items) {
@@ -192,13 +208,11 @@ struct XWalk {
   }
 };
 
-// Forward and dQ: warps 0..7 softmax, 8 TMA, 9 and 10 MMA (11 idles). Softmax warp w has TMEM lane quarter w % 4 and
-// columns 32 (w / 4) .. + 31 of every score tile: two warps share a row. The score products and the products with the
-// probabilities are issued by warps of their own: a warp alone takes some ten cycles an instruction, and with one
-// issuer for both, its loop set the time of a tile. A score tile's packed results lie over the scores of the same warp:
-// k-step k at column 32 (k / 2) + 8 (k % 2).
+// A CTA's softmax warps come first, then a warp that loads and two that issue products: the score products and the
+// products with the probabilities have issuers of their own. A warp alone takes some ten cycles an instruction, and
+// with one issuer for both, its loop set the time of a tile.
 constexpr int XA_THREADS = 384;
-constexpr int XA_SOFTMAX = 8;      // softmax warps of a CTA: arrivals on the barriers that they release
+constexpr int XA_SOFTMAX = 8;      // softmax warps of the dQ kernel: arrivals on the barriers that they release
 constexpr int XA_REGS_LAUNCH = 80;  // two CTAs an SM
 constexpr int XA_REGS_LOW = 48;     // loads and MMA after the split
 constexpr int XA_REGS_HIGH = 96;    // softmax after the split
@@ -210,57 +224,67 @@ __device__ __forceinline__ void regs_high() { asm volatile("setmaxnreg.inc.sync.
 __device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); }
 
 // ------------------------------------------------------------------------------------------------ forward
-// Persistent, two CTAs an SM: while one CTA's softmax warps exponentiate, the other's tensor core and loads run.
-// Work item = (query tile of 128 rows, head, sequence), query tile fastest, so CTAs that run together share K/V in
-// L2. TMEM (256 columns): two score buffers of 64 columns, P (packed pairs) over the buffer of its scores, O behind.
-// S of key tile t + 1 is multiplied while the softmax works on tile t. Bound by the exponentials at D = 64 (64 * 128
-// of them take 512 cycles of the SM's 16 a cycle, the two products 320), by the shared-memory reads of the products
-// at D = 128.
+// Persistent, two CTAs an SM. A unit is a query tile of 128 rows with four softmax warps (a thread a row) and an issuing
+// warp; D = 64 has two units a CTA, which share the key tiles, D = 128 one. A unit owns 128 or 256 columns of TMEM:
+// two score buffers of SB = 32 or 64 columns and O. It works in steps of SB keys: S = Q K^T, the softmax (which writes
+// P over its S), O (+)= P V. The next step's S is ready before the softmax gets to it; S of step n + 2 is sent right
+// behind P V of step n, whose P it overwrites: one thread's products run in order, so nothing has to come back in
+// between. What bounds a step is the chain score - exponentials - barrier, some 1800 cycles when S waited for P V.
+// Work item = (query rows of the CTA's units, head, part of the keys, sequence), query rows fastest, so CTAs that run
+// together share K/V in L2. The softmax takes a row's maximum over its first visible step only, as the reference of
+// the exponentials, and moves it when a step's sum shows that a score lies far above.
 template <int D>
 struct XFwd {
   static constexpr int SUBS = D / 64;
-  static constexpr int QS = D == 64 ? 2 : 1, KS = D == 64 ? 4 : 2, VS = KS;
-  static constexpr int Q_BYTES = SUBS * XA_SUB_M, T_BYTES = SUBS * XA_SUB_N;
-  static constexpr int TILES = QS * Q_BYTES + (KS + VS) * T_BYTES;
-  static constexpr int PAIRS = 6 * XA_BM * 4;  // maxima [2][2][rows] and sums [2][rows] of the warp pairs
-  static constexpr int SMEM = TILES + XA_SOFTMAX * XA_STAGE + PAIRS + 1024 + 256;
+  static constexpr int UNITS = D == 64 ? 2 : 1, BN = 64, COLS = 256 / UNITS;
+  static constexpr int SB = (COLS - D) / 2, SPT = BN / SB;  // keys of a step, steps of a key tile
+  static constexpr int SOFTMAX = 4 * UNITS, THREADS = 32 * (SOFTMAX + 4);
+  static constexpr int QS = D == 64 ? 2 : 1, KS = 2;
+  static constexpr int SUB_N = BN * 128;  // bytes of 64 columns of a key tile
+  static constexpr int Q_BYTES = SUBS * XA_SUB_M, T_BYTES = SUBS * SUB_N;
+  static constexpr int TILES = UNITS * QS * Q_BYTES + 2 * KS * T_BYTES;
+  static constexpr int CW = D == 64 ? 32 : 64, STAGE = 64 * CW;  // columns of a store pass, bytes of a warp's
+  static constexpr int SMEM = TILES + SOFTMAX * STAGE + 320;
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(XA_THREADS, 2)
+__global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
     cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const XParams p, int num_items, int qtiles) {
   using C = XFwd<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  auto sQ = [&](int s) { return smem + s * C::Q_BYTES; };
-  auto sK = [&](int s) { return smem + C::QS * C::Q_BYTES + s * C::T_BYTES; };
-  auto sV = [&](int s) { return smem + C::QS * C::Q_BYTES + (C::KS + s) * C::T_BYTES; };
-  uint8_t* stage = smem + C::TILES;  // XA_STAGE bytes a softmax warp
-  float* sh_m = reinterpret_cast<float*>(stage + XA_SOFTMAX * XA_STAGE);
-  float* sh_l = sh_m + 4 * XA_BM;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sh_m + 6 * XA_BM);
-  uint64_t* q_full = bars;        // [QS]
-  uint64_t* q_empty = bars + 2;   // [QS]
-  uint64_t* k_full = bars + 4;    // [KS]
-  uint64_t* k_empty = bars + 8;   // [KS]
-  uint64_t* v_full = bars + 12;   // [VS]
-  uint64_t* v_empty = bars + 16;  // [VS]
-  uint64_t* s_full = bars + 20;   // [2] scores of a tile are in TMEM
-  uint64_t* p_full = bars + 22;   // [2] its probabilities are (XA_SOFTMAX arrivals)
-  // [2] P V of a tile is done. Two, since the softmax skips most of these phases: when it waits for tile g's it
-  // knows that tile g - 2's is over, so the parity on the tile's own barrier cannot be that of an older phase.
+  using Walk = XWalk<C::UNITS * XA_BM, C::BN>;
+  constexpr int U = C::UNITS, BN = C::BN, SB = C::SB;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw;
+  if (!aligned_base(smem)) return;
+  auto sQ = [&](int u, int s) { return smem + (u * C::QS + s) * C::Q_BYTES; };
+  auto sK = [&](int s) { return smem + U * C::QS * C::Q_BYTES + s * C::T_BYTES; };
+  auto sV = [&](int s) { return smem + U * C::QS * C::Q_BYTES + (C::KS + s) * C::T_BYTES; };
+  uint8_t* stage = smem + C::TILES;  // STAGE bytes a softmax warp
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stage + C::SOFTMAX * C::STAGE);
+  uint64_t* q_full = bars;        // [unit][QS]
+  uint64_t* q_empty = bars + 4;   // [unit][QS]
+  uint64_t* k_full = bars + 8;    // [KS]
+  uint64_t* k_empty = bars + 10;  // [KS] (an arrival of each unit)
+  uint64_t* v_full = bars + 12;   // [KS]
+  uint64_t* v_empty = bars + 14;  // [KS] (an arrival of each unit)
+  uint64_t* s_full = bars + 16;   // [unit][2] scores of a step are in TMEM
+  uint64_t* p_full = bars + 20;   // [unit][2] its probabilities are (4 arrivals)
+  // [unit][2] P V of a step is done. Two, since the softmax skips most of these phases: when it waits for step n's it
+  // knows that step n - 2's is over, so the parity on the step's own barrier cannot be that of an older phase.
   uint64_t* o_full = bars + 24;
-  uint64_t* o_empty = bars + 26;  // the softmax has read an item's O (XA_SOFTMAX arrivals)
-  uint64_t* done = bars + 27;     // [2]
-  constexpr int NBARS = 29;
+  uint64_t* o_empty = bars + 28;  // [unit] the softmax has read an item's O (4 arrivals)
+  uint64_t* done = bars + 30;     // [unit]
+  constexpr int NBARS = 32;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert(NBARS * 8 + 8 <= 320, "barriers");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < NBARS; ++i) mbar_init(&bars[i], (i == 22 || i == 23 || i == 26) ? XA_SOFTMAX : 1);
+    for (int i = 0; i < NBARS; ++i)
+      mbar_init(&bars[i], (i >= 20 && i < 24) || i == 28 || i == 29 ? 4 : i == 10 || i == 11 || i == 14 || i == 15 ? U : 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -276,228 +300,257 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   grid_dep_wait();
+  // units of an item that have query rows
+  auto units_of = [&](const Walk& it) { return U == 1 || (it.tile * U + 1) * XA_BM >= it.s.lq ? 1 : U; };
 
-  if (warp >= XA_SOFTMAX) regs_low();
-  if (warp == 8) {
+  if (U == 2 && warp >= C::SOFTMAX) regs_low();
+  if (warp == C::SOFTMAX) {
     if (lane == 0) {
-      int g = 0, qc = 0;
+      int g = 0, qc[2] = {0, 0};
       bool ok = true, v_out = true;  // v_out: V of the last counted tile was issued
-      for (XWalk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+      for (Walk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
         if (it.T == 0) continue;
         const XSeq& s = it.s;
-        const int cq = it.h * D, ck = (it.h / p.group) * D;
-        const int qs = qc % C::QS;
-        if (qc >= C::QS && !mbar_wait(&q_empty[qs], ((qc / C::QS) - 1) & 1, abort_flag, 100)) break;
-        mbar_arrive_expect_tx(&q_full[qs], C::Q_BYTES);
-        for (int c = 0; c < C::SUBS; ++c)
-          tma_load_2d(sQ(qs) + c * XA_SUB_M, &tmQ, &q_full[qs], cq + 64 * c, s.qs + it.tile * XA_BM);
-        qc++;
-        for (int t = 0; t < it.T; ++t, ++g) {
-          const int ks = g % C::KS, row = s.ks + it.j0 + t * XA_BN;
+        const int cq = it.h * D, ck = (it.h / p.group) * D, nu = units_of(it);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (u >= nu || !ok) break;
+          const int qs = qc[u] % C::QS;
+          uint64_t* full = &q_full[u * 2 + qs];
+          if (qc[u] >= C::QS && !mbar_wait(&q_empty[u * 2 + qs], ((qc[u] / C::QS) - 1) & 1, abort_flag, 100)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(full, C::Q_BYTES);
+          for (int c = 0; c < C::SUBS; ++c)
+            tma_load_2d(sQ(u, qs) + c * XA_SUB_M, &tmQ, full, cq + 64 * c, s.qs + (it.tile * U + u) * XA_BM);
+          qc[u]++;
+        }
+        for (int t = 0; t < it.T && ok; ++t, ++g) {
+          const int ks = g % C::KS, row = s.ks + it.j0 + t * BN;
           if (g >= C::KS && !mbar_wait(&k_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 101)) {
             ok = false;
             break;
           }
           mbar_arrive_expect_tx(&k_full[ks], C::T_BYTES);
-          for (int c = 0; c < C::SUBS; ++c) tma_load_2d(sK(ks) + c * XA_SUB_N, &tmK, &k_full[ks], ck + 64 * c, row);
-          if (g >= C::VS && !mbar_wait(&v_empty[ks], ((g / C::VS) - 1) & 1, abort_flag, 102)) {
+          for (int c = 0; c < C::SUBS; ++c) tma_load_2d(sK(ks) + c * C::SUB_N, &tmK, &k_full[ks], ck + 64 * c, row);
+          if (g >= C::KS && !mbar_wait(&v_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 102)) {
             g++;
             ok = v_out = false;
             break;
           }
           mbar_arrive_expect_tx(&v_full[ks], C::T_BYTES);
-          for (int c = 0; c < C::SUBS; ++c) tma_load_2d(sV(ks) + c * XA_SUB_N, &tmV, &v_full[ks], ck + 64 * c, row);
+          for (int c = 0; c < C::SUBS; ++c) tma_load_2d(sV(ks) + c * C::SUB_N, &tmV, &v_full[ks], ck + 64 * c, row);
         }
       }
       if (*abort_flag) {
         // wait (bounded, ignoring the abort flag) for the last loads this thread issued
         volatile int never = 0;
-        for (int c = max(qc - C::QS, 0); c < qc; ++c) mbar_wait(&q_full[c % C::QS], (c / C::QS) & 1, &never, 103);
+        for (int u = 0; u < U; ++u)
+          for (int c = max(qc[u] - C::QS, 0); c < qc[u]; ++c)
+            mbar_wait(&q_full[u * 2 + c % C::QS], (c / C::QS) & 1, &never, 103);
         for (int c = max(g - C::KS, 0); c < g; ++c) {
           mbar_wait(&k_full[c % C::KS], (c / C::KS) & 1, &never, 103);
-          if (c + 1 < g || v_out) mbar_wait(&v_full[c % C::VS], (c / C::VS) & 1, &never, 103);
+          if (c + 1 < g || v_out) mbar_wait(&v_full[c % C::KS], (c / C::KS) & 1, &never, 103);
         }
       }
     }
-  } else if (warp == 9) {
-    // S of every tile: the buffer of tile g held the probabilities of tile g - 2
+  } else if (warp > C::SOFTMAX && warp <= C::SOFTMAX + U) {
+    // ------------------------------------------------------------------ products of unit u
+    const int u = uniform_int(warp) - C::SOFTMAX - 1;
     const int fmt = F16 ? 0 : 1;
-    const uint32_t base = smem_u32(smem);
-    const uint64_t dk = sdesc_kmajor_sw128(base);
+    const uint32_t base = uniform_int(smem_u32(smem));
+    const uint64_t dk = sdesc_kmajor_sw128(base), dv = sdesc_mnmajor_sw128(base + U * C::QS * C::Q_BYTES + C::KS * C::T_BYTES, C::SUB_N);
     const uint32_t k_hi = (uint32_t)(dk >> 32), k_lo = (uint32_t)dk;
-    const uint32_t idesc_full = make_idesc(128, XA_BN, fmt, fmt, 0, 0);
-    int g = 0, qc = 0;
+    const uint32_t v_hi = (uint32_t)(dv >> 32), v_lo = (uint32_t)dv;
+    const uint32_t idesc_full = make_idesc(128, SB, fmt, fmt, 0, 0), idesc_o = make_idesc(128, D, fmt, fmt, 0, 1);
+    const uint32_t tm = uniform_int(tmem), t_s = tm + C::COLS * u, t_o = t_s + 2 * SB;
+    uint64_t *my_s = &s_full[2 * u], *my_p = &p_full[2 * u], *my_o = &o_full[2 * u];
+    int g = 0, gn = 0, qc = 0;  // key tiles seen, steps of this unit's items, its items
     bool ok = true;
-    for (XWalk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
-      if (it.T == 0) continue;
+    for (Walk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+      const int T = uniform_int(it.T);
+      if (T == 0) continue;
+      if (u >= uniform_int(units_of(it))) {
+        // the other unit's item: hand its tiles back
+        for (int t = 0; t < T && ok; ++t, ++g) {
+          ok = warp_wait(&k_full[g % C::KS], (g / C::KS) & 1, abort_flag, 105) &&
+               warp_wait(&v_full[g % C::KS], (g / C::KS) & 1, abort_flag, 106);
+          if (ok && lane == 0) {
+            mbar_arrive(&k_empty[g % C::KS]);
+            mbar_arrive(&v_empty[g % C::KS]);
+          }
+        }
+        continue;
+      }
       const int qs = qc % C::QS;
-      const uint32_t qlo = k_lo + ((qs * C::Q_BYTES) >> 4);
-      int left = it.s.seen - it.j0;
-      ok = warp_wait(&q_full[qs], (qc / C::QS) & 1, abort_flag, 104);
-      for (int t = 0; t < it.T && ok; ++t, ++g, left -= XA_BN) {
-        const int ks = g % C::KS;
-        ok = warp_wait(&k_full[ks], (g / C::KS) & 1, abort_flag, 105) &&
-             (g < 2 || warp_wait(&o_full[g & 1], ((g - 2) >> 1) & 1, abort_flag, 105));
-        if (!ok) break;
+      const uint32_t qlo = k_lo + (((u * C::QS + qs) * C::Q_BYTES) >> 4);
+      const int keys = uniform_int(min(it.s.seen - it.j0, T * BN)), N = (keys + SB - 1) / SB;  // keys and steps of the item
+      auto scores = [&](int n) {
+        const int tile = g + n / C::SPT, ks = tile % C::KS;
+        if (n % C::SPT == 0 && !warp_wait(&k_full[ks], (tile / C::KS) & 1, abort_flag, 105)) return false;
         tc_fence_after();
-        const uint32_t idesc = left >= XA_BN ? idesc_full : make_idesc(128, (left + 15) & ~15, fmt, fmt, 0, 0);
-        const uint32_t klo = k_lo + ((C::QS * C::Q_BYTES + ks * C::T_BYTES) >> 4);
+        const int left = keys - n * SB;
+        const uint32_t idesc = left >= SB ? idesc_full : make_idesc(128, (left + 15) & ~15, fmt, fmt, 0, 0);
+        const uint32_t klo = k_lo + ((U * C::QS * C::Q_BYTES + ks * C::T_BYTES + (n % C::SPT) * SB * 128) >> 4);
+        const int b = (gn + n) & 1;
 #pragma unroll
         for (int c = 0; c < C::SUBS; ++c)
-          mma4_ss(tmem + 64 * (g & 1), qlo + c * (XA_SUB_M >> 4), klo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
-        commit2_elect(&s_full[g & 1], &k_empty[ks]);
-        if (t == it.T - 1) commit_elect(&q_empty[qs]);
-      }
-      qc++;
-    }
-    commit_elect(&done[0]);
-    volatile int never = 0;
-    warp_wait(&done[0], 0, &never, 109);
-  } else if (warp == 10) {
-    // O (+)= P V
-    const int fmt = F16 ? 0 : 1;
-    const uint64_t dv = sdesc_mnmajor_sw128(smem_u32(sV(0)), XA_SUB_N);
-    const uint32_t v_hi = (uint32_t)(dv >> 32), v_lo = (uint32_t)dv;
-    const uint32_t idesc_o = make_idesc(128, D, fmt, fmt, 0, 1);
-    const uint32_t t_o = tmem + 128;
-    int g = 0, qc = 0;
-    bool ok = true;
-    for (XWalk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
-      if (it.T == 0) continue;
-      ok = qc == 0 || warp_wait(o_empty, (qc - 1) & 1, abort_flag, 108);
-      for (int t = 0; t < it.T && ok; ++t, ++g) {
-        const int vs = g % C::VS, j0 = it.j0 + t * XA_BN;
-        ok = warp_wait(&v_full[vs], (g / C::VS) & 1, abort_flag, 106);
-        if (!ok) break;
-        const int steps = min(XA_BN / 16, (it.s.seen - j0 + 15) >> 4);
-        if (p.key_mask || it.s.seen - j0 < XA_BN) {
-          const uint64_t vis = visible64(p, it.s, j0, lane), all = low_bits64(16 * steps);
-          if ((vis & all) != all) zero_rows(sV(vs), C::SUBS, 16 * steps, vis, lane);
+          mma4_ss(t_s + SB * b, qlo + c * (XA_SUB_M >> 4), klo + c * (C::SUB_N >> 4), k_hi, idesc, c != 0);
+        if (n % C::SPT == C::SPT - 1 || n == N - 1)
+          commit2_elect(&my_s[b], &k_empty[ks]);
+        else
+          commit_elect(&my_s[b]);
+        if (n == N - 1) commit_elect(&q_empty[u * 2 + qs]);
+        return true;
+      };
+      ok = warp_wait(&q_full[u * 2 + qs], (qc / C::QS) & 1, abort_flag, 104) && scores(0) && (N < 2 || scores(1)) &&
+           (qc == 0 || warp_wait(&o_empty[u], (qc - 1) & 1, abort_flag, 108));
+      for (int n = 0; n < N && ok; ++n) {
+        const int tile = g + n / C::SPT, vs = tile % C::KS, left = keys - n * SB;
+        if (n % C::SPT == 0) {
+          ok = warp_wait(&v_full[vs], (tile / C::KS) & 1, abort_flag, 106);
+          if (!ok) break;
+          if (p.key_mask || left < BN) {
+            // V of hidden keys, which P V multiplies by zero (the CTA's other unit may write the same zeros)
+            const int rows = min(BN, (left + 15) & ~15);
+            const uint64_t vis = visible64(p, it.s, it.j0 + n * SB, lane), all = low_bits64(rows);
+            if ((vis & all) != all) zero_rows(sV(vs), C::SUBS, C::SUB_N, rows, vis, lane);
+          }
         }
-        ok = warp_wait(&p_full[g & 1], (g >> 1) & 1, abort_flag, 107);
+        const int b = (gn + n) & 1;
+        ok = warp_wait(&my_p[b], ((gn + n) >> 1) & 1, abort_flag, 107);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t vlo = v_lo + ((vs * C::T_BYTES) >> 4), t_p = tmem + 64 * (g & 1);
-        if (steps == XA_BN / 16) {
-          mma4_ts(t_o, t_p, t_p + 32, vlo, v_hi, idesc_o, t > 0);
+        const uint32_t vlo = v_lo + ((vs * C::T_BYTES + (n % C::SPT) * SB * 128) >> 4), t_p = t_s + SB * b;
+        if (SB == 64 && left >= SB) {
+          mma4_ts(t_o, t_p, t_p + 16, vlo, v_hi, idesc_o, n > 0);
         } else {
-          for (int k = 0; k < steps; ++k)
-            mma_ts_lo(t_o, t_p + 32 * (k >> 1) + 8 * (k & 1), vlo + k * (2048 >> 4), v_hi, idesc_o, (t > 0 || k > 0) ? 1u : 0u);
+#pragma unroll
+          for (int k = 0; k < SB / 16; ++k)
+            if (left > 16 * k)
+              mma_ts_lo(t_o, t_p + 8 * k, vlo + k * (2048 >> 4), v_hi, idesc_o, (n > 0 || k > 0) ? 1u : 0u);
         }
-        commit2_elect(&o_full[g & 1], &v_empty[vs]);
+        if (n % C::SPT == C::SPT - 1 || n == N - 1)
+          commit2_elect(&my_o[b], &v_empty[vs]);
+        else
+          commit_elect(&my_o[b]);
+        if (n + 2 < N) ok = scores(n + 2);
       }
+      g += T;
+      gn += N;
       qc++;
     }
-    commit_elect(&done[1]);
+    commit_elect(&done[u]);
     volatile int never = 0;
-    warp_wait(&done[1], 0, &never, 109);
-  } else if (warp < XA_SOFTMAX) {
-    regs_high();
-    const int quarter = warp & 3, half = warp >> 2;
-    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-    const uint32_t t_o = tmem + lane_off + 128 + half * (D / 2);  // this warp's half of O's columns
-    float* own_m = sh_m + half * XA_BM + quarter * 32 + lane;     // + 2 * XA_BM for odd tiles
-    const float* other_m = sh_m + (1 - half) * XA_BM + quarter * 32 + lane;
+    warp_wait(&done[u], 0, &never, 109);
+  } else if (warp < C::SOFTMAX) {
+    if (U == 2) regs_high();
+    const int u = warp >> 2, quarter = warp & 3;
+    const uint32_t t_u = tmem + ((uint32_t)(quarter * 32) << 16) + C::COLS * u, t_o = t_u + 2 * SB;
+    uint64_t *my_s = &s_full[2 * u], *my_p = &p_full[2 * u], *my_o = &o_full[2 * u];
     const float NEG_INF = -INFINITY;
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
-    int g = 0;
-    for (XWalk it(p, qtiles, num_items); it.item < num_items; it.next(p, num_items)) {
+    int gn = 0;
+    for (Walk it(p, qtiles, num_items); it.item < num_items; it.next(p, num_items)) {
       const XSeq& s = it.s;
-      const int T = it.T;
-      if (it.tile * XA_BM >= s.lq) continue;
-      const int rows = min(32, s.lq - it.tile * XA_BM - quarter * 32);  // of this warp that exist
+      const int T = it.T, i0 = (it.tile * U + u) * XA_BM;
+      if (i0 >= s.lq) continue;
+      const int rows = min(32, s.lq - i0 - quarter * 32);  // of this warp that exist
       bool bad = false;
       float m = NEG_INF, l = 0.f;
-      int left = s.seen - it.j0;  // keys of this tile and the following ones
-      for (int t = 0; t < T; ++t, ++g, left -= XA_BN) {
-        uint32_t vis = (uint32_t)(low_bits64(left) >> (32 * half));
-        if (p.key_mask) vis = (uint32_t)(visible64(p, s, it.j0 + t * XA_BN, lane) >> (32 * half));
-        const uint32_t t_s = tmem + lane_off + 64 * (g & 1) + 32 * half;
-        if (!mbar_wait(&s_full[g & 1], (g >> 1) & 1, abort_flag, 110)) bad = true;
+      int left = min(s.seen - it.j0, T * BN);  // keys of this step and the following ones
+      const int N = (left + SB - 1) / SB;
+      for (int n = 0; n < N; ++n, ++gn, left -= SB) {
+        const bool masked = p.key_mask != nullptr || left < SB;
+        uint64_t vis = ~0ull;
+        if (masked) vis = visible64(p, s, it.j0 + n * SB, lane);
+        const int b = gn & 1;
+        const uint32_t t_s = t_u + SB * b;
+        if (!mbar_wait(&my_s[b], (gn >> 1) & 1, abort_flag, 110)) bad = true;
         tc_fence_after();
         if (rows > 0) {  // else no row of this warp exists: what P holds there is multiplied and never stored
-          uint32_t sa[32];
-          tmem_ld32_async(t_s, sa);
+          uint32_t sc[SB / 32][32], w[SB / 2];
+#pragma unroll
+          for (int c = 0; c < SB / 32; ++c) tmem_ld32_async(t_s + 32 * c, sc[c]);
           tmem_wait_ld();
-          float mx;
-          if (vis == 0xffffffffu) {
-            mx = max32(sa);
-          } else {
-            hide32(sa, vis);
-            mx = max32(sa);
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < SB / 32; ++c) hide32(sc[c], (uint32_t)(vis >> (32 * c)));
           }
-          // the other half of the row
-          own_m[(g & 1) * 2 * XA_BM] = mx;
-          pair_sync(quarter);
-          mx = fmaxf(mx, other_m[(g & 1) * 2 * XA_BM]);
-          const float m_tile = mx * p.scale_log2;  // scale > 0; -inf when the row sees none of these keys
-          const bool move = m_tile > m + XA_RESCALE_LOG2;
-          if (__any_sync(0xffffffffu, move)) {
-            const float alpha = move ? fast_exp2(m - m_tile) : 1.f;
+          float sum;
+          auto exponentials = [&]() {
+            const float mu = m == NEG_INF ? 0.f : m;
+            const uint64_t negm2 = f2(-mu, -mu);
+            uint64_t acc[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < SB / 32; ++c)
+              exp_chunk(sc[c], scale2, negm2, acc, reinterpret_cast<uint32_t(&)[16]>(w[16 * c]), F16);
+            const float2 r = f2_split(fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3])));
+            sum = r.x + r.y;
+          };
+          // m becomes the maximum of the visible scores so far (scale > 0); what was summed with the old one is scaled
+          auto move = [&]() {
+            float mx = max32(sc[0]);
+            if (SB == 64) mx = fmaxf(mx, max32(sc[SB / 32 - 1]));
+            const float top = fmaxf(m, mx * p.scale_log2);
+            const float alpha = top > m ? fast_exp2(m - top) : 1.f;
+            m = top;
             l *= alpha;
-            if (t > 0) {
-              // rescale this warp's half of O once P V of the last tile is done
-              if (!mbar_wait(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 111)) bad = true;
+            if (n > 0) {
+              if (!mbar_wait(&my_o[b ^ 1], ((gn - 1) >> 1) & 1, abort_flag, 111)) bad = true;
               tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D / 64; ++c) {
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t o[16];
+                tmem_ld16(t_o + 16 * c, o);
 #pragma unroll
-                for (int hh = 0; hh < 2; ++hh) {
-                  uint32_t o[16];
-                  tmem_ld16(t_o + 32 * c + 16 * hh, o);
-#pragma unroll
-                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                  tmem_st16(t_o + 32 * c + 16 * hh, o);
-                }
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st16(t_o + 16 * c, o);
               }
             }
-            if (move) m = m_tile;
+          };
+          if (__any_sync(0xffffffffu, m == NEG_INF)) move();
+          exponentials();
+          // A later step is tried with the reference that is there: its sum tells whether a score lies too far above it
+          // (P stays below fp16's largest number). Then the reference moves and the step is done again.
+          if (__any_sync(0xffffffffu, !(sum <= XA_MOST))) {
+            move();
+            exponentials();
           }
-          if (left > 32 * half) {  // columns behind the last key are not multiplied
-            const float mu = m == NEG_INF ? 0.f : m;
-            uint64_t acc[4] = {0, 0, 0, 0};
-            uint32_t w[16];
-            exp_chunk(sa, scale2, f2(-mu, -mu), acc, w, F16);
-            tmem_st16(t_s, w);
-            const float2 sum = f2_split(fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3])));
-            l += sum.x + sum.y;
-          }
+          l += sum;
+#pragma unroll
+          for (int c = 0; c < SB / 32; ++c) tmem_st16(t_s + 16 * c, reinterpret_cast<uint32_t(&)[16]>(w[16 * c]));
           tmem_wait_st();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[g & 1]);
+        if (lane == 0) mbar_arrive(&my_p[b]);
       }
-      const long long row0 = s.qs + it.tile * XA_BM + quarter * 32;
+      const long long row0 = s.qs + i0 + quarter * 32;
       const long long at = ((long long)it.part * p.heads + it.h) * p.total_q + row0;  // one part: of lse itself
-      float* lse = half ? nullptr : p.parts > 1 ? p.part_lse + at : p.lse ? p.lse + at : nullptr;
-      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + row0 * p.ldo + it.h * D + half * (D / 2);
+      float* lse = p.parts > 1 ? p.part_lse + at : p.lse ? p.lse + at : nullptr;
+      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + row0 * p.ldo + it.h * D;
       if (T == 0) {
         if (lane < rows) {
-          if (p.parts == 1) zero_row16<D / 2>(dst + lane * p.ldo);  // else a part of weight zero: its output is not read
+          if (p.parts == 1) zero_row16<D>(dst + lane * p.ldo);  // else a part of weight zero: its output is not read
           if (lse) lse[lane] = NEG_INF;
         }
         continue;
       }
-      if (rows > 0) {
-        float* x = sh_l + quarter * 32 + lane;
-        x[half * XA_BM] = l;
-        pair_sync(quarter);
-        l += x[(1 - half) * XA_BM];
-      }
-      if (!mbar_wait(&o_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 112)) bad = true;
+      if (!mbar_wait(&my_o[(gn - 1) & 1], ((gn - 1) >> 1) & 1, abort_flag, 112)) bad = true;
       tc_fence_after();
       const int put = bad || *abort_flag ? 0 : rows;
       const float inv = l > 0.f ? 1.f / l : 0.f;
       if (rows > 0) {
         if (p.parts > 1)
-          store_rows32<D / 2>(t_o, inv, true, lane < put, p.part_o + (at + lane) * D + half * (D / 2));
+          store_rows32<D>(t_o, inv, true, lane < put, p.part_o + (at + lane) * D);
         else
-          store_rows16<D / 2>(t_o, inv, true, F16, stage + warp * XA_STAGE, lane, put, dst, p.ldo);
+          store_rows16<D, C::CW>(t_o, inv, true, F16, stage + warp * C::STAGE, lane, put, dst, p.ldo);
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(o_empty);
+      if (lane == 0) mbar_arrive(&o_empty[u]);
       if (lane < put && lse) lse[lane] = l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : NEG_INF;
     }
   }
@@ -534,11 +587,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
   using C = XDq<D>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
-  if (smem_u32(smem_raw) & 1023) {
-    // dynamic shared memory starts on a 1024-byte boundary when there is no static one; the swizzled tiles need that
-    if (threadIdx.x == 0) record_error(SA3_DEVERR_TIMEOUT, 119);
-    return;
-  }
+  if (!aligned_base(smem)) return;
   auto sQ = [&](int s) { return smem + s * C::Q_BYTES; };
   auto sDO = [&](int s) { return smem + (C::QS + s) * C::Q_BYTES; };
   auto sK = [&](int s) { return smem + 2 * C::QS * C::Q_BYTES + s * C::T_BYTES; };
@@ -588,7 +637,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     if (lane == 0) {
       int g = 0, qc = 0;
       bool ok = true, v_out = true;  // v_out: V of the last counted tile was issued
-      for (XWalk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+      for (XWalk<XA_BM, XA_BN> it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
         if (it.T == 0) continue;
         const XSeq& s = it.s;
         const int cq = it.h * D, ck = (it.h / p.group) * D;
@@ -628,25 +677,26 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
   } else if (warp == 9) {
     // S = Q K^T and dP = dO V^T
     const int fmt = F16 ? 0 : 1;
-    const uint32_t base = smem_u32(smem);
+    const uint32_t base = uniform_int(smem_u32(smem)), tm = uniform_int(tmem);
     const uint64_t dk = sdesc_kmajor_sw128(base);
     const uint32_t k_hi = (uint32_t)(dk >> 32), k_lo = (uint32_t)dk;
     const uint32_t idesc_full = make_idesc(128, XA_BN, fmt, fmt, 0, 0);
     int g = 0, qc = 0;
     bool ok = true;
-    for (XWalk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
-      if (it.T == 0) continue;
+    for (XWalk<XA_BM, XA_BN> it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+      const int T = uniform_int(it.T), seen = uniform_int(it.s.seen);
+      if (T == 0) continue;
       const int qs = qc % C::QS;
       const uint32_t qlo = k_lo + ((qs * C::Q_BYTES) >> 4), dlo = k_lo + (((C::QS + qs) * C::Q_BYTES) >> 4);
       ok = warp_wait(&q_full[qs], (qc / C::QS) & 1, abort_flag, 124);
-      for (int t = 0; t < it.T && ok; ++t, ++g) {
-        const int ks = g % C::KS, vs = g % C::VS, left = it.s.seen - t * XA_BN;
+      for (int t = 0; t < T && ok; ++t, ++g) {
+        const int ks = g % C::KS, vs = g % C::VS, left = seen - t * XA_BN;
         ok = warp_wait(&k_full[ks], (g / C::KS) & 1, abort_flag, 125);
         if (!ok) break;
         const int cols = min(XA_BN, (left + 15) & ~15);
         if (p.key_mask || left < XA_BN) {
           const uint64_t vis = visible64(p, it.s, t * XA_BN, lane), all = low_bits64(cols);
-          if ((vis & all) != all) zero_rows(sK(ks), C::SUBS, cols, vis, lane);  // dS K multiplies them by zero
+          if ((vis & all) != all) zero_rows(sK(ks), C::SUBS, XA_SUB_N, cols, vis, lane);  // dS K multiplies them by zero
         }
         ok = g == 0 || warp_wait(sdp_empty, (g - 1) & 1, abort_flag, 126);
         if (!ok) break;
@@ -656,16 +706,16 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
         const uint32_t vlo = k_lo + ((2 * C::QS * C::Q_BYTES + (C::KS + vs) * C::T_BYTES) >> 4);
 #pragma unroll
         for (int c = 0; c < C::SUBS; ++c)
-          mma4_ss(tmem, qlo + c * (XA_SUB_M >> 4), klo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
+          mma4_ss(tm, qlo + c * (XA_SUB_M >> 4), klo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
         ok = warp_wait(&v_full[vs], (g / C::VS) & 1, abort_flag, 125) &&
              (C::SEP || g == 0 || warp_wait(&dq_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 125));
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < C::SUBS; ++c)
-          mma4_ss(tmem + 64, dlo + c * (XA_SUB_M >> 4), vlo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
+          mma4_ss(tm + 64, dlo + c * (XA_SUB_M >> 4), vlo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
         commit2_elect(sdp_full, &v_empty[vs]);
-        if (t == it.T - 1) commit_elect(&q_empty[qs]);
+        if (t == T - 1) commit_elect(&q_empty[qs]);
       }
       qc++;
     }
@@ -675,23 +725,25 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
   } else if (warp == 10) {
     // dQ (+)= dS K
     const int fmt = F16 ? 0 : 1;
-    const uint64_t dm = sdesc_mnmajor_sw128(smem_u32(sK(0)), XA_SUB_N);
+    const uint32_t tm = uniform_int(tmem);
+    const uint64_t dm = sdesc_mnmajor_sw128(uniform_int(smem_u32(sK(0))), XA_SUB_N);
     const uint32_t m_hi = (uint32_t)(dm >> 32), m_lo = (uint32_t)dm;
     const uint32_t idesc = make_idesc(128, D, fmt, fmt, 0, 1);
-    const uint32_t t_dq = tmem + C::COL_DQ;
+    const uint32_t t_dq = tm + C::COL_DQ;
     int g = 0, qc = 0;
     bool ok = true;
-    for (XWalk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
-      if (it.T == 0) continue;
+    for (XWalk<XA_BM, XA_BN> it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+      const int T = uniform_int(it.T), seen = uniform_int(it.s.seen);
+      if (T == 0) continue;
       ok = qc == 0 || warp_wait(dq_empty, (qc - 1) & 1, abort_flag, 128);
-      for (int t = 0; t < it.T && ok; ++t, ++g) {
+      for (int t = 0; t < T && ok; ++t, ++g) {
         const int ks = g % C::KS;
         ok = warp_wait(&ds_full[g & 1], (g >> 1) & 1, abort_flag, 127);
         if (!ok) break;
         tc_fence_after();
-        const int steps = min(XA_BN / 16, (it.s.seen - t * XA_BN + 15) >> 4);
+        const int steps = min(XA_BN / 16, (seen - t * XA_BN + 15) >> 4);
         const uint32_t mlo = m_lo + ((ks * C::T_BYTES) >> 4);
-        const uint32_t t_ds = tmem + C::COL_DS + (C::SEP ? 32 * (g & 1) : 0);
+        const uint32_t t_ds = tm + C::COL_DS + (C::SEP ? 32 * (g & 1) : 0);
         if (steps == XA_BN / 16) {
           mma4_ts(t_dq, t_ds, t_ds + (C::SEP ? 16 : 32), mlo, m_hi, idesc, t > 0);
         } else {
@@ -712,7 +764,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     const uint32_t t_s = tmem + lane_off + 32 * half, t_dq = tmem + lane_off + C::COL_DQ + half * (D / 2);
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
     int g = 0;
-    for (XWalk it(p, qtiles, num_items); it.item < num_items; it.next(p, num_items)) {
+    for (XWalk<XA_BM, XA_BN> it(p, qtiles, num_items); it.item < num_items; it.next(p, num_items)) {
       const XSeq& s = it.s;
       if (it.tile * XA_BM >= s.lq) continue;
       const int h = it.h, T = it.T;
@@ -809,7 +861,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
       const int put = bad || *abort_flag ? 0 : rows;
       if (rows > 0) {
         if (C::SEP)
-          store_rows16<D / 2>(t_dq, p.scale, true, F16, stage + warp * XA_STAGE, lane, put, dst, gr.lddq);
+          store_rows16<D / 2, 16>(t_dq, p.scale, true, F16, stage + warp * XA_STAGE, lane, put, dst, gr.lddq);
         else
           store_row16<D / 2>(t_dq, p.scale, F16, lane < put, dst + lane * gr.lddq);
       }
@@ -954,26 +1006,28 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
   } else if (warp == 17) {
     // S^T = K Q^T and dP^T = V dO^T
     const int fmt = F16 ? 0 : 1;
-    const uint64_t dk = sdesc_kmajor_sw128(smem_u32(smem));
+    const uint32_t tm = uniform_int(tmem);
+    const int n = uniform_int(T), first = uniform_int(t0), per = uniform_int(qtiles), lq = uniform_int(s.lq);
+    const uint64_t dk = sdesc_kmajor_sw128(uniform_int(smem_u32(smem)));
     const uint32_t k_hi = (uint32_t)(dk >> 32), k_lo = (uint32_t)dk, v_lo = k_lo + (C::K_BYTES >> 4);
     const uint32_t idesc = make_idesc(128, XA_BN, fmt, fmt, 0, 0);
-    bool ok = T > 0 && warp_wait(kv_full, 0, abort_flag, 142);
-    int i0 = T > 0 ? (t0 % qtiles) * XA_BN : 0;  // first row of the tile in its sequence
-    for (int t = 0; t < T && ok; ++t) {
+    bool ok = n > 0 && warp_wait(kv_full, 0, abort_flag, 142);
+    int i0 = n > 0 ? (first % per) * XA_BN : 0;  // first row of the tile in its sequence
+    for (int t = 0; t < n && ok; ++t) {
       const int st = t % C::STAGES;
       ok = warp_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 143) &&
            (t < 2 || warp_wait(&used[t & 1], ((t - 2) >> 1) & 1, abort_flag, 143));
       if (!ok) break;
-      const int rows = s.lq - i0;
+      const int rows = lq - i0;
       if (rows < XA_BN) {
         // rows behind the end: dV and dK multiply them by zero probabilities
-        zero_rows(sQ(st), C::SUBS, XA_BN, low_bits64(rows), lane);
-        zero_rows(sDO(st), C::SUBS, XA_BN, low_bits64(rows), lane);
+        zero_rows(sQ(st), C::SUBS, XA_SUB_N, XA_BN, low_bits64(rows), lane);
+        zero_rows(sDO(st), C::SUBS, XA_SUB_N, XA_BN, low_bits64(rows), lane);
       }
       i0 = rows > XA_BN ? i0 + XA_BN : 0;
       tc_fence_after();
       const uint32_t qlo = k_lo + ((2 * C::K_BYTES + 2 * st * C::T_BYTES) >> 4), dlo = qlo + (C::T_BYTES >> 4);
-      const uint32_t t_s = tmem + 128 * (t & 1);
+      const uint32_t t_s = tm + 128 * (t & 1);
 #pragma unroll
       for (int c = 0; c < C::SUBS; ++c)
         mma4_ss(t_s, k_lo + c * (XA_SUB_M >> 4), qlo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
@@ -988,19 +1042,21 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
   } else if (warp == 18) {
     // dV += P^T dO, dK += dS^T Q
     const int fmt = F16 ? 0 : 1;
-    const uint64_t dm = sdesc_mnmajor_sw128(smem_u32(sQ(0)), XA_SUB_N);
+    const uint32_t tm = uniform_int(tmem);
+    const int n = uniform_int(T);
+    const uint64_t dm = sdesc_mnmajor_sw128(uniform_int(smem_u32(sQ(0))), XA_SUB_N);
     const uint32_t m_hi = (uint32_t)(dm >> 32), m_lo = (uint32_t)dm;
     const uint32_t idesc = make_idesc(128, D, fmt, fmt, 0, 1);
     bool ok = true;
-    for (int t = 0; t < T && ok; ++t) {
+    for (int t = 0; t < n && ok; ++t) {
       ok = warp_wait(&ds_full[t & 1], (t >> 1) & 1, abort_flag, 144);
       if (!ok) break;
       tc_fence_after();
       const int st = t % C::STAGES;
       const uint32_t qlo = m_lo + ((2 * st * C::T_BYTES) >> 4), dlo = qlo + (C::T_BYTES >> 4);
-      const uint32_t t_s = tmem + 128 * (t & 1);
-      mma4_ts(tmem + C::COL_DV, t_s, t_s + 32, dlo, m_hi, idesc, t > 0);
-      mma4_ts(tmem + C::COL_DK, t_s + 64, t_s + 96, qlo, m_hi, idesc, t > 0);
+      const uint32_t t_s = tm + 128 * (t & 1);
+      mma4_ts(tm + C::COL_DV, t_s, t_s + 32, dlo, m_hi, idesc, t > 0);
+      mma4_ts(tm + C::COL_DK, t_s + 64, t_s + 96, qlo, m_hi, idesc, t > 0);
       commit2_elect(&empty[st], &used[t & 1]);
     }
     commit_elect(&done[1]);
@@ -1064,7 +1120,7 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
       const long long ld = grp ? gr.lddk : gr.lddv;
       uint16_t* dst = reinterpret_cast<uint16_t*>(grp ? gr.dk : gr.dv) + (row - lane) * ld + hk * D + half * (D / 2);
       if (T > 0)
-        store_rows16<D / 2>(t_g, f, vis, F16, sQ(0) + warp * XA_STAGE, lane, rows, dst, ld);
+        store_rows16<D / 2, 16>(t_g, f, vis, F16, sQ(0) + warp * XA_STAGE, lane, rows, dst, ld);
       else if (lane < rows)
         zero_row16<D / 2>(dst + lane * ld);
     } else {
@@ -1227,12 +1283,13 @@ static int launch_fwd(const XParams& p, const void* q, const void* k, const void
   int rc;
   const long long wq = (long long)p.heads * D, wk = (long long)p.kv_heads * D;
   if ((rc = token_map(&mq, q, q, p.f16, wq, p.total_q, ldq, XA_BM))) return rc;
-  if ((rc = token_map(&mk, k, q, p.f16, wk, p.total_k, ldk, XA_BN))) return rc;
-  if ((rc = token_map(&mv, v, q, p.f16, wk, p.total_k, ldv, XA_BN))) return rc;
-  const int qtiles = (p.Lq + XA_BM - 1) / XA_BM;
+  using C = XFwd<D>;
+  if ((rc = token_map(&mk, k, q, p.f16, wk, p.total_k, ldk, C::BN))) return rc;
+  if ((rc = token_map(&mv, v, q, p.f16, wk, p.total_k, ldv, C::BN))) return rc;
+  const int qtiles = (p.Lq + C::UNITS * XA_BM - 1) / (C::UNITS * XA_BM);
   const int items = qtiles * p.heads * p.batch * p.parts;
-  if ((rc = ensure_smem(cross_fwd_kernel<D, F16>, XFwd<D>::SMEM))) return rc;
-  launch_ex(cross_fwd_kernel<D, F16>, dim3(items < 2 * sms ? items : 2 * sms), dim3(XA_THREADS), XFwd<D>::SMEM, st, 1, mq,
+  if ((rc = ensure_smem(cross_fwd_kernel<D, F16>, C::SMEM))) return rc;
+  launch_ex(cross_fwd_kernel<D, F16>, dim3(items < 2 * sms ? items : 2 * sms), dim3(C::THREADS), C::SMEM, st, 1, mq,
             mk, mv, p, items, qtiles);
   return launch_status();
 }
