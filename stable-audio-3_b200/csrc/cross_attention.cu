@@ -582,8 +582,9 @@ struct XDq {
 template <int D, bool F16>
 __global__ void __launch_bounds__(XA_THREADS, 2)
     cross_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
-                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const XParams p,
-                    const XGrad gr, int num_items, int qtiles) {
+                    const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmK,
+                    const __grid_constant__ CUtensorMap tmV, const XParams p, const XGrad gr, int num_items,
+                    int qtiles) {
   using C = XDq<D>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
@@ -647,6 +648,8 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
         for (int c = 0; c < C::SUBS; ++c) {
           tma_load_2d(sQ(qs) + c * XA_SUB_M, &tmQ, &q_full[qs], cq + 64 * c, s.qs + it.tile * XA_BM);
           tma_load_2d(sDO(qs) + c * XA_SUB_M, &tmDO, &q_full[qs], cq + 64 * c, s.qs + it.tile * XA_BM);
+          // O of these rows, which the softmax warps read for delta when they get to the item
+          tma_prefetch_l2_2d(&tmO, cq + 64 * c, s.qs + it.tile * XA_BM);
         }
         qc++;
         for (int t = 0; t < it.T; ++t, ++g) {
@@ -883,7 +886,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
 // dV += P^T dO and dK += dS^T Q, with dO and Q read as they lie. Two score buffers, each with a softmax warpgroup of
 // its own: one forms P and dS while the tensor core works on the other. TMEM (512 columns): 2 x (S^T 64, dP^T 64),
 // dV, dK.
-constexpr int XB_THREADS = 608;  // warps 0..15 softmax (8 to a score buffer, two to a row), 16 loads, 17 and 18 MMA
+constexpr int XB_THREADS = 576;  // warps 0..15 softmax (8 to a score buffer, two to a row), 16 loads, 17 MMA
 constexpr int XB_SOFTMAX = 8;
 template <int D>
 struct XDkv {
@@ -915,9 +918,8 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
   uint64_t* empty = bars + 5;     // [STAGES]
   uint64_t* sdp_full = bars + 9;  // [2]
   uint64_t* ds_full = bars + 11;  // [2] XB_SOFTMAX arrivals
-  uint64_t* used = bars + 13;     // [2] P and dS of a buffer have been multiplied
-  uint64_t* done = bars + 15;     // [2]
-  constexpr int NBARS = 17;
+  uint64_t* done = bars + 13;
+  constexpr int NBARS = 14;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -1004,20 +1006,20 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
       }
     }
   } else if (warp == 17) {
-    // S^T = K Q^T and dP^T = V dO^T
+    // S^T = K Q^T and dP^T = V dO^T, dV += P^T dO and dK += dS^T Q. The scores of tile t + 2 are sent right behind the
+    // products that read tile t's P and dS, which they overwrite: one thread's products run in order.
     const int fmt = F16 ? 0 : 1;
-    const uint32_t tm = uniform_int(tmem);
+    const uint32_t tm = uniform_int(tmem), base = uniform_int(smem_u32(smem));
     const int n = uniform_int(T), first = uniform_int(t0), per = uniform_int(qtiles), lq = uniform_int(s.lq);
-    const uint64_t dk = sdesc_kmajor_sw128(uniform_int(smem_u32(smem)));
+    const uint64_t dk = sdesc_kmajor_sw128(base), dm = sdesc_mnmajor_sw128(base + 2 * C::K_BYTES, XA_SUB_N);
     const uint32_t k_hi = (uint32_t)(dk >> 32), k_lo = (uint32_t)dk, v_lo = k_lo + (C::K_BYTES >> 4);
-    const uint32_t idesc = make_idesc(128, XA_BN, fmt, fmt, 0, 0);
+    const uint32_t m_hi = (uint32_t)(dm >> 32), m_lo = (uint32_t)dm;
+    const uint32_t idesc_s = make_idesc(128, XA_BN, fmt, fmt, 0, 0), idesc_g = make_idesc(128, D, fmt, fmt, 0, 1);
     bool ok = n > 0 && warp_wait(kv_full, 0, abort_flag, 142);
-    int i0 = n > 0 ? (first % per) * XA_BN : 0;  // first row of the tile in its sequence
-    for (int t = 0; t < n && ok; ++t) {
+    int i0 = n > 0 ? (first % per) * XA_BN : 0;  // first row of the next scores' tile in its sequence
+    auto scores = [&](int t) {
       const int st = t % C::STAGES;
-      ok = warp_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 143) &&
-           (t < 2 || warp_wait(&used[t & 1], ((t - 2) >> 1) & 1, abort_flag, 143));
-      if (!ok) break;
+      if (!warp_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 143)) return false;
       const int rows = lq - i0;
       if (rows < XA_BN) {
         // rows behind the end: dV and dK multiply them by zero probabilities
@@ -1030,24 +1032,14 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
       const uint32_t t_s = tm + 128 * (t & 1);
 #pragma unroll
       for (int c = 0; c < C::SUBS; ++c)
-        mma4_ss(t_s, k_lo + c * (XA_SUB_M >> 4), qlo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
+        mma4_ss(t_s, k_lo + c * (XA_SUB_M >> 4), qlo + c * (XA_SUB_N >> 4), k_hi, idesc_s, c != 0);
 #pragma unroll
       for (int c = 0; c < C::SUBS; ++c)
-        mma4_ss(t_s + 64, v_lo + c * (XA_SUB_M >> 4), dlo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
+        mma4_ss(t_s + 64, v_lo + c * (XA_SUB_M >> 4), dlo + c * (XA_SUB_N >> 4), k_hi, idesc_s, c != 0);
       commit_elect(&sdp_full[t & 1]);
-    }
-    commit_elect(&done[0]);
-    volatile int never = 0;
-    warp_wait(&done[0], 0, &never, 145);
-  } else if (warp == 18) {
-    // dV += P^T dO, dK += dS^T Q
-    const int fmt = F16 ? 0 : 1;
-    const uint32_t tm = uniform_int(tmem);
-    const int n = uniform_int(T);
-    const uint64_t dm = sdesc_mnmajor_sw128(uniform_int(smem_u32(sQ(0))), XA_SUB_N);
-    const uint32_t m_hi = (uint32_t)(dm >> 32), m_lo = (uint32_t)dm;
-    const uint32_t idesc = make_idesc(128, D, fmt, fmt, 0, 1);
-    bool ok = true;
+      return true;
+    };
+    ok = ok && scores(0) && (n < 2 || scores(1));
     for (int t = 0; t < n && ok; ++t) {
       ok = warp_wait(&ds_full[t & 1], (t >> 1) & 1, abort_flag, 144);
       if (!ok) break;
@@ -1055,13 +1047,14 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
       const int st = t % C::STAGES;
       const uint32_t qlo = m_lo + ((2 * st * C::T_BYTES) >> 4), dlo = qlo + (C::T_BYTES >> 4);
       const uint32_t t_s = tm + 128 * (t & 1);
-      mma4_ts(tm + C::COL_DV, t_s, t_s + 32, dlo, m_hi, idesc, t > 0);
-      mma4_ts(tm + C::COL_DK, t_s + 64, t_s + 96, qlo, m_hi, idesc, t > 0);
-      commit2_elect(&empty[st], &used[t & 1]);
+      mma4_ts(tm + C::COL_DV, t_s, t_s + 32, dlo, m_hi, idesc_g, t > 0);
+      mma4_ts(tm + C::COL_DK, t_s + 64, t_s + 96, qlo, m_hi, idesc_g, t > 0);
+      commit_elect(&empty[st]);
+      if (t + 2 < n) ok = scores(t + 2);
     }
-    commit_elect(&done[1]);
+    commit_elect(done);
     volatile int never = 0;
-    warp_wait(&done[1], 0, &never, 145);
+    warp_wait(done, 0, &never, 145);
   } else {
     const int grp = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
     const int r = quarter * 32 + lane;
@@ -1111,7 +1104,7 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
     }
     // Warps 0..7 store dV, 8..15 dK, half of the columns each. The row of a hidden key has accumulated whatever its K
     // and V gave (rows of the products do not mix): it is stored as zeros.
-    if (!mbar_wait(&done[1], 0, abort_flag, 148)) bad = true;
+    if (!mbar_wait(done, 0, abort_flag, 148)) bad = true;
     tc_fence_after();
     const int rows = bad || *abort_flag ? 0 : s.lk - j0 - quarter * 32;  // of this warp that exist, if positive
     const uint32_t t_g = tmem + lane_off + (grp ? C::COL_DK : C::COL_DV) + half * (D / 2);
@@ -1297,13 +1290,14 @@ static int launch_fwd(const XParams& p, const void* q, const void* k, const void
 template <int D, bool F16>
 static int launch_bwd(const XParams& p, const XGrad& g, const void* q, const void* k, const void* v, long long ldq,
                       long long ldk, long long ldv, int splits, int sms, cudaStream_t st) {
-  CUtensorMap q128, do128, q64, do64, k64, v64, k128, v128;
+  CUtensorMap q128, do128, o128, q64, do64, k64, v64, k128, v128;
   int rc;
   const long long wq = (long long)p.heads * D, wk = (long long)p.kv_heads * D;
   const void* any = p.total_q > 0 ? q : k;
   if ((rc = token_map(&q128, q, any, p.f16, wq, p.total_q, ldq, XA_BM))) return rc;
   if ((rc = token_map(&q64, q, any, p.f16, wq, p.total_q, ldq, XA_BN))) return rc;
   if ((rc = token_map(&do128, g.dout, any, p.f16, wq, p.total_q, g.lddo, XA_BM))) return rc;
+  if ((rc = token_map(&o128, p.out, any, p.f16, wq, p.total_q, p.ldo, XA_BM))) return rc;
   if ((rc = token_map(&do64, g.dout, any, p.f16, wq, p.total_q, g.lddo, XA_BN))) return rc;
   if ((rc = token_map(&k64, k, any, p.f16, wk, p.total_k, ldk, XA_BN))) return rc;
   if ((rc = token_map(&v64, v, any, p.f16, wk, p.total_k, ldv, XA_BN))) return rc;
@@ -1314,7 +1308,7 @@ static int launch_bwd(const XParams& p, const XGrad& g, const void* q, const voi
     const int items = qtiles * p.heads * p.batch;
     if ((rc = ensure_smem(cross_dq_kernel<D, F16>, XDq<D>::SMEM))) return rc;
     launch_ex(cross_dq_kernel<D, F16>, dim3(items < 2 * sms ? items : 2 * sms), dim3(XA_THREADS), XDq<D>::SMEM, st, 1, q128,
-              do128, k64, v64, p, g, items, qtiles);
+              do128, o128, k64, v64, p, g, items, qtiles);
     if ((rc = launch_status())) return rc;
   }
   if (p.total_k > 0 && p.Lk > 0) {
