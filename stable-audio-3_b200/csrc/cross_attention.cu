@@ -53,6 +53,11 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int subs, int sub, int 
   __syncwarp();
 }
 
+// 4 bytes from global to shared memory, or zeros
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+
 __device__ __forceinline__ float unpack_lo(uint32_t w, bool f16) {
   return f16 ? __half2float(__ushort_as_half((unsigned short)(w & 0xffffu))) : __uint_as_float(w << 16);
 }
@@ -561,8 +566,8 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
 
 // ------------------------------------------------------------------------------------------------ dQ
 // The forward's walk again: a CTA holds Q and dO of a query tile, walks the keys, recomputes P from the stored lse
-// and accumulates dQ in TMEM. It also forms delta = rowsum(dO * O), which the dK / dV kernel reads, so O and dO are
-// read once here and delta needs no launch of its own. TMEM (256 columns): S, dP, dQ, and dS (packed pairs) in two
+// and accumulates dQ in TMEM. It also forms delta = rowsum(dO * O) and stores it for the dK / dV kernel, so O and dO
+// are read once here and delta needs no launch of its own. TMEM (256 columns): S, dP, dQ, and dS (packed pairs) in two
 // buffers of its own where they fit (D = 64); at D = 128 dS lies over dP. S of the next tile is multiplied as soon as
 // the softmax has read this one's, dP with it at D = 64, and after this tile's dS K at D = 128.
 template <int D>
@@ -811,15 +816,18 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
       pair_sync(quarter);
       const float delta = sh_delta[quarter * 32 + lane];
       pair_sync(quarter);  // both have read it before the next item's is written
-      if (half == 0 && lane < rows) gr.delta[stat + lane] = delta;
       uint16_t* dst = reinterpret_cast<uint16_t*>(gr.dq) + row0 * gr.lddq + h * D + half * (D / 2);
       if (T == 0) {
         if (lane < rows) zero_row16<D / 2>(dst + lane * gr.lddq);
         continue;
       }
-      // a row that saw no key has lse = -inf: with +inf instead its probabilities come out as zero
-      const float l2 = lse == -INFINITY ? INFINITY : lse * XA_LOG2E;
-      const uint64_t negl2 = f2(-l2, -l2), negd2 = f2(-delta, -delta);
+      // a row that saw no key has lse = -inf, which stays -inf here: its probabilities come out as zero
+      const float nl = lse == -INFINITY ? -INFINITY : -lse * XA_LOG2E;
+      const uint64_t negl2 = f2(nl, nl), negd2 = f2(-delta, -delta);
+      if (half == 0 && lane < rows) {
+        gr.stats[stat + lane] = nl;
+        gr.stats[(long long)p.heads * p.total_q + stat + lane] = -delta;
+      }
       bool bad = false;
       int left = s.seen;
       for (int t = 0; t < T; ++t, ++g, left -= XA_BN) {
@@ -914,7 +922,7 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
   float* stats = reinterpret_cast<float*>(smem + C::TILES);  // per stage: -lse * log2(e) [64], -delta [64]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::TILES + C::STATS);
   uint64_t* kv_full = bars;
-  uint64_t* full = bars + 1;      // [STAGES]
+  uint64_t* full = bars + 1;      // [STAGES] (33 arrivals: the tiles, and each lane's copies)
   uint64_t* empty = bars + 5;     // [STAGES]
   uint64_t* sdp_full = bars + 9;  // [2]
   uint64_t* ds_full = bars + 11;  // [2] XB_SOFTMAX arrivals
@@ -926,7 +934,7 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
   static_assert(2 * XB_SOFTMAX * XA_STAGE <= C::STAGES * 2 * C::T_BYTES, "room for the stores");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < NBARS; ++i) mbar_init(&bars[i], (i == 11 || i == 12) ? XB_SOFTMAX : 1);
+    for (int i = 0; i < NBARS; ++i) mbar_init(&bars[i], (i == 11 || i == 12) ? XB_SOFTMAX : (i >= 1 && i < 5) ? 33 : 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -965,32 +973,11 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
           tma_load_2d(sV + c * XA_SUB_M, &tmV, kv_full, hk * D + 64 * c, s.ks + j0);
         }
       }
-      int t = 0;
+      int t = 0, h = hk * p.group + t0 / qtiles, i0 = (t0 % qtiles) * XA_BN;
+      const long long both = (long long)p.heads * p.total_q;  // from -lse * log2(e) to -delta of a row
       for (; t < T; ++t) {
         const int st = t % C::STAGES;
-        const int h = hk * p.group + (t0 + t) / qtiles, i0 = ((t0 + t) % qtiles) * XA_BN;
-        // the row statistics travel with the tile; rows behind the end get probability zero
-        float l2[2], dl[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = i0 + lane + 32 * e;
-          float lse = -INFINITY, d = 0.f;
-          if (i < s.lq) {
-            const long long at = (long long)h * p.total_q + s.qs + i;
-            lse = __ldg(p.lse + at);
-            d = gr.delta[at];
-          }
-          l2[e] = lse == -INFINITY ? -INFINITY : -lse * XA_LOG2E;
-          dl[e] = -d;
-        }
         if (t >= C::STAGES && !warp_wait(&empty[st], ((t / C::STAGES) - 1) & 1, abort_flag, 140)) break;
-        float* sp = stats + st * 2 * XA_BN;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          sp[lane + 32 * e] = l2[e];
-          sp[XA_BN + lane + 32 * e] = dl[e];
-        }
-        __syncwarp();
         if (lane == 0) {
           mbar_arrive_expect_tx(&full[st], 2 * C::T_BYTES);
           for (int c = 0; c < C::SUBS; ++c) {
@@ -998,7 +985,26 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
             tma_load_2d(sDO(st) + c * XA_SUB_N, &tmDO, &full[st], h * D + 64 * c, s.qs + i0);
           }
         }
+        // The row statistics travel with the tile, copied asynchronously: a load that the warp waited for, and divisions
+        // for the tile's place, made its loop slower than the products. Rows behind the end get zeros: with their Q and
+        // dO zeroed below, their probability is one and they add nothing.
+        const float* src = gr.stats + (long long)h * p.total_q + s.qs + i0;
+        const uint32_t dst = smem_u32(stats + st * 2 * XA_BN);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = lane + 32 * e;
+          const bool on = i0 + i < s.lq;
+          copy4(dst + 4 * i, on ? src + i : gr.stats, on);
+          copy4(dst + 4 * (XA_BN + i), on ? src + both + i : gr.stats, on);
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
+        i0 += XA_BN;
+        if (i0 >= s.lq) {
+          i0 = 0;
+          ++h;
+        }
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       if (*abort_flag && lane == 0) {
         volatile int never = 0;
         mbar_wait(kv_full, 0, &never, 141);
@@ -1022,7 +1028,7 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
       if (!warp_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 143)) return false;
       const int rows = lq - i0;
       if (rows < XA_BN) {
-        // rows behind the end: dV and dK multiply them by zero probabilities
+        // rows behind the end: whatever stands there must not enter the sums
         zero_rows(sQ(st), C::SUBS, XA_SUB_N, XA_BN, low_bits64(rows), lane);
         zero_rows(sDO(st), C::SUBS, XA_SUB_N, XA_BN, low_bits64(rows), lane);
       }
@@ -1332,8 +1338,8 @@ static long long fwd_bytes(int parts, int heads, int total_q, int head_dim) {
   return 4 * (((rows + 3) & ~3LL) + rows * head_dim);
 }
 
-// delta first, the parts of dK and dV behind it at a 16-byte boundary
-static long long delta_bytes(int heads, int total_q) { return (((long long)heads * total_q * 4) + 15) & ~15LL; }
+// the row statistics first, the parts of dK and dV behind them at a 16-byte boundary
+static long long stats_bytes(int heads, int total_q) { return (((long long)heads * total_q * 8) + 15) & ~15LL; }
 
 // Parts of the keys in the forward (one CTA each, joined by a second launch): when the query tiles alone leave half of
 // the CTA slots empty and every part still has 8 key tiles or more.
@@ -1411,7 +1417,7 @@ extern "C" int sa3_cross_attention_bwd_workspace(int batch, int max_seqlen_q, in
   const int sms = sm_count();
   if (sms <= 0) return SA3_ERR_LAUNCH;
   const int n = bwd_splits(batch, max_seqlen_q, max_seqlen_k, heads, kv_heads, sms);
-  *bytes = delta_bytes(heads, total_q) + (n > 1 ? 8LL * n * total_k * kv_heads * head_dim : 0);
+  *bytes = stats_bytes(heads, total_q) + (n > 1 ? 8LL * n * total_k * kv_heads * head_dim : 0);
   return SA3_OK;
 }
 
@@ -1438,7 +1444,7 @@ extern "C" int sa3_cross_attention_bwd(const void* dout, const void* q, const vo
   const int sms = sm_count();
   if (sms <= 0) return SA3_ERR_LAUNCH;
   const int splits = bwd_splits(batch, max_seqlen_q, max_seqlen_k, heads, kv_heads, sms);
-  const long long at = delta_bytes(heads, total_q);
+  const long long at = stats_bytes(heads, total_q);
   const long long need = at + (splits > 1 ? 8LL * splits * total_k * kv_heads * head_dim : 0);
   if (workspace_bytes < need || (need > 0 && !workspace)) return SA3_ERR_ARG;
   const XParams p = make_params(const_cast<void*>(out), const_cast<float*>(lse), cu_seqlens_q, cu_seqlens_k, k_lens,
@@ -1453,7 +1459,7 @@ extern "C" int sa3_cross_attention_bwd(const void* dout, const void* q, const vo
   g.lddk = lddk;
   g.dv = dv;
   g.lddv = lddv;
-  g.delta = static_cast<float*>(workspace);
+  g.stats = static_cast<float*>(workspace);
   g.partial = splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(workspace) + at) : nullptr;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return (head_dim == 64 ? p.f16 ? launch_bwd<64, true> : launch_bwd<64, false>

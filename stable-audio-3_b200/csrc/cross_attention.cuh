@@ -27,7 +27,7 @@ struct XGrad {
   const void* dout;
   void *dq, *dk, *dv;
   long long lddo, lddq, lddk, lddv;
-  float* delta;    // [heads, total_q]
+  float* stats;    // [-lse * log2(e), -delta][heads, total_q]
   float* partial;  // [parts][dV, dK][total_k, kv_heads * head_dim], NULL for one part
 };
 
