@@ -107,6 +107,36 @@ __device__ __forceinline__ void commit_elect(uint64_t* bar) {
       "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
       : "memory");
 }
+// mbar_wait whose tries suspend the thread for up to a millisecond each: a waiting warp then leaves the issue slots and
+// the shared-memory pipe to the others instead of trying again every few dozen cycles.
+__device__ __forceinline__ bool mbar_try_wait_1ms(uint32_t addr, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(addr), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int site) {
+  const uint32_t addr = smem_u32(bar);
+  if (mbar_try_wait_1ms(addr, parity)) return true;
+  const long long t0 = clock64();
+  while (true) {
+    if (mbar_try_wait_1ms(addr, parity)) return true;
+    if (*abort) return false;
+    if (clock64() - t0 > SA3_WAIT_BUDGET_CYCLES) {
+      record_error(SA3_DEVERR_TIMEOUT, site);
+      *abort = 1;
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool warp_bar_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int site) {
+  return __all_sync(0xffffffffu, bar_wait(bar, parity, abort, site));
+}
 // Bring one box of a tensor map into L2 (rows and columns outside the tensor are skipped).
 __device__ __forceinline__ void tma_prefetch_l2_2d(const CUtensorMap* m, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(m)),

@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
           if (u >= nu || !ok) break;
           const int qs = qc[u] % C::QS;
           uint64_t* full = &q_full[u * 2 + qs];
-          if (qc[u] >= C::QS && !mbar_wait(&q_empty[u * 2 + qs], ((qc[u] / C::QS) - 1) & 1, abort_flag, 100)) {
+          if (qc[u] >= C::QS && !bar_wait(&q_empty[u * 2 + qs], ((qc[u] / C::QS) - 1) & 1, abort_flag, 100)) {
             ok = false;
             break;
           }
@@ -333,13 +333,13 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
         }
         for (int t = 0; t < it.T && ok; ++t, ++g) {
           const int ks = g % C::KS, row = s.ks + it.j0 + t * BN;
-          if (g >= C::KS && !mbar_wait(&k_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 101)) {
+          if (g >= C::KS && !bar_wait(&k_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 101)) {
             ok = false;
             break;
           }
           mbar_arrive_expect_tx(&k_full[ks], C::T_BYTES);
           for (int c = 0; c < C::SUBS; ++c) tma_load_2d(sK(ks) + c * C::SUB_N, &tmK, &k_full[ks], ck + 64 * c, row);
-          if (g >= C::KS && !mbar_wait(&v_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 102)) {
+          if (g >= C::KS && !bar_wait(&v_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 102)) {
             g++;
             ok = v_out = false;
             break;
@@ -353,10 +353,10 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
         volatile int never = 0;
         for (int u = 0; u < U; ++u)
           for (int c = max(qc[u] - C::QS, 0); c < qc[u]; ++c)
-            mbar_wait(&q_full[u * 2 + c % C::QS], (c / C::QS) & 1, &never, 103);
+            bar_wait(&q_full[u * 2 + c % C::QS], (c / C::QS) & 1, &never, 103);
         for (int c = max(g - C::KS, 0); c < g; ++c) {
-          mbar_wait(&k_full[c % C::KS], (c / C::KS) & 1, &never, 103);
-          if (c + 1 < g || v_out) mbar_wait(&v_full[c % C::KS], (c / C::KS) & 1, &never, 103);
+          bar_wait(&k_full[c % C::KS], (c / C::KS) & 1, &never, 103);
+          if (c + 1 < g || v_out) bar_wait(&v_full[c % C::KS], (c / C::KS) & 1, &never, 103);
         }
       }
     }
@@ -379,8 +379,8 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
       if (u >= uniform_int(units_of(it))) {
         // the other unit's item: hand its tiles back
         for (int t = 0; t < T && ok; ++t, ++g) {
-          ok = warp_wait(&k_full[g % C::KS], (g / C::KS) & 1, abort_flag, 105) &&
-               warp_wait(&v_full[g % C::KS], (g / C::KS) & 1, abort_flag, 106);
+          ok = warp_bar_wait(&k_full[g % C::KS], (g / C::KS) & 1, abort_flag, 105) &&
+               warp_bar_wait(&v_full[g % C::KS], (g / C::KS) & 1, abort_flag, 106);
           if (ok && lane == 0) {
             mbar_arrive(&k_empty[g % C::KS]);
             mbar_arrive(&v_empty[g % C::KS]);
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
       const int keys = uniform_int(min(it.s.seen - it.j0, T * BN)), N = (keys + SB - 1) / SB;  // keys and steps of the item
       auto scores = [&](int n) {
         const int tile = g + n / C::SPT, ks = tile % C::KS;
-        if (n % C::SPT == 0 && !warp_wait(&k_full[ks], (tile / C::KS) & 1, abort_flag, 105)) return false;
+        if (n % C::SPT == 0 && !warp_bar_wait(&k_full[ks], (tile / C::KS) & 1, abort_flag, 105)) return false;
         tc_fence_after();
         const int left = keys - n * SB;
         const uint32_t idesc = left >= SB ? idesc_full : make_idesc(128, (left + 15) & ~15, fmt, fmt, 0, 0);
@@ -409,12 +409,12 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
         if (n == N - 1) commit_elect(&q_empty[u * 2 + qs]);
         return true;
       };
-      ok = warp_wait(&q_full[u * 2 + qs], (qc / C::QS) & 1, abort_flag, 104) && scores(0) && (N < 2 || scores(1)) &&
-           (qc == 0 || warp_wait(&o_empty[u], (qc - 1) & 1, abort_flag, 108));
+      ok = warp_bar_wait(&q_full[u * 2 + qs], (qc / C::QS) & 1, abort_flag, 104) && scores(0) && (N < 2 || scores(1)) &&
+           (qc == 0 || warp_bar_wait(&o_empty[u], (qc - 1) & 1, abort_flag, 108));
       for (int n = 0; n < N && ok; ++n) {
         const int tile = g + n / C::SPT, vs = tile % C::KS, left = keys - n * SB;
         if (n % C::SPT == 0) {
-          ok = warp_wait(&v_full[vs], (tile / C::KS) & 1, abort_flag, 106);
+          ok = warp_bar_wait(&v_full[vs], (tile / C::KS) & 1, abort_flag, 106);
           if (!ok) break;
           if (p.key_mask || left < BN) {
             // V of hidden keys, which P V multiplies by zero (the CTA's other unit may write the same zeros)
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
           }
         }
         const int b = (gn + n) & 1;
-        ok = warp_wait(&my_p[b], ((gn + n) >> 1) & 1, abort_flag, 107);
+        ok = warp_bar_wait(&my_p[b], ((gn + n) >> 1) & 1, abort_flag, 107);
         if (!ok) break;
         tc_fence_after();
         const uint32_t vlo = v_lo + ((vs * C::T_BYTES + (n % C::SPT) * SB * 128) >> 4), t_p = t_s + SB * b;
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
     }
     commit_elect(&done[u]);
     volatile int never = 0;
-    warp_wait(&done[u], 0, &never, 109);
+    warp_bar_wait(&done[u], 0, &never, 109);
   } else if (warp < C::SOFTMAX) {
     if (U == 2) regs_high();
     const int u = warp >> 2, quarter = warp & 3;
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
         if (masked) vis = visible64(p, s, it.j0 + n * SB, lane);
         const int b = gn & 1;
         const uint32_t t_s = t_u + SB * b;
-        if (!mbar_wait(&my_s[b], (gn >> 1) & 1, abort_flag, 110)) bad = true;
+        if (!bar_wait(&my_s[b], (gn >> 1) & 1, abort_flag, 110)) bad = true;
         tc_fence_after();
         if (rows > 0) {  // else no row of this warp exists: what P holds there is multiplied and never stored
           uint32_t sc[SB / 32][32], w[SB / 2];
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
             m = top;
             l *= alpha;
             if (n > 0) {
-              if (!mbar_wait(&my_o[b ^ 1], ((gn - 1) >> 1) & 1, abort_flag, 111)) bad = true;
+              if (!bar_wait(&my_o[b ^ 1], ((gn - 1) >> 1) & 1, abort_flag, 111)) bad = true;
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / 16; ++c) {
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
         }
         continue;
       }
-      if (!mbar_wait(&my_o[(gn - 1) & 1], ((gn - 1) >> 1) & 1, abort_flag, 112)) bad = true;
+      if (!bar_wait(&my_o[(gn - 1) & 1], ((gn - 1) >> 1) & 1, abort_flag, 112)) bad = true;
       tc_fence_after();
       const int put = bad || *abort_flag ? 0 : rows;
       const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
         const XSeq& s = it.s;
         const int cq = it.h * D, ck = (it.h / p.group) * D;
         const int qs = qc % C::QS;
-        if (qc >= C::QS && !mbar_wait(&q_empty[qs], ((qc / C::QS) - 1) & 1, abort_flag, 120)) break;
+        if (qc >= C::QS && !bar_wait(&q_empty[qs], ((qc / C::QS) - 1) & 1, abort_flag, 120)) break;
         mbar_arrive_expect_tx(&q_full[qs], 2 * C::Q_BYTES);
         for (int c = 0; c < C::SUBS; ++c) {
           tma_load_2d(sQ(qs) + c * XA_SUB_M, &tmQ, &q_full[qs], cq + 64 * c, s.qs + it.tile * XA_BM);
@@ -659,13 +659,13 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
         qc++;
         for (int t = 0; t < it.T; ++t, ++g) {
           const int ks = g % C::KS, vs = g % C::VS, row = s.ks + t * XA_BN;
-          if (g >= C::KS && !mbar_wait(&k_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 121)) {
+          if (g >= C::KS && !bar_wait(&k_empty[ks], ((g / C::KS) - 1) & 1, abort_flag, 121)) {
             ok = false;
             break;
           }
           mbar_arrive_expect_tx(&k_full[ks], C::T_BYTES);
           for (int c = 0; c < C::SUBS; ++c) tma_load_2d(sK(ks) + c * XA_SUB_N, &tmK, &k_full[ks], ck + 64 * c, row);
-          if (g >= C::VS && !mbar_wait(&v_empty[vs], ((g / C::VS) - 1) & 1, abort_flag, 122)) {
+          if (g >= C::VS && !bar_wait(&v_empty[vs], ((g / C::VS) - 1) & 1, abort_flag, 122)) {
             g++;
             ok = v_out = false;
             break;
@@ -676,10 +676,10 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
       }
       if (*abort_flag) {
         volatile int never = 0;
-        for (int c = max(qc - C::QS, 0); c < qc; ++c) mbar_wait(&q_full[c % C::QS], (c / C::QS) & 1, &never, 123);
-        for (int c = max(g - C::KS, 0); c < g; ++c) mbar_wait(&k_full[c % C::KS], (c / C::KS) & 1, &never, 123);
+        for (int c = max(qc - C::QS, 0); c < qc; ++c) bar_wait(&q_full[c % C::QS], (c / C::QS) & 1, &never, 123);
+        for (int c = max(g - C::KS, 0); c < g; ++c) bar_wait(&k_full[c % C::KS], (c / C::KS) & 1, &never, 123);
         const int gv = v_out ? g : g - 1;
-        for (int c = max(gv - C::VS, 0); c < gv; ++c) mbar_wait(&v_full[c % C::VS], (c / C::VS) & 1, &never, 123);
+        for (int c = max(gv - C::VS, 0); c < gv; ++c) bar_wait(&v_full[c % C::VS], (c / C::VS) & 1, &never, 123);
       }
     }
   } else if (warp == 9) {
@@ -696,17 +696,17 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
       if (T == 0) continue;
       const int qs = qc % C::QS;
       const uint32_t qlo = k_lo + ((qs * C::Q_BYTES) >> 4), dlo = k_lo + (((C::QS + qs) * C::Q_BYTES) >> 4);
-      ok = warp_wait(&q_full[qs], (qc / C::QS) & 1, abort_flag, 124);
+      ok = warp_bar_wait(&q_full[qs], (qc / C::QS) & 1, abort_flag, 124);
       for (int t = 0; t < T && ok; ++t, ++g) {
         const int ks = g % C::KS, vs = g % C::VS, left = seen - t * XA_BN;
-        ok = warp_wait(&k_full[ks], (g / C::KS) & 1, abort_flag, 125);
+        ok = warp_bar_wait(&k_full[ks], (g / C::KS) & 1, abort_flag, 125);
         if (!ok) break;
         const int cols = min(XA_BN, (left + 15) & ~15);
         if (p.key_mask || left < XA_BN) {
           const uint64_t vis = visible64(p, it.s, t * XA_BN, lane), all = low_bits64(cols);
           if ((vis & all) != all) zero_rows(sK(ks), C::SUBS, XA_SUB_N, cols, vis, lane);  // dS K multiplies them by zero
         }
-        ok = g == 0 || warp_wait(sdp_empty, (g - 1) & 1, abort_flag, 126);
+        ok = g == 0 || warp_bar_wait(sdp_empty, (g - 1) & 1, abort_flag, 126);
         if (!ok) break;
         tc_fence_after();
         const uint32_t idesc = left >= XA_BN ? idesc_full : make_idesc(128, cols, fmt, fmt, 0, 0);
@@ -715,8 +715,8 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
 #pragma unroll
         for (int c = 0; c < C::SUBS; ++c)
           mma4_ss(tm, qlo + c * (XA_SUB_M >> 4), klo + c * (XA_SUB_N >> 4), k_hi, idesc, c != 0);
-        ok = warp_wait(&v_full[vs], (g / C::VS) & 1, abort_flag, 125) &&
-             (C::SEP || g == 0 || warp_wait(&dq_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 125));
+        ok = warp_bar_wait(&v_full[vs], (g / C::VS) & 1, abort_flag, 125) &&
+             (C::SEP || g == 0 || warp_bar_wait(&dq_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 125));
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -729,7 +729,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     }
     commit_elect(&done[0]);
     volatile int never = 0;
-    warp_wait(&done[0], 0, &never, 129);
+    warp_bar_wait(&done[0], 0, &never, 129);
   } else if (warp == 10) {
     // dQ (+)= dS K
     const int fmt = F16 ? 0 : 1;
@@ -743,10 +743,10 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     for (XWalk<XA_BM, XA_BN> it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
       const int T = uniform_int(it.T), seen = uniform_int(it.s.seen);
       if (T == 0) continue;
-      ok = qc == 0 || warp_wait(dq_empty, (qc - 1) & 1, abort_flag, 128);
+      ok = qc == 0 || warp_bar_wait(dq_empty, (qc - 1) & 1, abort_flag, 128);
       for (int t = 0; t < T && ok; ++t, ++g) {
         const int ks = g % C::KS;
-        ok = warp_wait(&ds_full[g & 1], (g >> 1) & 1, abort_flag, 127);
+        ok = warp_bar_wait(&ds_full[g & 1], (g >> 1) & 1, abort_flag, 127);
         if (!ok) break;
         tc_fence_after();
         const int steps = min(XA_BN / 16, (seen - t * XA_BN + 15) >> 4);
@@ -764,7 +764,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     }
     commit_elect(&done[1]);
     volatile int never = 0;
-    warp_wait(&done[1], 0, &never, 129);
+    warp_bar_wait(&done[1], 0, &never, 129);
   } else if (warp < XA_SOFTMAX) {
     regs_high();
     const int quarter = warp & 3, half = warp >> 2;
@@ -834,9 +834,9 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
         uint32_t vis = (uint32_t)(low_bits64(left) >> (32 * half));
         if (p.key_mask) vis = (uint32_t)(visible64(p, s, t * XA_BN, lane) >> (32 * half));
         const uint32_t t_ds = tmem + lane_off + C::COL_DS + (C::SEP ? 32 * (g & 1) + 16 * half : 32 * half);
-        if (!mbar_wait(sdp_full, g & 1, abort_flag, 130)) bad = true;
+        if (!bar_wait(sdp_full, g & 1, abort_flag, 130)) bad = true;
         // the dS that last lay in this tile's columns has been multiplied (D = 128: dP was multiplied after it)
-        if (C::SEP && g > 1 && !mbar_wait(&dq_full[g & 1], ((g - 2) >> 1) & 1, abort_flag, 131)) bad = true;
+        if (C::SEP && g > 1 && !bar_wait(&dq_full[g & 1], ((g - 2) >> 1) & 1, abort_flag, 131)) bad = true;
         tc_fence_after();
         if (rows > 0 && left > 32 * half) {  // else no row of this warp exists, or no column: nothing of it is used
           uint32_t sc[32], dp[32], w[16];
@@ -867,7 +867,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
         __syncwarp();
         if (lane == 0) mbar_arrive(&ds_full[g & 1]);
       }
-      if (!mbar_wait(&dq_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 132)) bad = true;
+      if (!bar_wait(&dq_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 132)) bad = true;
       tc_fence_after();
       const int put = bad || *abort_flag ? 0 : rows;
       if (rows > 0) {
@@ -977,7 +977,7 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
       const long long both = (long long)p.heads * p.total_q;  // from -lse * log2(e) to -delta of a row
       for (; t < T; ++t) {
         const int st = t % C::STAGES;
-        if (t >= C::STAGES && !warp_wait(&empty[st], ((t / C::STAGES) - 1) & 1, abort_flag, 140)) break;
+        if (t >= C::STAGES && !warp_bar_wait(&empty[st], ((t / C::STAGES) - 1) & 1, abort_flag, 140)) break;
         if (lane == 0) {
           mbar_arrive_expect_tx(&full[st], 2 * C::T_BYTES);
           for (int c = 0; c < C::SUBS; ++c) {
@@ -1007,8 +1007,8 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
       asm volatile("cp.async.wait_all;" ::: "memory");
       if (*abort_flag && lane == 0) {
         volatile int never = 0;
-        mbar_wait(kv_full, 0, &never, 141);
-        for (int c = max(t - C::STAGES, 0); c < t; ++c) mbar_wait(&full[c % C::STAGES], (c / C::STAGES) & 1, &never, 141);
+        bar_wait(kv_full, 0, &never, 141);
+        for (int c = max(t - C::STAGES, 0); c < t; ++c) bar_wait(&full[c % C::STAGES], (c / C::STAGES) & 1, &never, 141);
       }
     }
   } else if (warp == 17) {
@@ -1021,11 +1021,11 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
     const uint32_t k_hi = (uint32_t)(dk >> 32), k_lo = (uint32_t)dk, v_lo = k_lo + (C::K_BYTES >> 4);
     const uint32_t m_hi = (uint32_t)(dm >> 32), m_lo = (uint32_t)dm;
     const uint32_t idesc_s = make_idesc(128, XA_BN, fmt, fmt, 0, 0), idesc_g = make_idesc(128, D, fmt, fmt, 0, 1);
-    bool ok = n > 0 && warp_wait(kv_full, 0, abort_flag, 142);
+    bool ok = n > 0 && warp_bar_wait(kv_full, 0, abort_flag, 142);
     int i0 = n > 0 ? (first % per) * XA_BN : 0;  // first row of the next scores' tile in its sequence
-    auto scores = [&](int t) {
+    auto ready = [&](int t) {
       const int st = t % C::STAGES;
-      if (!warp_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 143)) return false;
+      if (!warp_bar_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 143)) return false;
       const int rows = lq - i0;
       if (rows < XA_BN) {
         // rows behind the end: whatever stands there must not enter the sums
@@ -1033,7 +1033,10 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
         zero_rows(sDO(st), C::SUBS, XA_SUB_N, XA_BN, low_bits64(rows), lane);
       }
       i0 = rows > XA_BN ? i0 + XA_BN : 0;
-      tc_fence_after();
+      return true;
+    };
+    auto scores = [&](int t) {
+      const int st = t % C::STAGES;
       const uint32_t qlo = k_lo + ((2 * C::K_BYTES + 2 * st * C::T_BYTES) >> 4), dlo = qlo + (C::T_BYTES >> 4);
       const uint32_t t_s = tm + 128 * (t & 1);
 #pragma unroll
@@ -1043,11 +1046,18 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
       for (int c = 0; c < C::SUBS; ++c)
         mma4_ss(t_s + 64, v_lo + c * (XA_SUB_M >> 4), dlo + c * (XA_SUB_N >> 4), k_hi, idesc_s, c != 0);
       commit_elect(&sdp_full[t & 1]);
-      return true;
     };
-    ok = ok && scores(0) && (n < 2 || scores(1));
+    for (int t = 0; t < 2 && t < n && ok; ++t) {
+      ok = ready(t);
+      if (!ok) break;
+      tc_fence_after();
+      scores(t);
+    }
     for (int t = 0; t < n && ok; ++t) {
-      ok = warp_wait(&ds_full[t & 1], (t >> 1) & 1, abort_flag, 144);
+      // D = 64: both waits lie before the products, while those of the last tile still run, since a wait takes a few
+      // hundred cycles here even for a phase that is over (127 -> 110 us). At D = 128 a tile is twice the bytes and may
+      // not be there yet: it is waited for behind this tile's products (214 against 225 us).
+      ok = (D == 128 || t + 2 >= n || ready(t + 2)) && warp_bar_wait(&ds_full[t & 1], (t >> 1) & 1, abort_flag, 144);
       if (!ok) break;
       tc_fence_after();
       const int st = t % C::STAGES;
@@ -1056,11 +1066,18 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
       mma4_ts(tm + C::COL_DV, t_s, t_s + 32, dlo, m_hi, idesc_g, t > 0);
       mma4_ts(tm + C::COL_DK, t_s + 64, t_s + 96, qlo, m_hi, idesc_g, t > 0);
       commit_elect(&empty[st]);
-      if (t + 2 < n) ok = scores(t + 2);
+      if (t + 2 < n) {
+        if (D == 128) {
+          ok = ready(t + 2);
+          if (!ok) break;
+          tc_fence_after();
+        }
+        scores(t + 2);
+      }
     }
     commit_elect(done);
     volatile int never = 0;
-    warp_wait(done, 0, &never, 145);
+    warp_bar_wait(done, 0, &never, 145);
   } else {
     const int grp = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
     const int r = quarter * 32 + lane;
@@ -1076,8 +1093,8 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
     for (int t = grp; t < T; t += 2) {
       const int st = t % C::STAGES;
       const float* sp = stats + st * 2 * XA_BN + 32 * half;
-      if (!mbar_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 146)) bad = true;
-      if (!mbar_wait(&sdp_full[grp], (t >> 1) & 1, abort_flag, 147)) bad = true;
+      if (!bar_wait(&full[st], (t / C::STAGES) & 1, abort_flag, 146)) bad = true;
+      if (!bar_wait(&sdp_full[grp], (t >> 1) & 1, abort_flag, 147)) bad = true;
       tc_fence_after();
       if (some) {
         uint32_t sc[32], dp[32], wp[16], wd[16];
@@ -1110,7 +1127,7 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
     }
     // Warps 0..7 store dV, 8..15 dK, half of the columns each. The row of a hidden key has accumulated whatever its K
     // and V gave (rows of the products do not mix): it is stored as zeros.
-    if (!mbar_wait(done, 0, abort_flag, 148)) bad = true;
+    if (!bar_wait(done, 0, abort_flag, 148)) bad = true;
     tc_fence_after();
     const int rows = bad || *abort_flag ? 0 : s.lk - j0 - quarter * 32;  // of this warp that exist, if positive
     const uint32_t t_g = tmem + lane_off + (grp ? C::COL_DK : C::COL_DV) + half * (D / 2);
