@@ -24,10 +24,11 @@ namespace sa3 {
 constexpr int ROT_THREADS = 256;
 constexpr int ROT_MAX_DIM = 512;
 constexpr int ROT_MAX_RPB = 4;
+constexpr int ROT_BATCH = 2;
 
 struct RotaryParams {
   const void* x[2];  // q, k
-  void* y[2];
+  void* y[2];  // may be x: a thread reads an element before it writes it, and no other thread touches it
   long long ldx[2], ldy[2];
   int heads[2];
   int dim, rot;           // columns of a head, rotated ones
@@ -40,6 +41,7 @@ struct RotaryParams {
   long long rows_per_batch, offset;
   float scale;
   float sign;
+  bool stream;
 };
 
 template <typename T>
@@ -64,6 +66,18 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
+// stream: evicted first, for outputs that L2 could not keep for their reader anyway
+template <typename T, int VEC>
+__device__ __forceinline__ void put(T* dst, const Pack<T, VEC>& v, bool stream) {
+  if constexpr (sizeof(Pack<T, VEC>) == 16) {
+    if (stream) {
+      __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(&v));
+      return;
+    }
+  }
+  *reinterpret_cast<Pack<T, VEC>*>(dst) = v;
+}
+
 template <typename T, int VEC, bool IL>
 __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotaryParams p) {
   __shared__ float2 cs[ROT_MAX_RPB * ROT_MAX_DIM / 2];
@@ -81,10 +95,31 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotaryParams p) {
   const int c1 = IL || !rotates ? c0 + VEC : half + u * VEC;
   const bool has1 = VEC > 1 || c1 < p.dim;  // an odd width leaves the last one-element unit without its second half
   const int total = p.heads[0] + p.heads[1];
+  auto at = [&](int r, int h, const void* const* base, const long long* ld) {
+    const int w = h >= p.heads[0];
+    return reinterpret_cast<const T*>(base[w]) + (row0 + r) * ld[w] + (long long)(h - (w ? p.heads[0] : 0)) * p.dim;
+  };
+  // The thread's steps: heads hq, hq + heads_par, .. of the first row, then of the next. ROT_BATCH steps are loaded
+  // before the first of them is stored.
+  V a[ROT_BATCH], b[ROT_BATCH];
+  auto fetch = [&](int r, int h) {
+#pragma unroll
+    for (int n = 0; n < ROT_BATCH; ++n) {
+      if (r < nrows) {
+        const T* x = at(r, h, p.x, p.ldx);
+        a[n] = *reinterpret_cast<const V*>(x + c0);
+        b[n] = a[n];
+        if (has1) b[n] = *reinterpret_cast<const V*>(x + c1);
+      }
+      h += p.heads_par;
+      if (h >= total) h = hq, ++r;
+    }
+  };
+  fetch(0, hq);  // in flight while the angles are computed
 
   for (int i = tid; i < nrows * half; i += blockDim.x) {
-    const int r = i / half, f = i - r * half;
-    const long long row = row0 + r;
+    const int rr = i / half, f = i - rr * half;
+    const long long row = row0 + rr;
     const long long pos = p.row_pos ? (long long)__ldg(p.row_pos + row)
                                     : p.offset + (p.rows_per_batch > 0 ? row % p.rows_per_batch : row);
     double t = (double)pos * (__ldg(p.inv_freq + f) * 0.15915494309189533577);  // 1 / (2 pi)
@@ -95,48 +130,42 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotaryParams p) {
   }
   __syncthreads();
 
-  for (int r = 0; r < nrows; ++r) {
-    float co[VEC], si[VEC];
-    if (rotates) {
+  int r = 0, h = hq;
+  while (true) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float2 w = cs[r * half + u * VEC + e];
-        co[e] = w.x;
-        si[e] = w.y;
-      }
-    }
-    const long long row = row0 + r;
-#pragma unroll 2
-    for (int h = hq; h < total; h += p.heads_par) {
-      const int w = h >= p.heads[0];
-      const int hh = w ? h - p.heads[0] : h;
-      const T* x = reinterpret_cast<const T*>(p.x[w]) + row * p.ldx[w] + (long long)hh * p.dim;
-      T* y = reinterpret_cast<T*>(p.y[w]) + row * p.ldy[w] + (long long)hh * p.dim;
-      V a = *reinterpret_cast<const V*>(x + c0), b = a;
-      if (has1) b = *reinterpret_cast<const V*>(x + c1);
-      if (rotates) {
-        if (IL) {
-          // VEC pairs in 2 * VEC consecutive elements: pair e sits at elements 2e and 2e + 1
+    for (int n = 0; n < ROT_BATCH; ++n) {
+      if (r < nrows) {
+        V &x = a[n], &y = b[n];
+        if (rotates) {
+          const float2* w = cs + r * half + u * VEC;
+          if (IL) {
+            // VEC pairs in 2 * VEC consecutive elements: pair e sits at elements 2e and 2e + 1
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            T& lo = 2 * e < VEC ? a.v[(2 * e) % VEC] : b.v[(2 * e) % VEC];
-            T& hi = 2 * e + 1 < VEC ? a.v[(2 * e + 1) % VEC] : b.v[(2 * e + 1) % VEC];
-            const float f = to_f32(lo), g = to_f32(hi);
-            lo = from_f32<T>(f * co[e] - g * si[e]);
-            hi = from_f32<T>(g * co[e] + f * si[e]);
-          }
-        } else {
+            for (int e = 0; e < VEC; ++e) {
+              T& lo = 2 * e < VEC ? x.v[(2 * e) % VEC] : y.v[(2 * e) % VEC];
+              T& hi = 2 * e + 1 < VEC ? x.v[(2 * e + 1) % VEC] : y.v[(2 * e + 1) % VEC];
+              const float f = to_f32(lo), g = to_f32(hi);
+              lo = from_f32<T>(f * w[e].x - g * w[e].y);
+              hi = from_f32<T>(g * w[e].x + f * w[e].y);
+            }
+          } else {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float f = to_f32(a.v[e]), g = to_f32(b.v[e]);
-            a.v[e] = from_f32<T>(f * co[e] - g * si[e]);
-            b.v[e] = from_f32<T>(g * co[e] + f * si[e]);
+            for (int e = 0; e < VEC; ++e) {
+              const float f = to_f32(x.v[e]), g = to_f32(y.v[e]);
+              x.v[e] = from_f32<T>(f * w[e].x - g * w[e].y);
+              y.v[e] = from_f32<T>(g * w[e].x + f * w[e].y);
+            }
           }
         }
+        T* dst = const_cast<T*>(at(r, h, p.y, p.ldy));
+        put(dst + c0, x, p.stream);
+        if (has1) put(dst + c1, y, p.stream);
       }
-      *reinterpret_cast<V*>(y + c0) = a;
-      if (has1) *reinterpret_cast<V*>(y + c1) = b;
+      h += p.heads_par;
+      if (h >= total) h = hq, ++r;
     }
+    if (r >= nrows) break;
+    fetch(r, h);
   }
 }
 
@@ -149,8 +178,12 @@ int launch_rotary(RotaryParams p, bool il, bool in_place, cudaStream_t st) {
   const int turns = (total + most - 1) / most;
   p.heads_par = (total + turns - 1) / turns;
   const int threads = p.units * p.heads_par;
-  // More rows to a block save blocks once every SM has several; below that one row each spreads the work.
+  // More rows to a block save blocks and overlap one's angles with another's data once every SM has several blocks
+  // (1, 2, 4, 8 rows: 51, 44, 41, 40 us for 16494 rows x 48 heads); below that one row each spreads the work.
   p.rpb = p.rows >= 148LL * 8 * ROT_MAX_RPB ? ROT_MAX_RPB : 1;
+  // Outputs above a quarter of L2 are stored evict-first: 39.7 -> 33.5 us for 101 MB out of a fused buffer (16494 rows x
+  // 48 heads x 64), 69 -> 65 us for 210 MB. Smaller ones are left for the attention that reads them next.
+  p.stream = p.rows * total * p.dim * (long long)sizeof(T) > (32LL << 20);
   const long long blocks = (p.rows + p.rpb - 1) / p.rpb;
   if (blocks > 0x7fffffffLL) return SA3_ERR_UNSUPPORTED;
   auto kern = il ? rotary_kernel<T, VEC, true> : rotary_kernel<T, VEC, false>;
