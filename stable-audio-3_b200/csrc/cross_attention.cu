@@ -165,14 +165,21 @@ __device__ __forceinline__ void store_rows32(uint32_t t_src, float f, bool keep,
   }
 }
 
-// The walk of a persistent CTA over work items: query rows (fastest), head, part of the keys, sequence. Steps by the
-// grid without divisions: every role of the CTA walks by itself, and a division there delays each item's first product.
-template <int ROWS, int KEYS>  // query rows of an item, keys of a tile
+// The walk of a persistent CTA over work items: query rows (fastest), head, part of the keys, sequence. Every role of
+// the CTA walks by itself. Uniform batches step by the grid without divisions, which would delay each item's first
+// product. Packed ones number only the tiles that their sequences have (XA_SCAN sequences at most: finding an item's
+// sequence takes a step for each): CTA i takes items i, i + grid, .. of all sequences alike, where numbering the tiles
+// up to the longest sequence leaves some CTAs with few that exist (4 sequences of 1255 .. 2500 queries: 111 -> 77 us
+// forward, 172 -> 124 us dQ).
+constexpr int XA_SCAN = 64;
+template <int ROWS, int KEYS, bool SCAN>  // query rows of an item, keys of a tile, packed numbering
 struct XWalk {
   XSeq s;
   int tile, h, part, b;  // the item
   int j0, T;             // its keys: from j0, in T tiles; T = 0 also for a tile behind the end of its sequence
+  bool live;             // there is an item
   int item, dt, dh, dp, db, qtiles;
+  int start, count;  // packed: items before this sequence's, and its own
   __device__ __forceinline__ void load(const XParams& p) {
     const int all = tile * ROWS < s.lq ? (s.seen + KEYS - 1) / KEYS : 0;
     T = all;
@@ -183,20 +190,48 @@ struct XWalk {
       j0 = t0 * KEYS;
     }
   }
+  // packed: the sequence, tile, head and part of `item`
+  __device__ __forceinline__ void find(const XParams& p) {
+    while (item >= start + count) {
+      start += count;
+      if (++b >= p.batch) {
+        live = false;
+        return;
+      }
+      s = make_seq(p, b);
+      count = (s.lq + ROWS - 1) / ROWS * p.heads * p.parts;
+    }
+    const int tiles = (s.lq + ROWS - 1) / ROWS;
+    int x = item - start;
+    tile = x % tiles, x /= tiles, h = x % p.heads, part = x / p.heads;
+    load(p);
+  }
   __device__ __forceinline__ XWalk(const XParams& p, int qt, int num_items) {
     qtiles = qt;
     int x = item = blockIdx.x;
+    live = item < num_items;
+    if (SCAN) {
+      start = count = 0;
+      b = -1;
+      if (live) find(p);
+      return;
+    }
     tile = x % qt, x /= qt, h = x % p.heads, x /= p.heads, part = x % p.parts, b = x / p.parts;
     x = gridDim.x;
     dt = x % qt, x /= qt, dh = x % p.heads, x /= p.heads, dp = x % p.parts, db = x / p.parts;
-    if (item < num_items) {
+    if (live) {
       s = make_seq(p, b);
       load(p);
     }
   }
   __device__ __forceinline__ void next(const XParams& p, int num_items) {
     item += gridDim.x;
-    if (item >= num_items) return;
+    live = item < num_items;
+    if (!live) return;
+    if (SCAN) {
+      find(p);
+      return;
+    }
     tile += dt;
     int c = tile >= qtiles;
     tile -= c ? qtiles : 0;
@@ -253,12 +288,12 @@ struct XFwd {
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
-template <int D, bool F16>
+template <int D, bool F16, bool SCAN>
 __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
     cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const XParams p, int num_items, int qtiles) {
   using C = XFwd<D>;
-  using Walk = XWalk<C::UNITS * XA_BM, C::BN>;
+  using Walk = XWalk<C::UNITS * XA_BM, C::BN, SCAN>;
   constexpr int U = C::UNITS, BN = C::BN, SB = C::SB;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
@@ -313,7 +348,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
     if (lane == 0) {
       int g = 0, qc[2] = {0, 0};
       bool ok = true, v_out = true;  // v_out: V of the last counted tile was issued
-      for (Walk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+      for (Walk it(p, qtiles, num_items); it.live && ok; it.next(p, num_items)) {
         if (it.T == 0) continue;
         const XSeq& s = it.s;
         const int cq = it.h * D, ck = (it.h / p.group) * D, nu = units_of(it);
@@ -373,7 +408,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
     uint64_t *my_s = &s_full[2 * u], *my_p = &p_full[2 * u], *my_o = &o_full[2 * u];
     int g = 0, gn = 0, qc = 0;  // key tiles seen, steps of this unit's items, its items
     bool ok = true;
-    for (Walk it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+    for (Walk it(p, qtiles, num_items); it.live && ok; it.next(p, num_items)) {
       const int T = uniform_int(it.T);
       if (T == 0) continue;
       if (u >= uniform_int(units_of(it))) {
@@ -457,7 +492,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
     const float NEG_INF = -INFINITY;
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
     int gn = 0;
-    for (Walk it(p, qtiles, num_items); it.item < num_items; it.next(p, num_items)) {
+    for (Walk it(p, qtiles, num_items); it.live; it.next(p, num_items)) {
       const XSeq& s = it.s;
       const int T = it.T, i0 = (it.tile * U + u) * XA_BM;
       if (i0 >= s.lq) continue;
@@ -584,7 +619,7 @@ struct XDq {
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
-template <int D, bool F16>
+template <int D, bool F16, bool SCAN>
 __global__ void __launch_bounds__(XA_THREADS, 2)
     cross_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                     const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmK,
@@ -643,7 +678,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     if (lane == 0) {
       int g = 0, qc = 0;
       bool ok = true, v_out = true;  // v_out: V of the last counted tile was issued
-      for (XWalk<XA_BM, XA_BN> it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+      for (XWalk<XA_BM, XA_BN, SCAN> it(p, qtiles, num_items); it.live && ok; it.next(p, num_items)) {
         if (it.T == 0) continue;
         const XSeq& s = it.s;
         const int cq = it.h * D, ck = (it.h / p.group) * D;
@@ -691,7 +726,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     const uint32_t idesc_full = make_idesc(128, XA_BN, fmt, fmt, 0, 0);
     int g = 0, qc = 0;
     bool ok = true;
-    for (XWalk<XA_BM, XA_BN> it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+    for (XWalk<XA_BM, XA_BN, SCAN> it(p, qtiles, num_items); it.live && ok; it.next(p, num_items)) {
       const int T = uniform_int(it.T), seen = uniform_int(it.s.seen);
       if (T == 0) continue;
       const int qs = qc % C::QS;
@@ -740,7 +775,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     const uint32_t t_dq = tm + C::COL_DQ;
     int g = 0, qc = 0;
     bool ok = true;
-    for (XWalk<XA_BM, XA_BN> it(p, qtiles, num_items); it.item < num_items && ok; it.next(p, num_items)) {
+    for (XWalk<XA_BM, XA_BN, SCAN> it(p, qtiles, num_items); it.live && ok; it.next(p, num_items)) {
       const int T = uniform_int(it.T), seen = uniform_int(it.s.seen);
       if (T == 0) continue;
       ok = qc == 0 || warp_bar_wait(dq_empty, (qc - 1) & 1, abort_flag, 128);
@@ -772,7 +807,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     const uint32_t t_s = tmem + lane_off + 32 * half, t_dq = tmem + lane_off + C::COL_DQ + half * (D / 2);
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
     int g = 0;
-    for (XWalk<XA_BM, XA_BN> it(p, qtiles, num_items); it.item < num_items; it.next(p, num_items)) {
+    for (XWalk<XA_BM, XA_BN, SCAN> it(p, qtiles, num_items); it.live; it.next(p, num_items)) {
       const XSeq& s = it.s;
       if (it.tile * XA_BM >= s.lq) continue;
       const int h = it.h, T = it.T;
@@ -1178,48 +1213,81 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const XParams p, const 
 }
 
 // The forward's output from the parts of the keys: out = sum_s exp(lse_s - lse) out_s, lse = log sum_s exp(lse_s).
-// grid (rows of a sequence x heads x vectors, sequence).
+// A block takes a row of a head; its 8 warps take every eighth part, all loads in flight at once, and join in shared
+// memory. grid (rows of a sequence x heads, sequence).
 template <int D>
 __global__ void __launch_bounds__(256) cross_merge_kernel(const XParams p) {
+  __shared__ float sh[8][D];
+  __shared__ float sh_l[8];
   grid_dep_wait();
   const XSeq s = make_seq(p, blockIdx.y);
-  const long long n = (long long)s.lq * p.heads * (D / 4);
-  for (long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x; at < n; at += (long long)gridDim.x * blockDim.x) {
-    const int d = 4 * (int)(at % (D / 4)), h = (int)(at / (D / 4) % p.heads);
-    const long long row = s.qs + at / (D / 4) / p.heads;
-    const long long one = (long long)p.heads * p.total_q, src = (long long)h * p.total_q + row;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const long long n = (long long)s.lq * p.heads, one = (long long)p.heads * p.total_q;
+  for (long long at = blockIdx.x; at < n; at += gridDim.x) {
+    const int h = (int)(at % p.heads);
+    const long long row = s.qs + at / p.heads, src = (long long)h * p.total_q + row;
     float top = -INFINITY;
-    for (int sp = 0; sp < p.parts; ++sp) top = fmaxf(top, p.part_lse[sp * one + src]);
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-    if (top != -INFINITY)
-      for (int sp = 0; sp < p.parts; ++sp) {
-        const float e = p.part_lse[sp * one + src];
-        if (e == -INFINITY) continue;
-        const float f = fast_exp2((e - top) * XA_LOG2E);
-        const float4 v = *reinterpret_cast<const float4*>(p.part_o + (sp * one + src) * D + d);
-        l += f;
-        a.x = fmaf(v.x, f, a.x);
-        a.y = fmaf(v.y, f, a.y);
-        a.z = fmaf(v.z, f, a.z);
-        a.w = fmaf(v.w, f, a.w);
+    for (int sp = lane; sp < p.parts; sp += 32) top = fmaxf(top, p.part_lse[sp * one + src]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    float a[D / 32], l = 0.f;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) a[e] = 0.f;
+#pragma unroll 4
+    for (int sp = warp; sp < p.parts; sp += 8) {
+      // a part of weight zero may hold anything
+      const float e = p.part_lse[sp * one + src];
+      const float f = e == -INFINITY ? 0.f : fast_exp2((e - top) * XA_LOG2E);
+      const float* o = p.part_o + (sp * one + src) * D + lane;
+      l += f;
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) {
+        const float v = o[32 * x];
+        a[x] = fmaf(f, f != 0.f ? v : 0.f, a[x]);
       }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + h * D + d;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_2(a.x * inv, a.y * inv, p.f16), pack_2(a.z * inv, a.w * inv, p.f16));
-    if (d == 0 && p.lse) p.lse[src] = l > 0.f ? top + __log2f(l) * 0.6931471805599453f : -INFINITY;
+    }
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) sh[warp][32 * x + lane] = a[x];
+    if (lane == 0) sh_l[warp] = l;
+    __syncthreads();
+    if (tid < D / 2) {
+      float x = 0.f, y = 0.f, t = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) x += sh[w][2 * tid], y += sh[w][2 * tid + 1], t += sh_l[w];
+      const float inv = t > 0.f ? 1.f / t : 0.f;
+      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + h * D + 2 * tid;
+      *reinterpret_cast<uint32_t*>(dst) = pack_2(x * inv, y * inv, p.f16);
+      if (tid == 0 && p.lse) p.lse[src] = t > 0.f ? top + __log2f(t) * 0.6931471805599453f : -INFINITY;
+    }
+    __syncthreads();
   }
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// Parts of the dK / dV walk: the number that ends soonest when every wave of CTAs costs its longest walk plus the
-// set-up, epilogue and joining of a part (about 6 tiles). One part writes its result at once.
+// Parts of the dK / dV walk: the number that ends soonest. A part's set-up and epilogue cost about 12 tiles, the
+// joining launch 6 and 2 a part.
+// Uniform batches: every wave of CTAs costs its longest walk. One part writes its result at once.
 static int dkv_splits(long long ctas, long long tiles, int sms) {
   long long best = 1, cost = -1;
   for (long long n = 1; n <= 32 && n <= tiles; ++n) {
     const long long waves = (ctas * n + sms - 1) / sms;
-    const long long c = waves * ((tiles + n - 1) / n + 6) + (n > 1 ? 6 : 0);
+    const long long c = waves * ((tiles + n - 1) / n + 12) + (n > 1 ? 6 + 2 * n : 0);
     if (cost < 0 || c < cost) {
+      cost = c;
+      best = n;
+    }
+  }
+  return (int)best;
+}
+// Packed batches: the lengths are on the device, the totals are not. The SMs share the work of all CTAs, and the end is
+// ragged by half of the longest one (4 sequences of 1255 .. 2500 queries and 528 .. 2111 keys: 158, 138, 150, 161 us
+// with 1, 2, 3, 4 parts, the joining included).
+static int dkv_splits_packed(long long ctas, long long tiles_mean, long long tiles_most, int sms) {
+  long long best = 1;
+  double cost = -1.;
+  for (long long n = 1; n <= 32 && n <= tiles_most; ++n) {
+    const double c = (double)ctas * (tiles_mean + 12. * n) / sms + tiles_most / (2. * n) + (n > 1 ? 6. + 2. * n : 0.);
+    if (cost < 0. || c < cost) {
       cost = c;
       best = n;
     }
@@ -1286,6 +1354,8 @@ static int token_map(CUtensorMap* m, const void* x, const void* other, int f16, 
   return make_tmap_2d(m, rows > 0 ? x : other, dt, 2, width, rows > 0 ? rows : 1, ld, 64, box);
 }
 
+static bool scans(const XParams& p) { return p.cu_q && p.batch <= XA_SCAN; }
+
 // Grid of the joining kernels: enough blocks of 256 threads for `n` elements of a sequence, about 8 an SM in all.
 static dim3 rows_grid(long long n, int batch, int sms) {
   const long long need = (n + 255) / 256, most = (8LL * sms + batch - 1) / batch;
@@ -1304,8 +1374,9 @@ static int launch_fwd(const XParams& p, const void* q, const void* k, const void
   if ((rc = token_map(&mv, v, q, p.f16, wk, p.total_k, ldv, C::BN))) return rc;
   const int qtiles = (p.Lq + C::UNITS * XA_BM - 1) / (C::UNITS * XA_BM);
   const int items = qtiles * p.heads * p.batch * p.parts;
-  if ((rc = ensure_smem(cross_fwd_kernel<D, F16>, C::SMEM))) return rc;
-  launch_ex(cross_fwd_kernel<D, F16>, dim3(items < 2 * sms ? items : 2 * sms), dim3(C::THREADS), C::SMEM, st, 1, mq,
+  auto kern = scans(p) ? cross_fwd_kernel<D, F16, true> : cross_fwd_kernel<D, F16, false>;
+  if ((rc = ensure_smem(kern, C::SMEM))) return rc;
+  launch_ex(kern, dim3(items < 2 * sms ? items : 2 * sms), dim3(C::THREADS), C::SMEM, st, 1, mq,
             mk, mv, p, items, qtiles);
   return launch_status();
 }
@@ -1329,8 +1400,9 @@ static int launch_bwd(const XParams& p, const XGrad& g, const void* q, const voi
   if (p.total_q > 0 && p.Lq > 0) {
     const int qtiles = (p.Lq + XA_BM - 1) / XA_BM;
     const int items = qtiles * p.heads * p.batch;
-    if ((rc = ensure_smem(cross_dq_kernel<D, F16>, XDq<D>::SMEM))) return rc;
-    launch_ex(cross_dq_kernel<D, F16>, dim3(items < 2 * sms ? items : 2 * sms), dim3(XA_THREADS), XDq<D>::SMEM, st, 1, q128,
+    auto kern = scans(p) ? cross_dq_kernel<D, F16, true> : cross_dq_kernel<D, F16, false>;
+    if ((rc = ensure_smem(kern, XDq<D>::SMEM))) return rc;
+    launch_ex(kern, dim3(items < 2 * sms ? items : 2 * sms), dim3(XA_THREADS), XDq<D>::SMEM, st, 1, q128,
               do128, o128, k64, v64, p, g, items, qtiles);
     if ((rc = launch_status())) return rc;
   }
@@ -1368,10 +1440,15 @@ static int fwd_parts(int batch, int max_q, int max_k, int heads, int kv_heads, i
   return n >= 2 ? (int)n : 1;
 }
 
-static int bwd_splits(int batch, int max_q, int max_k, int heads, int kv_heads, int sms) {
+static int bwd_splits(int batch, int max_q, int max_k, int total_q, int total_k, int heads, int kv_heads, int sms) {
+  if (batch <= 0) return 1;
+  const long long most = (long long)(heads / kv_heads) * ((max_q + XA_BN - 1) / XA_BN);
   const long long ctas = (long long)((max_k + XA_BM - 1) / XA_BM) * kv_heads * batch;
-  const long long tiles = (long long)(heads / kv_heads) * ((max_q + XA_BN - 1) / XA_BN);
-  return ctas > 0 && tiles > 0 ? dkv_splits(ctas, tiles, sms) : 1;
+  if (ctas <= 0 || most <= 0) return 1;
+  if ((long long)batch * max_q == total_q && (long long)batch * max_k == total_k) return dkv_splits(ctas, most, sms);
+  const long long some = (total_k / XA_BM + batch) * kv_heads;
+  const long long mean = (long long)(heads / kv_heads) * (total_q / XA_BN / batch + 1);
+  return dkv_splits_packed(some < ctas ? some : ctas, mean < most ? mean : most, most, sms);
 }
 
 }  // namespace sa3
@@ -1407,7 +1484,7 @@ extern "C" int sa3_cross_attention(const void* q, const void* k, const void* v, 
     rc = (head_dim == 64 ? p.f16 ? launch_fwd<64, true> : launch_fwd<64, false>
                          : p.f16 ? launch_fwd<128, true> : launch_fwd<128, false>)(p, q, k, v, ldq, ldk, ldv, sms, st);
   if (rc || p.parts == 1) return rc;
-  const dim3 grid = rows_grid((long long)max_seqlen_q * heads * head_dim / 4, batch, sms);
+  const dim3 grid = rows_grid((long long)max_seqlen_q * heads * 256, batch, sms);
   launch_ex(head_dim == 64 ? cross_merge_kernel<64> : cross_merge_kernel<128>, grid, dim3(256), 0, st, 1, p);
   return launch_status();
 }
@@ -1433,7 +1510,7 @@ extern "C" int sa3_cross_attention_bwd_workspace(int batch, int max_seqlen_q, in
   if (head_dim != 64 && head_dim != 128) return SA3_ERR_UNSUPPORTED;
   const int sms = sm_count();
   if (sms <= 0) return SA3_ERR_LAUNCH;
-  const int n = bwd_splits(batch, max_seqlen_q, max_seqlen_k, heads, kv_heads, sms);
+  const int n = bwd_splits(batch, max_seqlen_q, max_seqlen_k, total_q, total_k, heads, kv_heads, sms);
   *bytes = stats_bytes(heads, total_q) + (n > 1 ? 8LL * n * total_k * kv_heads * head_dim : 0);
   return SA3_OK;
 }
@@ -1460,7 +1537,7 @@ extern "C" int sa3_cross_attention_bwd(const void* dout, const void* q, const vo
   if (batch == 0 || (total_q == 0 && total_k == 0)) return SA3_OK;
   const int sms = sm_count();
   if (sms <= 0) return SA3_ERR_LAUNCH;
-  const int splits = bwd_splits(batch, max_seqlen_q, max_seqlen_k, heads, kv_heads, sms);
+  const int splits = bwd_splits(batch, max_seqlen_q, max_seqlen_k, total_q, total_k, heads, kv_heads, sms);
   const long long at = stats_bytes(heads, total_q);
   const long long need = at + (splits > 1 ? 8LL * splits * total_k * kv_heads * head_dim : 0);
   if (workspace_bytes < need || (need > 0 && !workspace)) return SA3_ERR_ARG;

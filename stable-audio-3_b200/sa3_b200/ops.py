@@ -303,16 +303,16 @@ def diff_attn_swa(q_bat: torch.Tensor, k_bat: torch.Tensor, v_bat: torch.Tensor,
 
 
 # ---------------------------------------------------------------------- rotary positions, cross-attention
-def _device_of(*ts: Optional[torch.Tensor]) -> int:
+def _device_of(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
     """The device index of the tensors, which must be CUDA tensors of one device."""
-    dev = ts[0].get_device()
+    dev = first.get_device()
     if dev < 0:
         raise RuntimeError("sa3_b200 ops run on CUDA tensors only (no CPU path)")
-    for t in ts:
+    for t in others:
         if t is not None and t.get_device() != dev:
             if not t.is_cuda:
                 raise RuntimeError("sa3_b200 ops run on CUDA tensors only (no CPU path)")
-            raise RuntimeError(f"tensors on {ts[0].device} and {t.device}: one call works on one device")
+            raise RuntimeError(f"tensors on {first.device} and {t.device}: one call works on one device")
     return dev
 
 
@@ -329,14 +329,16 @@ def _rows_view(t: torch.Tensor, rows: int, cols: int, name: str, dtype: torch.dt
     """Row stride of a token-row view [rows, cols]; refuses other shapes, types and strides."""
     if t.dtype is not dtype:
         raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != (rows, cols):
+    if t.shape != (rows, cols):
         raise RuntimeError(f"{name} must be [{rows}, {cols}], got {tuple(t.shape)}")
     ld, inner = t.stride()
-    if rows <= 1:
-        ld = cols  # one row has no stride of its own: torch may report anything there
     if inner != 1 and cols > 1 and rows > 0:
         raise RuntimeError(f"{name} must be a row-major view, got strides {t.stride()}")
-    return ld
+    # one row has no stride of its own: torch may report anything there
+    return ld if rows > 1 else cols
+
+
+_DT16 = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 
 
 def _index(t: Optional[torch.Tensor], n: int, name: str) -> Optional[int]:
@@ -434,7 +436,7 @@ def _cross_args(q, k, v, heads, kv_heads, head_dim, batch, max_seqlen_q, max_seq
                 k_lens, key_mask, softmax_scale):
     """Checks shared by the two passes; (kv_heads, strides of q k v, index pointers, batch, scale)."""
     dtype = q.dtype
-    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+    if dtype not in _DT16:
         raise RuntimeError(f"cross_attention works on bf16 or fp16, got {dtype}")
     if kv_heads is None:
         kv_heads = heads
@@ -458,8 +460,10 @@ def _cross_args(q, k, v, heads, kv_heads, head_dim, batch, max_seqlen_q, max_seq
     if key_mask is not None and (key_mask.dtype not in (torch.bool, torch.uint8) or not key_mask.is_contiguous()
                                  or key_mask.numel() != krows):
         raise RuntimeError("key_mask must be a contiguous bool or uint8 tensor with one element a key row")
-    idx = (_index(cu_seqlens_q, batch + 1, "cu_seqlens_q"), _index(cu_seqlens_k, batch + 1, "cu_seqlens_k"),
-           _index(k_lens, batch, "k_lens"), _ptr(key_mask))
+    idx = (cu_seqlens_q if cu_seqlens_q is None else _index(cu_seqlens_q, batch + 1, "cu_seqlens_q"),
+           cu_seqlens_k if cu_seqlens_k is None else _index(cu_seqlens_k, batch + 1, "cu_seqlens_k"),
+           k_lens if k_lens is None else _index(k_lens, batch, "k_lens"),
+           key_mask if key_mask is None else key_mask.data_ptr())
     scale = head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not 0.0 < scale < math.inf:
         raise RuntimeError("softmax_scale must be positive and finite")
@@ -511,7 +515,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, heads:
     _count()
     rc = _on_device(dev, _lib.load().sa3_cross_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                     _ptr(lse), *idx, batch, max_seqlen_q, max_seqlen_k, rows, k.shape[0], heads, kv_heads, head_dim,
-                    *ld, ldo, scale, _dt(q), _ptr(ws), n)
+                    *ld, ldo, scale, _DT16[q.dtype], _ptr(ws), n)
     if rc:
         _lib.check(rc, "sa3_cross_attention")
     return (out, lse) if return_lse else out
@@ -552,7 +556,7 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     rc = _on_device(dev, _lib.load().sa3_cross_attention_bwd, dout.data_ptr(), q.data_ptr(), k.data_ptr(),
                     v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *idx,
                     batch, max_seqlen_q, max_seqlen_k, rows, krows, heads, kv_heads, head_dim, lddo, *ld, ldo, lddq,
-                    lddk, lddv, scale, _dt(q), ws.data_ptr(), n)
+                    lddk, lddv, scale, _DT16[dtype], ws.data_ptr(), n)
     if rc:
         _lib.check(rc, "sa3_cross_attention_bwd")
     return dq, dk, dv
