@@ -248,9 +248,9 @@ struct XWalk {
   }
 };
 
-// A CTA's softmax warps come first, then a warp that loads and two that issue products: the score products and the
-// products with the probabilities have issuers of their own. A warp alone takes some ten cycles an instruction, and
-// with one issuer for both, its loop set the time of a tile.
+// A CTA's softmax warps come first, then a warp that loads and two that issue products: in the forward one a unit, in
+// dQ one for the scores and one for dS K. A warp alone takes some ten cycles an instruction; with one issuer for all,
+// its loop set the time of a tile (dQ of 2 x 8247 queries x 257 keys x 24 heads: 162 -> 113 us).
 constexpr int XA_THREADS = 384;
 constexpr int XA_SOFTMAX = 8;      // softmax warps of the dQ kernel: arrivals on the barriers that they release
 constexpr int XA_REGS_LAUNCH = 80;  // two CTAs an SM
@@ -269,7 +269,9 @@ __device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync 
 // two score buffers of SB = 32 or 64 columns and O. It works in steps of SB keys: S = Q K^T, the softmax (which writes
 // P over its S), O (+)= P V. The next step's S is ready before the softmax gets to it; S of step n + 2 is sent right
 // behind P V of step n, whose P it overwrites: one thread's products run in order, so nothing has to come back in
-// between. What bounds a step is the chain score - exponentials - barrier, some 1800 cycles when S waited for P V.
+// between. Bound by the chain barrier - TMEM load - exponentials - TMEM store - barrier - products of a step, of which
+// an SM has four (D = 64) or two (D = 128) to run past each other: 68 us on 2 x 8247 queries x 257 keys x 24 heads (23
+// for the exponentials alone), 1034 TFLOP/s on 4099 x 6001 with 16 heads of 128 columns (62 % of the measured peak).
 // Work item = (query rows of the CTA's units, head, part of the keys, sequence), query rows fastest, so CTAs that run
 // together share K/V in L2. The softmax takes a row's maximum over its first visible step only, as the reference of
 // the exponentials, and moves it when a step's sum shows that a score lies far above.
@@ -601,10 +603,12 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
 
 // ------------------------------------------------------------------------------------------------ dQ
 // The forward's walk again: a CTA holds Q and dO of a query tile, walks the keys, recomputes P from the stored lse
-// and accumulates dQ in TMEM. It also forms delta = rowsum(dO * O) and stores it for the dK / dV kernel, so O and dO
-// are read once here and delta needs no launch of its own. TMEM (256 columns): S, dP, dQ, and dS (packed pairs) in two
+// and accumulates dQ in TMEM. It also forms delta (rowsum(dO * O), or with a single key tile the equal sum of P * dP)
+// and stores it for the dK / dV kernel, so delta needs no launch of its own. TMEM (256 columns): S, dP, dQ, and dS (packed pairs) in two
 // buffers of its own where they fit (D = 64); at D = 128 dS lies over dP. S of the next tile is multiplied as soon as
-// the softmax has read this one's, dP with it at D = 64, and after this tile's dS K at D = 128.
+// the softmax has read this one's, dP with it at D = 64, and after this tile's dS K at D = 128. 106 us on 2 x 8247
+// queries x 257 keys x 24 heads: some 1050 cycles a key tile and SM, and 5000 for an item's start and end, where its
+// 64 KB come from DRAM (31 us in all).
 template <int D>
 struct XDq {
   static constexpr int SUBS = D / 64;
@@ -816,8 +820,12 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
       const long long stat = (long long)h * p.total_q + row0;
       float lse = -INFINITY;
       if (lane < rows) lse = __ldg(p.lse + stat + lane);
-      {
-        // delta: this warp's 16 of the pair's 32 rows, D / 8 lanes a row, 16 bytes each
+      // One key tile: delta = sum P * dP over the row's scores below, without O's rounding, which is felt where few keys
+      // are averaged, and without reading O and dO. Else delta = rowsum(dO * O).
+      const bool single = T == 1;
+      float delta = 0.f;
+      if (T > 1) {
+        // this warp's 16 of the pair's 32 rows, D / 8 lanes a row, 16 bytes each
         constexpr int LPR = D / 8, RPI = 32 / LPR;
         const int c = lane % LPR, first = 16 * half + lane / LPR;
         const uint16_t* po = reinterpret_cast<const uint16_t*>(p.out) + (row0 + first) * p.ldo + h * D + 8 * c;
@@ -847,10 +855,10 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
             if (c == 0) sh_delta[quarter * 32 + n + e * RPI + first] = sum;
           }
         }
+        pair_sync(quarter);
+        delta = sh_delta[quarter * 32 + lane];
+        pair_sync(quarter);  // both have read it before the next item's is written
       }
-      pair_sync(quarter);
-      const float delta = sh_delta[quarter * 32 + lane];
-      pair_sync(quarter);  // both have read it before the next item's is written
       uint16_t* dst = reinterpret_cast<uint16_t*>(gr.dq) + row0 * gr.lddq + h * D + half * (D / 2);
       if (T == 0) {
         if (lane < rows) zero_row16<D / 2>(dst + lane * gr.lddq);
@@ -858,11 +866,8 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
       }
       // a row that saw no key has lse = -inf, which stays -inf here: its probabilities come out as zero
       const float nl = lse == -INFINITY ? -INFINITY : -lse * XA_LOG2E;
-      const uint64_t negl2 = f2(nl, nl), negd2 = f2(-delta, -delta);
-      if (half == 0 && lane < rows) {
-        gr.stats[stat + lane] = nl;
-        gr.stats[(long long)p.heads * p.total_q + stat + lane] = -delta;
-      }
+      const uint64_t negl2 = f2(nl, nl);
+      if (half == 0 && lane < rows) gr.stats[stat + lane] = nl;
       bool bad = false;
       int left = s.seen;
       for (int t = 0; t < T; ++t, ++g, left -= XA_BN) {
@@ -873,7 +878,26 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
         // the dS that last lay in this tile's columns has been multiplied (D = 128: dP was multiplied after it)
         if (C::SEP && g > 1 && !bar_wait(&dq_full[g & 1], ((g - 2) >> 1) & 1, abort_flag, 131)) bad = true;
         tc_fence_after();
-        if (rows > 0 && left > 32 * half) {  // else no row of this warp exists, or no column: nothing of it is used
+        const bool some = rows > 0 && left > 32 * half;  // else no row of this warp exists, or no column
+        // the sum of both halves of a row
+        auto pair_sum = [&](float x) {
+          float* c = sh_delta + quarter * 32 + lane;
+          if (half) *c = x;
+          pair_sync(quarter);
+          if (!half) *c = x += *c;
+          pair_sync(quarter);
+          x = *c;
+          pair_sync(quarter);  // before the next item's is written
+          return x;
+        };
+        auto keep = [&](uint32_t(&w)[16]) {
+          if (vis != 0xffffffffu) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              w[e] &= ((vis >> (2 * e)) & 1u ? 0x0000ffffu : 0u) | ((vis >> (2 * e + 1)) & 1u ? 0xffff0000u : 0u);
+          }
+        };
+        if (some) {
           uint32_t sc[32], dp[32], w[16];
           tmem_ld32_async(t_s, sc);
           tmem_ld32_async(t_s + 64, dp);
@@ -881,27 +905,46 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(sdp_empty);
+          if (single) {
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 x = f2_split(ffma2(f2(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), scale2, negl2));
-            const uint64_t pr = f2(fast_exp2(x.x), fast_exp2(x.y));
-            const float2 d = f2_split(fmul2(pr, fadd2(f2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), negd2)));
-            w[e >> 1] = pack_2(d.x, d.y, F16);
-          }
-          if (vis != 0xffffffffu) {
+            for (int e = 0; e < 32; e += 2) {
+              const float2 x = f2_split(ffma2(f2(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), scale2, negl2));
+              const float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
+              sc[e] = __float_as_uint(p0);
+              sc[e + 1] = __float_as_uint(p1);
+              // hidden columns may hold anything
+              if ((vis >> e) & 1u) part[(e >> 1) & 3] = fmaf(p0, __uint_as_float(dp[e]), part[(e >> 1) & 3]);
+              if ((vis >> (e + 1)) & 1u) part[(e >> 1) & 3] = fmaf(p1, __uint_as_float(dp[e + 1]), part[(e >> 1) & 3]);
+            }
+            delta = pair_sum((part[0] + part[1]) + (part[2] + part[3]));
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              w[e] &= ((vis >> (2 * e)) & 1u ? 0x0000ffffu : 0u) | ((vis >> (2 * e + 1)) & 1u ? 0xffff0000u : 0u);
+            for (int e = 0; e < 32; e += 2)
+              w[e >> 1] = pack_2(__uint_as_float(sc[e]) * (__uint_as_float(dp[e]) - delta),
+                                 __uint_as_float(sc[e + 1]) * (__uint_as_float(dp[e + 1]) - delta), F16);
+          } else {
+            const uint64_t negd2 = f2(-delta, -delta);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 x = f2_split(ffma2(f2(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), scale2, negl2));
+              const uint64_t pr = f2(fast_exp2(x.x), fast_exp2(x.y));
+              const float2 d =
+                  f2_split(fmul2(pr, fadd2(f2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), negd2)));
+              w[e >> 1] = pack_2(d.x, d.y, F16);
+            }
           }
+          keep(w);
           tmem_st16(t_ds, w);
           tmem_wait_st();
-        } else if (lane == 0) {
-          mbar_arrive(sdp_empty);
+        } else {
+          if (lane == 0) mbar_arrive(sdp_empty);
+          if (single && rows > 0) delta = pair_sum(0.f);
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ds_full[g & 1]);
       }
+      if (half == 0 && lane < rows) gr.stats[(long long)p.heads * p.total_q + stat + lane] = -delta;
       if (!bar_wait(&dq_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, 132)) bad = true;
       tc_fence_after();
       const int put = bad || *abort_flag ? 0 : rows;
@@ -926,9 +969,10 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
 // the group, or a part of them when there are fewer key tiles than SMs: the parts are then written in fp32 and added
 // in a fixed order by a second launch, so results never depend on the order in which CTAs finish. The products are
 // taken transposed (S^T = K Q^T, dP^T = V dO^T), which puts P^T and dS^T into TMEM in the form of the A operand of
-// dV += P^T dO and dK += dS^T Q, with dO and Q read as they lie. Two score buffers, each with a softmax warpgroup of
-// its own: one forms P and dS while the tensor core works on the other. TMEM (512 columns): 2 x (S^T 64, dP^T 64),
-// dV, dK.
+// dV += P^T dO and dK += dS^T Q, with dO and Q read as they lie. Two score buffers, each with eight softmax warps of its
+// own (two to a row): they form P and dS while the tensor core works on the other. TMEM (512 columns): 2 x (S^T 64,
+// dP^T 64), dV, dK. Bound by the issuing warp's loop at D = 64 (16 products and two waits a tile: some 1500 cycles for
+// 656 of products; 105 us on 2 x 8247 queries x 257 keys x 24 heads), by the products at D = 128.
 constexpr int XB_THREADS = 576;  // warps 0..15 softmax (8 to a score buffer, two to a row), 16 loads, 17 MMA
 constexpr int XB_SOFTMAX = 8;
 template <int D>
@@ -1301,7 +1345,7 @@ static int check_common(const void* q, const void* k, const void* v, const void*
   if (batch < 0 || max_q < 0 || max_k < 0 || total_q < 0 || total_k < 0 || heads <= 0 || kv_heads <= 0 ||
       heads % kv_heads != 0)
     return SA3_ERR_ARG;
-  if (!(scale > 0.f) || scale > 3.4e38f) return SA3_ERR_ARG;
+  if (!(scale > 0.f) || !(scale * XA_LOG2E <= 3.4e38f)) return SA3_ERR_ARG;  // NaN and infinity fail both
   if (head_dim != 64 && head_dim != 128) return SA3_ERR_UNSUPPORTED;
   if (dtype != SA3_DT_BF16 && dtype != SA3_DT_F16) return SA3_ERR_DTYPE;
   if (!cu_q && (long long)batch * max_q != total_q) return SA3_ERR_ARG;

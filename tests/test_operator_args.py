@@ -52,6 +52,7 @@ SHARED = [
     (dict(heads=0), ARG), (dict(kv=0), ARG), (dict(kv=3), ARG), (dict(tq=9), ARG), (dict(tk=15), ARG),
     (dict(lq=-1, tq=0), ARG), (dict(ldq=255), ARG), (dict(ldk=64), ARG), (dict(ldv=64), ARG), (dict(ldo=128), ARG),
     (dict(scale=0.0), ARG), (dict(scale=-1.0), ARG), (dict(scale=math.nan), ARG), (dict(scale=math.inf), ARG),
+    (dict(scale=3e38), ARG),
     (dict(d=96, ldq=384, ldk=192, ldv=192, ldo=384), UNSUPPORTED), (dict(dtype=_lib.DT_F32), DTYPE),
     (dict(q=P + 8), ALIGN), (dict(k=P + 2), ALIGN), (dict(out=P + 8), ALIGN), (dict(ldq=260), ALIGN),
     (dict(ldv=132), ALIGN), (dict(lens=P + 1), ALIGN), (dict(lse=P + 2), ALIGN), (dict(cu_q=P + 2), ALIGN),
