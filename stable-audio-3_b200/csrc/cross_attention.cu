@@ -13,6 +13,8 @@
 //
 // Sums, softmax statistics and accumulators are fp32; P and dS are rounded once to the operands' 16-bit type, the
 // type of the matrix instructions.
+#include <type_traits>
+
 #include "attn_tile.cuh"
 #include "common.cuh"
 #include "cross_attention.cuh"
@@ -170,7 +172,8 @@ __device__ __forceinline__ void store_rows32(uint32_t t_src, float f, bool keep,
 // product. Packed ones number only the tiles that their sequences have (XA_SCAN sequences at most: finding an item's
 // sequence takes a step for each): CTA i takes items i, i + grid, .. of all sequences alike, where numbering the tiles
 // up to the longest sequence leaves some CTAs with few that exist (4 sequences of 1255 .. 2500 queries: 111 -> 77 us
-// forward, 172 -> 124 us dQ).
+// forward, 172 -> 124 us dQ). 64 sequences of 75 .. 435 queries, 24 heads of 64 columns: 124 -> 117 us forward, 478 ->
+// 422 us backward, but 70 -> 82 and 360 -> 370 where all are alike; 128 of half the length: 121 -> 143, 652 -> 638.
 constexpr int XA_SCAN = 64;
 template <int ROWS, int KEYS, bool SCAN>  // query rows of an item, keys of a tile, packed numbering
 struct XWalk {
@@ -1257,53 +1260,66 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const XParams p, const 
 }
 
 // The forward's output from the parts of the keys: out = sum_s exp(lse_s - lse) out_s, lse = log sum_s exp(lse_s).
-// A block takes a row of a head; its 8 warps take every eighth part, all loads in flight at once, and join in shared
+// WARPS warps take a row of a head: each reads every WARPS-th part, its loads in flight at once, and they join in shared
 // memory. grid (rows of a sequence x heads, sequence).
-template <int D>
+template <int D, int WARPS>
 __global__ void __launch_bounds__(256) cross_merge_kernel(const XParams p) {
+  constexpr int ROWS = 8 / WARPS, E = D / 32;
+  using V = typename std::conditional<E == 2, float2, float4>::type;
   __shared__ float sh[8][D];
   __shared__ float sh_l[8];
   grid_dep_wait();
   const XSeq s = make_seq(p, blockIdx.y);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WARPS;
   const long long n = (long long)s.lq * p.heads, one = (long long)p.heads * p.total_q;
-  for (long long at = blockIdx.x; at < n; at += gridDim.x) {
-    const int h = (int)(at % p.heads);
-    const long long row = s.qs + at / p.heads, src = (long long)h * p.total_q + row;
+  for (long long first = (long long)blockIdx.x * ROWS; first < n; first += (long long)gridDim.x * ROWS) {
+    const long long at = first + warp / WARPS;
+    const bool on = at < n;
+    const int h = on ? (int)(at % p.heads) : 0;
+    const long long row = s.qs + (on ? at / p.heads : 0), src = (long long)h * p.total_q + row;
     float top = -INFINITY;
-    for (int sp = lane; sp < p.parts; sp += 32) top = fmaxf(top, p.part_lse[sp * one + src]);
+    if (on)
+      for (int sp = lane; sp < p.parts; sp += 32) top = fmaxf(top, p.part_lse[sp * one + src]);
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    float a[D / 32], l = 0.f;
+    float a[E], l = 0.f;
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) a[e] = 0.f;
+    for (int e = 0; e < E; ++e) a[e] = 0.f;
+    if (on) {
 #pragma unroll 4
-    for (int sp = warp; sp < p.parts; sp += 8) {
-      // a part of weight zero may hold anything
-      const float e = p.part_lse[sp * one + src];
-      const float f = e == -INFINITY ? 0.f : fast_exp2((e - top) * XA_LOG2E);
-      const float* o = p.part_o + (sp * one + src) * D + lane;
-      l += f;
+      for (int sp = sub; sp < p.parts; sp += WARPS) {
+        // a part of weight zero may hold anything
+        const float e = p.part_lse[sp * one + src];
+        const float f = e == -INFINITY ? 0.f : fast_exp2((e - top) * XA_LOG2E);
+        const V v = *reinterpret_cast<const V*>(p.part_o + (sp * one + src) * D + E * lane);
+        const float* o = reinterpret_cast<const float*>(&v);
+        l += f;
 #pragma unroll
-      for (int x = 0; x < D / 32; ++x) {
-        const float v = o[32 * x];
-        a[x] = fmaf(f, f != 0.f ? v : 0.f, a[x]);
+        for (int x = 0; x < E; ++x) a[x] = fmaf(f, f != 0.f ? o[x] : 0.f, a[x]);
       }
     }
+    if (WARPS > 1) {
 #pragma unroll
-    for (int x = 0; x < D / 32; ++x) sh[warp][32 * x + lane] = a[x];
-    if (lane == 0) sh_l[warp] = l;
-    __syncthreads();
-    if (tid < D / 2) {
-      float x = 0.f, y = 0.f, t = 0.f;
+      for (int x = 0; x < E; ++x) sh[warp][E * lane + x] = a[x];
+      if (lane == 0) sh_l[warp] = l;
+      __syncthreads();
+      if (sub == 0) {
 #pragma unroll
-      for (int w = 0; w < 8; ++w) x += sh[w][2 * tid], y += sh[w][2 * tid + 1], t += sh_l[w];
-      const float inv = t > 0.f ? 1.f / t : 0.f;
-      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + h * D + 2 * tid;
-      *reinterpret_cast<uint32_t*>(dst) = pack_2(x * inv, y * inv, p.f16);
-      if (tid == 0 && p.lse) p.lse[src] = t > 0.f ? top + __log2f(t) * 0.6931471805599453f : -INFINITY;
+        for (int w = 1; w < WARPS; ++w) {
+#pragma unroll
+          for (int x = 0; x < E; ++x) a[x] += sh[warp + w][E * lane + x];
+          l += sh_l[warp + w];
+        }
+      }
     }
-    __syncthreads();
+    if (on && sub == 0) {
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.out) + row * p.ldo + h * D + E * lane);
+#pragma unroll
+      for (int x = 0; x < E; x += 2) dst[x / 2] = pack_2(a[x] * inv, a[x + 1] * inv, p.f16);
+      if (lane == 0 && p.lse) p.lse[src] = l > 0.f ? top + __log2f(l) * 0.6931471805599453f : -INFINITY;
+    }
+    if (WARPS > 1) __syncthreads();
   }
 }
 
@@ -1474,14 +1490,30 @@ static long long fwd_bytes(int parts, int heads, int total_q, int head_dim) {
 // the row statistics first, the parts of dK and dV behind them at a 16-byte boundary
 static long long stats_bytes(int heads, int total_q) { return (((long long)heads * total_q * 8) + 15) & ~15LL; }
 
-// Parts of the keys in the forward (one CTA each, joined by a second launch): when the query tiles alone leave half of
-// the CTA slots empty and every part still has 8 key tiles or more.
-static int fwd_parts(int batch, int max_q, int max_k, int heads, int kv_heads, int sms) {
+// Parts of the keys in the forward (one CTA each, joined by a second launch) while the query tiles alone leave CTA slots
+// empty: the number that ends soonest by these measured times. A step of 64 keys takes 1.3 us (D = 64; 1.6 with both
+// units at work) or 0.9 us (D = 128) alone on an SM, 1.45 / 2.8 / 1.4 us with two CTAs there, an item 2 us besides;
+// the joining launch 3 us, 0.1 us a part, and its bytes at 3 TB/s. 8 heads of 64 columns, 64 queries, 8192 keys: 168,
+// 89, 49, 29, 20, 19 us with 1, 2, 4, .. 32 parts; 148 heads of 128 columns, 128 queries: 137, 114, 127 with 1, 2, 4.
+static int fwd_parts(int batch, int max_q, int max_k, int heads, int kv_heads, int head_dim, int sms) {
   if (batch <= 0 || max_q <= 0) return 1;
   if ((long long)max_q * (heads / kv_heads) <= XT_MAX_ROWS) return cross_token_parts(batch, kv_heads, max_k, sms);
-  const long long items = (long long)((max_q + XA_BM - 1) / XA_BM) * heads * batch;
-  const long long fill = 2LL * sms / items, most = max_k / (8 * XA_BN), n = fill < most ? fill : most;
-  return n >= 2 ? (int)n : 1;
+  const bool narrow = head_dim == 64, pair = narrow && max_q > XA_BM;
+  const int rows = pair ? 2 * XA_BM : XA_BM;
+  const long long items = (long long)((max_q + rows - 1) / rows) * heads * batch, fill = 2LL * sms / items;
+  const int tiles = (max_k + XA_BN - 1) / XA_BN;
+  const float alone = narrow ? pair ? 1.6f : 1.3f : 0.9f, both = narrow ? pair ? 2.8f : 1.45f : 1.4f;
+  const float join = (float)heads * batch * max_q * head_dim * 8e-6f / 3.f;
+  int best = 1;
+  float cost = 0.f;
+  for (int n = 1; n <= fill && n <= 64 && (n == 1 || 2 * n <= tiles); ++n) {
+    const float c = (tiles + n - 1) / n * (items * n > sms ? both : alone) + 2.f + (n > 1 ? 3.f + n * (0.1f + join) : 0.f);
+    if (n == 1 || c < cost) {
+      cost = c;
+      best = n;
+    }
+  }
+  return best;
 }
 
 static int bwd_splits(int batch, int max_q, int max_k, int total_q, int total_k, int heads, int kv_heads, int sms) {
@@ -1514,7 +1546,7 @@ extern "C" int sa3_cross_attention(const void* q, const void* k, const void* v, 
   if (sms <= 0) return SA3_ERR_LAUNCH;
   XParams p = make_params(out, lse, cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, batch, max_seqlen_q, max_seqlen_k,
                           total_q, total_k, heads, kv_heads, ldo, softmax_scale, dtype);
-  p.parts = fwd_parts(batch, max_seqlen_q, max_seqlen_k, heads, kv_heads, sms);
+  p.parts = fwd_parts(batch, max_seqlen_q, max_seqlen_k, heads, kv_heads, head_dim, sms);
   if (p.parts > 1) {
     if (!workspace || workspace_bytes < fwd_bytes(p.parts, heads, total_q, head_dim)) return SA3_ERR_ARG;
     if (!aligned16(workspace)) return SA3_ERR_ALIGN;
@@ -1528,8 +1560,14 @@ extern "C" int sa3_cross_attention(const void* q, const void* k, const void* v, 
     rc = (head_dim == 64 ? p.f16 ? launch_fwd<64, true> : launch_fwd<64, false>
                          : p.f16 ? launch_fwd<128, true> : launch_fwd<128, false>)(p, q, k, v, ldq, ldk, ldv, sms, st);
   if (rc || p.parts == 1) return rc;
-  const dim3 grid = rows_grid((long long)max_seqlen_q * heads * 256, batch, sms);
-  launch_ex(head_dim == 64 ? cross_merge_kernel<64> : cross_merge_kernel<128>, grid, dim3(256), 0, st, 1, p);
+  // 8 warps a row where there are many parts and no more rows than blocks that run at once (32 parts of 136 rows: 52.4
+  // against 55.5 us with one warp, in all); else a warp a row (8 parts of 8192 rows: 51.6 against 81.3 us).
+  const long long all_rows = (long long)max_seqlen_q * heads * batch;
+  const bool few = p.parts <= 16 || all_rows > 8LL * sms;
+  const dim3 grid = rows_grid((long long)max_seqlen_q * heads * (few ? 32 : 256), batch, sms);
+  launch_ex(head_dim == 64 ? few ? cross_merge_kernel<64, 1> : cross_merge_kernel<64, 8>
+                           : few ? cross_merge_kernel<128, 1> : cross_merge_kernel<128, 8>,
+            grid, dim3(256), 0, st, 1, p);
   return launch_status();
 }
 
@@ -1541,7 +1579,7 @@ extern "C" int sa3_cross_attention_workspace(int batch, int max_seqlen_q, int ma
   if (head_dim != 64 && head_dim != 128) return SA3_ERR_UNSUPPORTED;
   const int sms = sm_count();
   if (sms <= 0) return SA3_ERR_LAUNCH;
-  const int n = fwd_parts(batch, max_seqlen_q, max_seqlen_k, heads, kv_heads, sms);
+  const int n = fwd_parts(batch, max_seqlen_q, max_seqlen_k, heads, kv_heads, head_dim, sms);
   *bytes = n > 1 ? fwd_bytes(n, heads, total_q, head_dim) : 0;
   return SA3_OK;
 }

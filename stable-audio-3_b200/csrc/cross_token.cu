@@ -27,7 +27,9 @@ constexpr int XT_WARPS = 4;
 constexpr int XT_THREADS = XT_WARPS * 32;
 constexpr int XT_KEYS = 16;          // keys of a step of a warp
 constexpr int XT_MAX_CLUSTER = 8;
-constexpr int XT_PART_KEYS = 512;    // least keys of a part of the split without clusters: 8 steps of a warp
+constexpr int XT_PART_KEYS = 256;    // least keys of a part of the split without clusters: 4 steps of a warp
+constexpr int XT_MAX_PARTS = 128;
+constexpr int XT_SPLIT_KEYS = 8192;  // keys from which that split is worth its second launch
 constexpr float XT_RESCALE_LOG2 = 8.f;
 // Steps in flight: 96 KB a CTA at either width, two CTAs an SM.
 template <int D>
@@ -368,15 +370,20 @@ static int launch_token(const XTokenParams& a, int csize, int sms, cudaStream_t 
 }
 
 // Parts of the keys that are joined by a second launch: when even clusters of 8 leave SMs empty and the keys are
-// long enough to pay for that launch. Two CTAs an SM.
+// long enough to pay for that launch. Two CTAs an SM. 8 key heads of 64 columns, cluster against parts: 7.5 and 7.9 us
+// at 4096 keys, 10.4 and 10.0 at 8192, 49.9 and 27.0 at 65536; one key head of 128 columns and 8192 keys: 13.2 us in a
+// cluster, 11.4, 8.6, 8.0 with 16, 32, 64 parts; 65536 keys: 13.9 with 128, 15.1 with 256.
 int cross_token_parts(int batch, int kv_heads, int max_k, int sms) {
   const long long units = (long long)batch * kv_heads;
-  if (units * XT_MAX_CLUSTER >= sms || max_k < 2 * XT_MAX_CLUSTER * XT_PART_KEYS) return 1;
+  if (units * XT_MAX_CLUSTER >= sms || max_k < XT_SPLIT_KEYS) return 1;
   const long long fill = 2LL * sms / units, most = max_k / XT_PART_KEYS;
-  return (int)(fill < most ? fill : most);
+  const long long n = fill < most ? fill : most;
+  return (int)(n < XT_MAX_PARTS ? n : XT_MAX_PARTS);
 }
 
-// Cluster size: more CTAs to a key head while the launch leaves room for them and every warp still has a step of keys.
+// Cluster size: more CTAs to a key head while the launch leaves room for them and every warp still has a step of keys
+// (8 key heads of 64 columns, 4096 keys: 26.6, 15.5, 10.3, 7.5 us with 1, 2, 4, 8; 16 sequences of 1024 keys: 10.7,
+// 10.0, 14.7, 22.8).
 int cross_token(const XParams& p, const void* q, const void* k, const void* v, long long ldq, long long ldk,
                 long long ldv, int head_dim, int sms, cudaStream_t st) {
   XTokenParams a = {p, q, k, v, ldq, ldk, ldv};

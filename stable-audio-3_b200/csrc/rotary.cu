@@ -15,7 +15,8 @@
 // rpb * r/2 cosines and sines into shared memory (once for all heads), while each thread's first data loads are
 // already in flight. A thread keeps one unit of the head (2 * VEC elements: VEC pairs, or 2 * VEC columns that
 // pass through) and walks heads and rows. VEC is the widest vector that the alignment of every pointer, stride
-// and part of the head allows, up to 16 bytes.
+// and part of the head allows, up to 16 bytes (16494 rows x 48 heads x 64 of bf16: 32.6, 43.2, 56.2, 99.6 us with
+// 16, 8, 4, 2 bytes).
 #include "common.cuh"
 #include "host_util.h"
 
@@ -178,9 +179,11 @@ int launch_rotary(RotaryParams p, bool il, bool in_place, cudaStream_t st) {
   const int turns = (total + most - 1) / most;
   p.heads_par = (total + turns - 1) / turns;
   const int threads = p.units * p.heads_par;
-  // More rows to a block save blocks and overlap one's angles with another's data once every SM has several blocks
-  // (1, 2, 4, 8 rows: 51, 44, 41, 40 us for 16494 rows x 48 heads); below that one row each spreads the work.
-  p.rpb = p.rows >= 148LL * 8 * ROT_MAX_RPB ? ROT_MAX_RPB : 1;
+  // More rows to a block save blocks and overlap one's angles with another's data once every SM has several blocks; below
+  // that one row each spreads the work. 1, 2, 4 rows: 2.1, 2.2, 3.0 us for 256 rows of 48 heads x 64, 6.2, 6.0, 6.1 for
+  // 2400, 38.0, 33.4, 32.6 for 16494; 3.8, 3.6, 4.5 for 2400 rows of 8 heads x 128, 13.4, 13.2, 13.7 for 16494.
+  const bool wide = p.rows >= 148 * 64 && total * p.dim * (int)sizeof(T) > 4096;
+  p.rpb = p.rows < 148 * 16 ? 1 : wide ? ROT_MAX_RPB : 2;
   // Outputs above a quarter of L2 are stored evict-first: 39.7 -> 33.5 us for 101 MB out of a fused buffer (16494 rows x
   // 48 heads x 64), 69 -> 65 us for 210 MB. Smaller ones are left for the attention that reads them next.
   p.stream = p.rows * total * p.dim * (long long)sizeof(T) > (32LL << 20);
