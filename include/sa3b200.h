@@ -293,7 +293,8 @@ int sa3_rotary(const void* q, void* q_out, const void* k, void* k_out, int dtype
  * of key_mask (uint8 [total_k] or NULL) is nonzero. Hidden keys may hold anything. A row without visible keys gives
  * out = 0, lse = -inf and zero gradients. Rows outside all sequences are left as they are.
  * lse (fp32 [heads, total_q], or NULL): natural log of the sum of the exponentials.
- * softmax_scale > 0. Zero lengths and batches are valid.
+ * softmax_scale > 0. Zero lengths and batches are valid. No output overlaps an input or another output; they may be
+ * column ranges of one buffer.
  * At most 16 query rows a key head (max_seqlen_q * heads / kv_heads, e.g. one decoded token) take a kernel that
  * splits the keys over a cluster; the rest take a tcgen05 kernel. With few query rows and long keys either splits the
  * keys over CTAs that a second launch joins (in a fixed order). That needs a workspace: 16-byte aligned device memory

@@ -1542,6 +1542,7 @@ extern "C" int sa3_cross_attention(const void* q, const void* k, const void* v, 
   if (rc) return rc;
   if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(k_lens)) & 3) return SA3_ERR_ALIGN;
   if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return SA3_OK;
+  if (out == q || (total_k > 0 && (out == k || out == v))) return SA3_ERR_ARG;
   const int sms = sm_count();
   if (sms <= 0) return SA3_ERR_LAUNCH;
   XParams p = make_params(out, lse, cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, batch, max_seqlen_q, max_seqlen_k,
@@ -1617,6 +1618,14 @@ extern "C" int sa3_cross_attention_bwd(const void* dout, const void* q, const vo
     return SA3_ERR_ALIGN;
   if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(k_lens)) & 3) return SA3_ERR_ALIGN;
   if (batch == 0 || (total_q == 0 && total_k == 0)) return SA3_OK;
+  // the dK / dV kernel reads q and dout after dq is written
+  const void* rows_q[] = {dout, q, out, dq};
+  const void* rows_k[] = {k, v, dk, dv};
+  for (const void* y : {(const void*)dq, (const void*)dk, (const void*)dv}) {
+    int same = 0;
+    for (int i = 0; i < 4; ++i) same += (total_q > 0 && rows_q[i] == y) + (total_k > 0 && rows_k[i] == y);
+    if (same > 1) return SA3_ERR_ARG;
+  }
   const int sms = sm_count();
   if (sms <= 0) return SA3_ERR_LAUNCH;
   const int splits = bwd_splits(batch, max_seqlen_q, max_seqlen_k, total_q, total_k, heads, kv_heads, sms);

@@ -217,6 +217,8 @@ extern "C" int sa3_rotary(const void* q, void* q_out, const void* k, void* k_out
   if (!q || !q_out || !inv_freq) return SA3_ERR_ARG;
   const uintptr_t any = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) |
                         reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(k_out);
+  if ((q == q_out && ldq != ldqo && rows > 1) || (k && k == k_out && ldk != ldko && rows > 1)) return SA3_ERR_ARG;
+  if (k && (q_out == k_out || q_out == k || k_out == q)) return SA3_ERR_ARG;
   if (any % esz || (reinterpret_cast<uintptr_t>(inv_freq) & 7) || (reinterpret_cast<uintptr_t>(row_pos) & 3))
     return SA3_ERR_ALIGN;
 

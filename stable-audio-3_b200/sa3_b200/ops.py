@@ -451,8 +451,8 @@ def _cross_args(q, k, v, heads, kv_heads, head_dim, batch, max_seqlen_q, max_seq
         batch = cu_seqlens_q.numel() - 1
     elif cu_seqlens_k is not None:
         batch = cu_seqlens_k.numel() - 1
-    if batch < 0 or max_seqlen_q < 0 or max_seqlen_k < 0:
-        raise RuntimeError("batch and lengths must not be negative")
+    if min(batch, max_seqlen_q, max_seqlen_k) < 0 or max(max_seqlen_q, max_seqlen_k) >= 2 ** 31:
+        raise RuntimeError("batch and lengths must not be negative, and lengths below 2**31")
     if cu_seqlens_q is None and rows != batch * max_seqlen_q:
         raise RuntimeError("uniform queries need rows = batch * max_seqlen_q")
     if cu_seqlens_k is None and krows != batch * max_seqlen_k:
@@ -495,7 +495,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, heads:
     Uniform sequences of max_seqlen_q / max_seqlen_k rows, or packed ones: cu_seqlens_q / cu_seqlens_k (int32
     [batch + 1], each optional), with max_seqlen the longest. k_lens (int32 [batch]): how many keys of a sequence are
     visible; key_mask (bool or uint8, one element a key row): zero hides a key. Rows that see no key give zeros and
-    lse = -inf. Scratch, where it is needed, comes from torch's allocator on the current stream. Returns out, or (out, lse) with return_lse (lse fp32 [heads, rows], which the backward pass takes).
+    lse = -inf. Scratch, where it is needed, comes from torch's allocator on the current stream. Returns out, or
+    (out, lse) with return_lse (lse fp32 [heads, rows], which the backward pass takes).
     """
     dev = _device_of(q, k, v, cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, out, lse)
     kv_heads, ld, idx, batch, scale = _cross_args(q, k, v, heads, kv_heads, head_dim, batch, max_seqlen_q, max_seqlen_k,

@@ -227,3 +227,43 @@ def test_large_scores_move_the_reference_maximum(cuda, d):
     """Scores spread over hundreds: the running maximum moves in most tiles."""
     run_case(cuda, 1, 200, 700, 2, 1, d, "bf16", spread=30.0, backward=False)
     run_case(cuda, 1, 1, 700, 2, 1, d, "fp16", spread=30.0, backward=False)
+
+
+def test_refuses_lengths_beyond_32_bits():
+    """Lengths that the library's 32-bit arguments would cut are refused before the call."""
+    from sa3_b200 import ops
+
+    x = torch.zeros(8, 64, device="cuda", dtype=torch.bfloat16)
+    cu = torch.tensor([0, 8], dtype=torch.int32, device="cuda")
+    for kw in (dict(max_seqlen_q=2 ** 32 + 8, max_seqlen_k=8), dict(max_seqlen_q=8, max_seqlen_k=2 ** 31)):
+        with pytest.raises(RuntimeError, match="2\\*\\*31"):
+            ops.cross_attention(x, x, x, heads=1, cu_seqlens_q=cu, cu_seqlens_k=cu, **kw)
+    with pytest.raises(RuntimeError):
+        ops.cross_attention(x, x.clone(), x.clone(), heads=1, cu_seqlens_q=cu, cu_seqlens_k=cu, max_seqlen_q=8,
+                            max_seqlen_k=8, out=x)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,lk,heads", [(40, 2048, 2), (129, 1030, 3), (300, 640, 4), (33, 9000, 8), (200, 4096, 1)])
+def test_parts_of_the_keys(d, lq, lk, heads):
+    """Long keys for few query rows are read in parts, joined by a warp or a block a row: against fp64, with lse."""
+    from sa3_b200 import ops
+
+    g = torch.Generator(device="cuda").manual_seed(lq + lk)
+    q, k, v = (torch.randn(n, heads * d, device="cuda", generator=g).bfloat16() for n in (lq, lk, lk))
+    mask = torch.rand(lk, device="cuda", generator=g) < 0.7
+    mask[:lk // 2] = False  # whole parts are hidden
+    o, lse = ops.cross_attention(q, k, v, heads=heads, head_dim=d, max_seqlen_q=lq, max_seqlen_k=lk, key_mask=mask,
+                                 return_lse=True)
+    qd, kd, vd = (t.double().view(-1, heads, d).transpose(0, 1) for t in (q, k, v))
+    s = (qd @ kd.transpose(1, 2)) * d ** -0.5
+    s = s.masked_fill(~mask, -math.inf)
+    want_l = torch.logsumexp(s, -1)
+    p = (s - want_l[..., None]).exp()
+    want = (p @ vd).transpose(0, 1).reshape(lq, -1)
+    # P is rounded to bf16 (2^-8 a term, against sum p|v|), O likewise; fp32 sums and exponentials: 2^-16 in all
+    room = (p @ vd.abs()).transpose(0, 1).reshape(lq, -1) * (2 ** -8 + 2 ** -16) + want.abs() * 2 ** -8 * 1.01
+    assert bool(((o.double() - want).abs() <= room + 1e-30).all())
+    # scores: fp32 sums of d products, each partial sum at most |q||k|
+    off = (qd.abs() @ kd.abs().transpose(1, 2)).amax(-1) * d ** -0.5 * d * 2 ** -24 + 2 ** -18 * (1 + want_l.abs())
+    assert bool(((lse.double() - want_l).abs() <= off).all())

@@ -77,6 +77,29 @@ def test_backward_refuses(kw, rc):
     assert backward(**kw) == rc
 
 
+A, B = 0x200000, 0x300000
+
+
+@pytest.mark.parametrize("kw", [
+    dict(qo=P, ldqo=256), dict(qo=A, k=P, ko=A, kv=2, ldk=128, ldko=128), dict(qo=A, k=A, ko=B, kv=2, ldk=128, ldko=128),
+    dict(qo=A, k=B, ko=P, kv=2, ldk=128, ldko=128), dict(qo=A, k=B, ko=B, kv=2, ldk=128, ldko=256),
+])
+def test_rotary_refuses_overlaps(kw):
+    assert rotary(**kw) == ARG
+
+
+@pytest.mark.parametrize("kw", [dict(out=P), dict(out=A, k=A), dict(out=A, v=A)])
+def test_forward_refuses_overlaps(kw):
+    assert forward(**kw) == ARG
+
+
+@pytest.mark.parametrize("which", [("dq", "dout"), ("dq", "q"), ("dq", "out"), ("dq", "k"), ("dk", "k"), ("dk", "dq"),
+                                   ("dk", "dout"), ("dv", "v"), ("dv", "dk"), ("dv", "q")])
+def test_backward_refuses_overlaps(which):
+    own = {n: P + i * 0x100000 for i, n in enumerate(("dout", "q", "k", "v", "out", "dq", "dk", "dv"))}
+    assert backward(**{**own, which[0]: own[which[1]]}) == ARG
+
+
 def test_workspace_queries_refuse():
     lib = _lib.load()
     n = ctypes.c_longlong(0)
