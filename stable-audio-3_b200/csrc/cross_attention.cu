@@ -169,20 +169,76 @@ __device__ __forceinline__ void store_rows32(uint32_t t_src, float f, bool keep,
 
 // The walk of a persistent CTA over work items: query rows (fastest), head, part of the keys, sequence. Every role of
 // the CTA walks by itself. Uniform batches step by the grid without divisions, which would delay each item's first
-// product. Packed ones number only the tiles that their sequences have (XA_SCAN sequences at most: finding an item's
-// sequence takes a step for each): CTA i takes items i, i + grid, .. of all sequences alike, where numbering the tiles
-// up to the longest sequence leaves some CTAs with few that exist (4 sequences of 1255 .. 2500 queries: 111 -> 77 us
-// forward, 172 -> 124 us dQ). 64 sequences of 75 .. 435 queries, 24 heads of 64 columns: 124 -> 117 us forward, 478 ->
-// 422 us backward, but 70 -> 82 and 360 -> 370 where all are alike; 128 of half the length: 121 -> 143, 652 -> 638.
+// product. Packed ones number only the tiles that their sequences have: numbering the tiles up to the longest sequence
+// leaves some CTAs with few that exist (4 sequences of 1255 .. 2500 queries: 111 -> 69 us forward, 172 -> 106 us dQ).
+// XA_SCAN sequences at most, since a CTA orders them first and finding an item's sequence takes a step for each: 64 of
+// 75 .. 435 queries, 24 heads of 64 columns: 123 -> 105 us forward, 476 -> 413 backward, and 69 -> 73, 358 -> 362 where
+// all are alike; 128 of half the length, without the order: 121 -> 143, 652 -> 638.
 constexpr int XA_SCAN = 64;
+// The sequences of a packed batch in the order of their items: longest keys first, so that no CTA begins with a long
+// item when the others are done. Where the key tiles differ, the CTAs take every other round of items backwards: the
+// one with a round's longest has the next round's shortest (337 -> 315 us for the four sequences, both passes; with
+// equal keys that only costs, 67 -> 72 us forward for 16384 queries x 257 keys x 24 heads).
+struct XOrder {
+  int back;                 // whether
+  int starts[XA_SCAN + 1];  // items before the sequence, and all items
+  uint8_t seq[XA_SCAN];
+};
+constexpr int XA_ORDER = sizeof(XOrder);
+// By one warp, for batches of 1 .. XA_SCAN.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ void make_order(XOrder* o, const XParams& p, int lane) {
+  static_assert(XA_SCAN == 64, "two sequences a lane");
+  int keys[2], items[2], rank[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int b = 32 * e + lane;
+    keys[e] = items[e] = 0;
+    if (b < p.batch) {
+      const XSeq s = make_seq(p, b);
+      keys[e] = s.seen;
+      items[e] = (s.lq + ROWS - 1) / ROWS * p.heads * p.parts;
+    }
+  }
+  int most = 0, least = 0x7fffffff;
+  for (int b = 0; b < p.batch; ++b) {
+    const int x = __shfl_sync(0xffffffffu, b < 32 ? keys[0] : keys[1], b & 31);
+    most = max(most, x);
+    least = min(least, x);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) rank[e] += x > keys[e] || (x == keys[e] && b < 32 * e + lane);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (32 * e + lane < p.batch) {
+      o->seq[rank[e]] = (uint8_t)(32 * e + lane);
+      o->starts[rank[e] + 1] = items[e];
+    }
+  }
+  __syncwarp();
+  const int at = 2 * lane;
+  const int x = at < p.batch ? o->starts[at + 1] : 0, y = at + 1 < p.batch ? o->starts[at + 2] : 0;
+  int sum = x + y;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += up;
+  }
+  if (lane == 0) {
+    o->starts[0] = 0;
+    o->back = (most + KEYS - 1) / KEYS != (least + KEYS - 1) / KEYS;
+  }
+  if (at < p.batch) o->starts[at + 1] = sum - y;
+  if (at + 1 < p.batch) o->starts[at + 2] = sum;
+}
 template <int ROWS, int KEYS, bool SCAN>  // query rows of an item, keys of a tile, packed numbering
 struct XWalk {
   XSeq s;
-  int tile, h, part, b;  // the item
+  int tile, h, part, b;  // the item; b: packed, its place in the order
   int j0, T;             // its keys: from j0, in T tiles; T = 0 also for a tile behind the end of its sequence
   bool live;             // there is an item
   int item, dt, dh, dp, db, qtiles;
-  int start, count;  // packed: items before this sequence's, and its own
+  const XOrder* order;
   __device__ __forceinline__ void load(const XParams& p) {
     const int all = tile * ROWS < s.lq ? (s.seen + KEYS - 1) / KEYS : 0;
     T = all;
@@ -195,27 +251,28 @@ struct XWalk {
   }
   // packed: the sequence, tile, head and part of `item`
   __device__ __forceinline__ void find(const XParams& p) {
-    while (item >= start + count) {
-      start += count;
-      if (++b >= p.batch) {
+    const int was = b;
+    if (b < 0) b = 0;
+    while (item >= order->starts[b + 1]) {
+      if (++b == p.batch) {
         live = false;
         return;
       }
-      s = make_seq(p, b);
-      count = (s.lq + ROWS - 1) / ROWS * p.heads * p.parts;
     }
+    if (b != was) s = make_seq(p, order->seq[b]);
     const int tiles = (s.lq + ROWS - 1) / ROWS;
-    int x = item - start;
+    int x = item - order->starts[b];
     tile = x % tiles, x /= tiles, h = x % p.heads, part = x / p.heads;
     load(p);
   }
-  __device__ __forceinline__ XWalk(const XParams& p, int qt, int num_items) {
+  __device__ __forceinline__ XWalk(const XParams& p, int qt, int num_items, const XOrder* o) {
     qtiles = qt;
     int x = item = blockIdx.x;
     live = item < num_items;
     if (SCAN) {
-      start = count = 0;
+      order = o;
       b = -1;
+      dt = o->back ? 2 * (int)(gridDim.x - blockIdx.x) - 1 : gridDim.x;
       if (live) find(p);
       return;
     }
@@ -228,7 +285,12 @@ struct XWalk {
     }
   }
   __device__ __forceinline__ void next(const XParams& p, int num_items) {
-    item += gridDim.x;
+    if (SCAN) {
+      item += dt;
+      dt = 2 * (int)gridDim.x - dt;
+    } else {
+      item += gridDim.x;
+    }
     live = item < num_items;
     if (!live) return;
     if (SCAN) {
@@ -289,7 +351,7 @@ struct XFwd {
   static constexpr int Q_BYTES = SUBS * XA_SUB_M, T_BYTES = SUBS * SUB_N;
   static constexpr int TILES = UNITS * QS * Q_BYTES + 2 * KS * T_BYTES;
   static constexpr int CW = D == 64 ? 32 : 64, STAGE = 64 * CW;  // columns of a store pass, bytes of a warp's
-  static constexpr int SMEM = TILES + SOFTMAX * STAGE + 320;
+  static constexpr int SMEM = TILES + SOFTMAX * STAGE + 320 + XA_ORDER;
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
@@ -325,6 +387,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   static_assert(NBARS * 8 + 8 <= 320, "barriers");
+  XOrder* order = reinterpret_cast<XOrder*>(bars + 40);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -345,6 +408,10 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   grid_dep_wait();
+  if (SCAN) {
+    if (warp == 0) make_order<U * XA_BM, BN>(order, p, lane);
+    __syncthreads();
+  }
   // units of an item that have query rows
   auto units_of = [&](const Walk& it) { return U == 1 || (it.tile * U + 1) * XA_BM >= it.s.lq ? 1 : U; };
 
@@ -353,7 +420,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
     if (lane == 0) {
       int g = 0, qc[2] = {0, 0};
       bool ok = true, v_out = true;  // v_out: V of the last counted tile was issued
-      for (Walk it(p, qtiles, num_items); it.live && ok; it.next(p, num_items)) {
+      for (Walk it(p, qtiles, num_items, order); it.live && ok; it.next(p, num_items)) {
         if (it.T == 0) continue;
         const XSeq& s = it.s;
         const int cq = it.h * D, ck = (it.h / p.group) * D, nu = units_of(it);
@@ -413,7 +480,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
     uint64_t *my_s = &s_full[2 * u], *my_p = &p_full[2 * u], *my_o = &o_full[2 * u];
     int g = 0, gn = 0, qc = 0;  // key tiles seen, steps of this unit's items, its items
     bool ok = true;
-    for (Walk it(p, qtiles, num_items); it.live && ok; it.next(p, num_items)) {
+    for (Walk it(p, qtiles, num_items, order); it.live && ok; it.next(p, num_items)) {
       const int T = uniform_int(it.T);
       if (T == 0) continue;
       if (u >= uniform_int(units_of(it))) {
@@ -497,7 +564,7 @@ __global__ void __launch_bounds__(XFwd<D>::THREADS, 2)
     const float NEG_INF = -INFINITY;
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
     int gn = 0;
-    for (Walk it(p, qtiles, num_items); it.live; it.next(p, num_items)) {
+    for (Walk it(p, qtiles, num_items, order); it.live; it.next(p, num_items)) {
       const XSeq& s = it.s;
       const int T = it.T, i0 = (it.tile * U + u) * XA_BM;
       if (i0 >= s.lq) continue;
@@ -621,7 +688,7 @@ struct XDq {
   static constexpr int TILES = 2 * QS * Q_BYTES + (KS + VS) * T_BYTES;
   // at D = 128 there is no room to stage the stores
   static constexpr int STAGE = SEP ? XA_SOFTMAX * XA_STAGE : 0;
-  static constexpr int SMEM = TILES + STAGE + XA_BM * 4 + 256;
+  static constexpr int SMEM = TILES + STAGE + XA_BM * 4 + 176 + XA_ORDER;
   static constexpr int COL_DQ = 128, COL_DS = SEP ? 192 : 64;
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
 };
@@ -658,7 +725,8 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
   constexpr int NBARS = 21;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert(NBARS * 8 + 8 <= 256, "barriers");
+  static_assert(NBARS * 8 + 8 <= 176, "barriers");
+  XOrder* order = reinterpret_cast<XOrder*>(bars + 22);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -679,13 +747,17 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   grid_dep_wait();
+  if (SCAN) {
+    if (warp == 0) make_order<XA_BM, XA_BN>(order, p, lane);
+    __syncthreads();
+  }
 
   if (warp >= XA_SOFTMAX) regs_low();
   if (warp == 8) {
     if (lane == 0) {
       int g = 0, qc = 0;
       bool ok = true, v_out = true;  // v_out: V of the last counted tile was issued
-      for (XWalk<XA_BM, XA_BN, SCAN> it(p, qtiles, num_items); it.live && ok; it.next(p, num_items)) {
+      for (XWalk<XA_BM, XA_BN, SCAN> it(p, qtiles, num_items, order); it.live && ok; it.next(p, num_items)) {
         if (it.T == 0) continue;
         const XSeq& s = it.s;
         const int cq = it.h * D, ck = (it.h / p.group) * D;
@@ -696,7 +768,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
           tma_load_2d(sQ(qs) + c * XA_SUB_M, &tmQ, &q_full[qs], cq + 64 * c, s.qs + it.tile * XA_BM);
           tma_load_2d(sDO(qs) + c * XA_SUB_M, &tmDO, &q_full[qs], cq + 64 * c, s.qs + it.tile * XA_BM);
           // O of these rows, which the softmax warps read for delta when they get to the item
-          tma_prefetch_l2_2d(&tmO, cq + 64 * c, s.qs + it.tile * XA_BM);
+          if (it.T > 1) tma_prefetch_l2_2d(&tmO, cq + 64 * c, s.qs + it.tile * XA_BM);
         }
         qc++;
         for (int t = 0; t < it.T; ++t, ++g) {
@@ -733,7 +805,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     const uint32_t idesc_full = make_idesc(128, XA_BN, fmt, fmt, 0, 0);
     int g = 0, qc = 0;
     bool ok = true;
-    for (XWalk<XA_BM, XA_BN, SCAN> it(p, qtiles, num_items); it.live && ok; it.next(p, num_items)) {
+    for (XWalk<XA_BM, XA_BN, SCAN> it(p, qtiles, num_items, order); it.live && ok; it.next(p, num_items)) {
       const int T = uniform_int(it.T), seen = uniform_int(it.s.seen);
       if (T == 0) continue;
       const int qs = qc % C::QS;
@@ -782,7 +854,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     const uint32_t t_dq = tm + C::COL_DQ;
     int g = 0, qc = 0;
     bool ok = true;
-    for (XWalk<XA_BM, XA_BN, SCAN> it(p, qtiles, num_items); it.live && ok; it.next(p, num_items)) {
+    for (XWalk<XA_BM, XA_BN, SCAN> it(p, qtiles, num_items, order); it.live && ok; it.next(p, num_items)) {
       const int T = uniform_int(it.T), seen = uniform_int(it.s.seen);
       if (T == 0) continue;
       ok = qc == 0 || warp_bar_wait(dq_empty, (qc - 1) & 1, abort_flag, 128);
@@ -814,7 +886,7 @@ __global__ void __launch_bounds__(XA_THREADS, 2)
     const uint32_t t_s = tmem + lane_off + 32 * half, t_dq = tmem + lane_off + C::COL_DQ + half * (D / 2);
     const uint64_t scale2 = f2(p.scale_log2, p.scale_log2);
     int g = 0;
-    for (XWalk<XA_BM, XA_BN, SCAN> it(p, qtiles, num_items); it.live; it.next(p, num_items)) {
+    for (XWalk<XA_BM, XA_BN, SCAN> it(p, qtiles, num_items, order); it.live; it.next(p, num_items)) {
       const XSeq& s = it.s;
       if (it.tile * XA_BM >= s.lq) continue;
       const int h = it.h, T = it.T;
