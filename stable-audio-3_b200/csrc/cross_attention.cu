@@ -1061,6 +1061,23 @@ struct XDkv {
   static constexpr int COL_DV = 256, COL_DK = 256 + D;
 };
 
+// The n-th sequence of a packed batch of at most XA_SCAN by its queries, longest first: by one warp. CTAs start in that
+// order, so that the long walks do not come last (8 sequences of 50 .. 2000 queries and 30 .. 600 keys, 16 heads of 128
+// columns: 104 -> 98 us, 48 such: 666 -> 624, dQ included).
+__device__ __forceinline__ int nth_longest(const XParams& p, int n, int lane) {
+  int rows[2], rank[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 2; ++e) rows[e] = 32 * e + lane < p.batch ? make_seq(p, 32 * e + lane).lq : -1;
+  for (int b = 0; b < p.batch; ++b) {
+    const int x = __shfl_sync(0xffffffffu, b < 32 ? rows[0] : rows[1], b & 31);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) rank[e] += x > rows[e] || (x == rows[e] && b < 32 * e + lane);
+  }
+  const unsigned lo = __ballot_sync(0xffffffffu, lane < p.batch && rank[0] == n);
+  const unsigned hi = __ballot_sync(0xffffffffu, 32 + lane < p.batch && rank[1] == n);
+  return lo ? __ffs(lo) - 1 : 31 + __ffs(hi);
+}
+
 template <int D, bool F16>
 __global__ void __launch_bounds__(XB_THREADS, 1)
     cross_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
@@ -1084,6 +1101,7 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
   constexpr int NBARS = 14;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* seq_slot = reinterpret_cast<int*>(tmem_slot + 2);
 
   static_assert(2 * XB_SOFTMAX * XA_STAGE <= C::STAGES * 2 * C::T_BYTES, "room for the stores");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -1109,7 +1127,16 @@ __global__ void __launch_bounds__(XB_THREADS, 1)
   const int part = blockIdx.x % splits;
   const int kt = (blockIdx.x / splits) % ktiles;
   const int rest = blockIdx.x / splits / ktiles;
-  const int hk = rest % p.kv_heads, b = rest / p.kv_heads;
+  const int hk = rest % p.kv_heads;
+  int b = rest / p.kv_heads;
+  if (p.cu_q && p.batch <= XA_SCAN) {
+    if (warp == 0) {
+      const int x = nth_longest(p, b, lane);
+      if (lane == 0) *seq_slot = x;
+    }
+    __syncthreads();
+    b = *seq_slot;
+  }
   const XSeq s = make_seq(p, b);
   const int j0 = kt * XA_BM;
   const int qtiles = (s.lq + XA_BN - 1) / XA_BN;
@@ -1411,14 +1438,19 @@ static int dkv_splits(long long ctas, long long tiles, int sms) {
   }
   return (int)best;
 }
-// Packed batches: the lengths are on the device, the totals are not. The SMs share the work of all CTAs, and the end is
-// ragged by half of the longest one (4 sequences of 1255 .. 2500 queries and 528 .. 2111 keys: 158, 138, 150, 161 us
-// with 1, 2, 3, 4 parts, the joining included).
-static int dkv_splits_packed(long long ctas, long long tiles_mean, long long tiles_most, int sms) {
+// Packed batches: the lengths are on the device, the totals are not. The SMs share the work of all CTAs, which start with
+// the longest walk, and the end is ragged by a quarter of one; no walk can be shorter than the longest. The joining
+// launch takes some 4 us and its bytes at 3 TB/s, in tiles of 1.2 us (D = 128) or 0.8. Backward in all of 4 sequences of
+// 1255 .. 2500 queries and 528 .. 2111 keys, 16 heads of 128 columns: 329, 357, 365, 374 us with 1, 2, 3, 4 parts; 8 of
+// 50 .. 2000 and 30 .. 600: 132, 98, 107, 111; 2 such: 144, 94, 75, 65, and 52 with 8.
+static int dkv_splits_packed(long long ctas, long long tiles_mean, long long tiles_most, long long bytes, int head_dim,
+                             int sms) {
   long long best = 1;
   double cost = -1.;
+  const double join = bytes / 3e6 / (head_dim == 128 ? 1.2 : 0.8);
   for (long long n = 1; n <= 32 && n <= tiles_most; ++n) {
-    const double c = (double)ctas * (tiles_mean + 12. * n) / sms + tiles_most / (2. * n) + (n > 1 ? 6. + 2. * n : 0.);
+    const double all = (double)ctas * (tiles_mean + 12. * n) / sms + tiles_most / (4. * n), walk = tiles_most / (double)n + 12.;
+    const double c = (all > walk ? all : walk) + (n > 1 ? 4. + n * join : 0.);
     if (cost < 0. || c < cost) {
       cost = c;
       best = n;
@@ -1588,7 +1620,8 @@ static int fwd_parts(int batch, int max_q, int max_k, int heads, int kv_heads, i
   return best;
 }
 
-static int bwd_splits(int batch, int max_q, int max_k, int total_q, int total_k, int heads, int kv_heads, int sms) {
+static int bwd_splits(int batch, int max_q, int max_k, int total_q, int total_k, int heads, int kv_heads, int head_dim,
+                      int sms) {
   if (batch <= 0) return 1;
   const long long most = (long long)(heads / kv_heads) * ((max_q + XA_BN - 1) / XA_BN);
   const long long ctas = (long long)((max_k + XA_BM - 1) / XA_BM) * kv_heads * batch;
@@ -1596,7 +1629,8 @@ static int bwd_splits(int batch, int max_q, int max_k, int total_q, int total_k,
   if ((long long)batch * max_q == total_q && (long long)batch * max_k == total_k) return dkv_splits(ctas, most, sms);
   const long long some = (total_k / XA_BM + batch) * kv_heads;
   const long long mean = (long long)(heads / kv_heads) * (total_q / XA_BN / batch + 1);
-  return dkv_splits_packed(some < ctas ? some : ctas, mean < most ? mean : most, most, sms);
+  return dkv_splits_packed(some < ctas ? some : ctas, mean < most ? mean : most, most,
+                           16LL * total_k * kv_heads * head_dim, head_dim, sms);
 }
 
 }  // namespace sa3
@@ -1665,7 +1699,7 @@ extern "C" int sa3_cross_attention_bwd_workspace(int batch, int max_seqlen_q, in
   if (head_dim != 64 && head_dim != 128) return SA3_ERR_UNSUPPORTED;
   const int sms = sm_count();
   if (sms <= 0) return SA3_ERR_LAUNCH;
-  const int n = bwd_splits(batch, max_seqlen_q, max_seqlen_k, total_q, total_k, heads, kv_heads, sms);
+  const int n = bwd_splits(batch, max_seqlen_q, max_seqlen_k, total_q, total_k, heads, kv_heads, head_dim, sms);
   *bytes = stats_bytes(heads, total_q) + (n > 1 ? 8LL * n * total_k * kv_heads * head_dim : 0);
   return SA3_OK;
 }
@@ -1700,7 +1734,7 @@ extern "C" int sa3_cross_attention_bwd(const void* dout, const void* q, const vo
   }
   const int sms = sm_count();
   if (sms <= 0) return SA3_ERR_LAUNCH;
-  const int splits = bwd_splits(batch, max_seqlen_q, max_seqlen_k, total_q, total_k, heads, kv_heads, sms);
+  const int splits = bwd_splits(batch, max_seqlen_q, max_seqlen_k, total_q, total_k, heads, kv_heads, head_dim, sms);
   const long long at = stats_bytes(heads, total_q);
   const long long need = at + (splits > 1 ? 8LL * splits * total_k * kv_heads * head_dim : 0);
   if (workspace_bytes < need || (need > 0 && !workspace)) return SA3_ERR_ARG;
