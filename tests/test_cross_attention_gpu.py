@@ -267,3 +267,48 @@ def test_parts_of_the_keys(d, lq, lk, heads):
     # scores: fp32 sums of d products, each partial sum at most |q||k|
     off = (qd.abs() @ kd.abs().transpose(1, 2)).amax(-1) * d ** -0.5 * d * 2 ** -24 + 2 ** -18 * (1 + want_l.abs())
     assert bool(((lse.double() - want_l).abs() <= off).all())
+
+
+@pytest.mark.parametrize("d,heads,kv", [(64, 24, 24), (128, 16, 4)])
+def test_order_of_packed_sequences(d, heads, kv):
+    """Several rounds of items of unequal lengths: the same bits for a sequence wherever it stands in the batch, and
+    among more sequences than the walk orders; sampled rows against 64 bits."""
+    from sa3_b200 import ops
+
+    lens = [(1500, 600), (1, 900), (0, 40), (1201, 1), (640, 0), (1777, 130), (900, 777), (333, 64)]
+    g = torch.Generator(device="cuda").manual_seed(d)
+    data = [[torch.randn(n, w * d, device="cuda", generator=g).bfloat16() for n, w in ((lq, heads), (lk, kv), (lk, kv), (lq, heads))]
+            for lq, lk in lens]
+
+    def go(order):
+        q, k, v, do = (torch.cat([data[i][j] for i in order]) for j in range(4))
+        cu = [torch.tensor([0] + [lens[i][j] for i in order]).cumsum(0).int().cuda() for j in range(2)]
+        how = dict(heads=heads, kv_heads=kv, head_dim=d, cu_seqlens_q=cu[0], cu_seqlens_k=cu[1], max_seqlen_q=1777,
+                   max_seqlen_k=900)
+        o, lse = ops.cross_attention(q, k, v, return_lse=True, **how)
+        dq, dk, dv = ops.cross_attention_backward(do, q, k, v, o, lse, **how)
+        at, ak = cu[0].tolist(), cu[1].tolist()
+        return {i: (o[at[n]:at[n + 1]], lse[:, at[n]:at[n + 1]], dq[at[n]:at[n + 1]], dk[ak[n]:ak[n + 1]], dv[ak[n]:ak[n + 1]])
+                for n, i in enumerate(order)}
+
+    want = go(list(range(8)))
+    for order in ([7, 2, 5, 0, 6, 4, 1, 3], [3, 1, 4, 6, 0, 5, 2, 7]):
+        got = go(order)
+        for i in range(8):
+            assert all(torch.equal(a, b) for a, b in zip(got[i], want[i])), (order, i)
+    many = go([0, 1] + [2] * 60 + [3, 4, 5, 6, 7])
+    for i in range(8):
+        assert all(torch.equal(a, b) for a, b in zip(many[i][:3], want[i][:3])), i
+    for i, (lq, lk) in enumerate(lens):
+        if lq and lk:
+            r = torch.arange(0, lq, max(1, lq // 37), device="cuda")
+            q, k, v = (data[i][j].double() for j in range(3))
+            q = q[r].view(-1, kv, heads // kv, d)
+            k, v = k.view(lk, kv, d), v.view(lk, kv, d)
+            p = torch.einsum("rhgd,khd->rhgk", q, k).mul(d ** -0.5).softmax(-1)
+            o = torch.einsum("rhgk,khd->rhgd", p, v).flatten(1)
+            room = torch.einsum("rhgk,khd->rhgd", p, v.abs()).flatten(1)
+            # P and O each rounded once to bf16; 2^-16 for the fp32 work
+            assert bool(((want[i][0][r].double() - o).abs() <= room * (2 ** -8 + 2 ** -16) + o.abs() * 2 ** -8 * 1.01).all())
+        elif lq:
+            assert not want[i][0].any() and bool((want[i][1] == -math.inf).all()) and not want[i][2].any()
