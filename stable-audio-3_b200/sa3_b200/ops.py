@@ -409,7 +409,7 @@ def rotary(q: torch.Tensor, inv_freq: torch.Tensor, *, heads: int, head_dim: int
     ldq = _rows_view(q, rows, wq, "q", dtype)
     ldqo, ldk, ldko = wq, 0, 0
     if out is None:
-        out = q.new_empty(rows, wq)
+        out = torch.empty_like(q)
     else:
         ldqo = _rows_view(out, rows, wq, "out", dtype)
     if k is not None:
@@ -417,7 +417,7 @@ def rotary(q: torch.Tensor, inv_freq: torch.Tensor, *, heads: int, head_dim: int
             raise RuntimeError("k needs kv_heads")
         ldk, ldko = _rows_view(k, rows, wk, "k", dtype), wk
         if k_out is None:
-            k_out = k.new_empty(rows, wk)
+            k_out = torch.empty_like(k)
         else:
             ldko = _rows_view(k_out, rows, wk, "k_out", dtype)
     elif k_out is not None or kv_heads:
@@ -503,7 +503,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, heads:
                                                   cu_seqlens_q, cu_seqlens_k, k_lens, key_mask, softmax_scale)
     rows, width = q.shape[0], heads * head_dim
     if out is None:
-        out, ldo = q.new_empty(rows, width), width
+        out, ldo = torch.empty_like(q), width
     else:
         ldo = _rows_view(out, rows, width, "out", q.dtype)
     if lse is not None:
@@ -539,15 +539,15 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     _check_lse(lse, heads, rows)
     lddq, lddk, lddv = wq, wk, wk
     if dq is None:
-        dq = q.new_empty(rows, wq)
+        dq = torch.empty_like(q)
     else:
         lddq = _rows_view(dq, rows, wq, "dq", dtype)
     if dk is None:
-        dk = k.new_empty(krows, wk)
+        dk = torch.empty_like(k)
     else:
         lddk = _rows_view(dk, krows, wk, "dk", dtype)
     if dv is None:
-        dv = v.new_empty(krows, wk)
+        dv = torch.empty_like(v)
     else:
         lddv = _rows_view(dv, krows, wk, "dv", dtype)
     n = _scratch_bytes("sa3_cross_attention_bwd_workspace", dev, batch, max_seqlen_q, max_seqlen_k, rows, krows, heads,
