@@ -1423,15 +1423,21 @@ __global__ void __launch_bounds__(256) cross_merge_kernel(const XParams p) {
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// Parts of the dK / dV walk: the number that ends soonest. A part's set-up and epilogue cost about 12 tiles, the
-// joining launch 6 and 2 a part.
-// Uniform batches: every wave of CTAs costs its longest walk. One part writes its result at once.
-static int dkv_splits(long long ctas, long long tiles, int sms) {
-  long long best = 1, cost = -1;
+// Parts of the dK / dV walk: the number that ends soonest, in tiles of 1.2 us (D = 128) or 0.8. A part's set-up and
+// epilogue cost about 12 tiles, the joining launch 4 and its bytes (`bytes` a part, written and read) at 3 TB/s. One part
+// writes its result at once.
+static double join_tiles(long long bytes, int head_dim) { return bytes / 3e6 / (head_dim == 128 ? 1.2 : 0.8); }
+// Uniform batches: every wave of CTAs costs its longest walk. Backward in all with 1, 2, 4, 8 parts: 24 heads of 64, 2 x
+// 8247 queries x 128 keys 167, 129, 139, 141 us and 115 with 3; x 257 keys 206, 225, 242, 269; 8 heads on one of 128, 700
+// queries x 64 keys 94, 57, 37, 27 and 23 with 32.
+static int dkv_splits(long long ctas, long long tiles, long long bytes, int head_dim, int sms) {
+  const double join = join_tiles(bytes, head_dim);
+  long long best = 1;
+  double cost = -1.;
   for (long long n = 1; n <= 32 && n <= tiles; ++n) {
     const long long waves = (ctas * n + sms - 1) / sms;
-    const long long c = waves * ((tiles + n - 1) / n + 12) + (n > 1 ? 6 + 2 * n : 0);
-    if (cost < 0 || c < cost) {
+    const double c = (double)waves * ((tiles + n - 1) / n + 12) + (n > 1 ? 4. + n * join : 0.);
+    if (cost < 0. || c < cost) {
       cost = c;
       best = n;
     }
@@ -1439,15 +1445,14 @@ static int dkv_splits(long long ctas, long long tiles, int sms) {
   return (int)best;
 }
 // Packed batches: the lengths are on the device, the totals are not. The SMs share the work of all CTAs, which start with
-// the longest walk, and the end is ragged by a quarter of one; no walk can be shorter than the longest. The joining
-// launch takes some 4 us and its bytes at 3 TB/s, in tiles of 1.2 us (D = 128) or 0.8. Backward in all of 4 sequences of
-// 1255 .. 2500 queries and 528 .. 2111 keys, 16 heads of 128 columns: 329, 357, 365, 374 us with 1, 2, 3, 4 parts; 8 of
-// 50 .. 2000 and 30 .. 600: 132, 98, 107, 111; 2 such: 144, 94, 75, 65, and 52 with 8.
+// the longest walk, and the end is ragged by a quarter of one; no walk can be shorter than the longest. Backward in all of
+// 4 sequences of 1255 .. 2500 queries and 528 .. 2111 keys, 16 heads of 128 columns, with 1, 2, 3, 4 parts: 329, 357, 365,
+// 374 us; 8 of 50 .. 2000 and 30 .. 600: 132, 98, 107, 111; 2 such: 144, 94, 75, 65, and 52 with 8.
 static int dkv_splits_packed(long long ctas, long long tiles_mean, long long tiles_most, long long bytes, int head_dim,
                              int sms) {
   long long best = 1;
   double cost = -1.;
-  const double join = bytes / 3e6 / (head_dim == 128 ? 1.2 : 0.8);
+  const double join = join_tiles(bytes, head_dim);
   for (long long n = 1; n <= 32 && n <= tiles_most; ++n) {
     const double all = (double)ctas * (tiles_mean + 12. * n) / sms + tiles_most / (4. * n), walk = tiles_most / (double)n + 12.;
     const double c = (all > walk ? all : walk) + (n > 1 ? 4. + n * join : 0.);
@@ -1626,11 +1631,12 @@ static int bwd_splits(int batch, int max_q, int max_k, int total_q, int total_k,
   const long long most = (long long)(heads / kv_heads) * ((max_q + XA_BN - 1) / XA_BN);
   const long long ctas = (long long)((max_k + XA_BM - 1) / XA_BM) * kv_heads * batch;
   if (ctas <= 0 || most <= 0) return 1;
-  if ((long long)batch * max_q == total_q && (long long)batch * max_k == total_k) return dkv_splits(ctas, most, sms);
+  const long long bytes = 16LL * total_k * kv_heads * head_dim;
+  if ((long long)batch * max_q == total_q && (long long)batch * max_k == total_k)
+    return dkv_splits(ctas, most, bytes, head_dim, sms);
   const long long some = (total_k / XA_BM + batch) * kv_heads;
   const long long mean = (long long)(heads / kv_heads) * (total_q / XA_BN / batch + 1);
-  return dkv_splits_packed(some < ctas ? some : ctas, mean < most ? mean : most, most,
-                           16LL * total_k * kv_heads * head_dim, head_dim, sms);
+  return dkv_splits_packed(some < ctas ? some : ctas, mean < most ? mean : most, most, bytes, head_dim, sms);
 }
 
 }  // namespace sa3
