@@ -8,7 +8,8 @@
 //   O^T (16 columns x rows) += V^T P^T    A = V^T by ldmatrix.trans, B = P^T: the S^T fragment, transposed by movmatrix
 // The keys are split over the warps of a cluster of CTAs, 16 keys a step. Each warp copies its steps asynchronously
 // into a ring of its own in shared memory (16-byte chunk c of key j at chunk c ^ (j & 7): no bank conflicts on either
-// side), several steps ahead, so the bytes in flight take no registers and no warp waits for another. Hidden keys are
+// side), several steps ahead, so the bytes in flight take no registers and no warp waits for another: 5.6 TB/s for 64
+// sequences of 375 .. 1500 keys, 8 key heads of 128 columns (45 us). Hidden keys are
 // not read: their rows are filled with zeros and their scores are -inf.
 // The reference maximum of a row moves only when a score exceeds it by more than 2^8; one vote a step finds out, and
 // the usual step has no reduction over lanes. The warps of a CTA join through shared memory and the CTAs of the
@@ -29,6 +30,8 @@ constexpr int XT_KEYS = 16;          // keys of a step of a warp
 constexpr int XT_MAX_CLUSTER = 8;
 constexpr int XT_PART_KEYS = 256;    // least keys of a part of the split without clusters: 4 steps of a warp
 constexpr int XT_MAX_PARTS = 128;
+constexpr int XT_MAX_ORDER = 64;     // sequences that are ordered: two a lane
+constexpr int XT_ORDER_KEYS = 1280;  // longest keys from which that is worth it
 constexpr int XT_SPLIT_KEYS = 8192;  // keys from which that split is worth its second launch
 constexpr float XT_RESCALE_LOG2 = 8.f;
 // Steps in flight: 96 KB a CTA at either width, two CTAs an SM.
@@ -76,9 +79,27 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
 
+// The n-th of at most XT_MAX_ORDER sequences by its visible keys, most first; every warp finds it by itself.
+__device__ __forceinline__ int nth_most_keys(const XParams& p, int n, int lane) {
+  int keys[2], rank[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 2; ++e) keys[e] = make_seq(p, min(32 * e + lane, p.batch - 1)).seen;
+  if (__reduce_max_sync(0xffffffffu, max(keys[0], keys[1])) == __reduce_min_sync(0xffffffffu, min(keys[0], keys[1])))
+    return n;
+#pragma unroll 8
+  for (int b = 0; b < p.batch; ++b) {
+    const int x = __shfl_sync(0xffffffffu, b < 32 ? keys[0] : keys[1], b & 31);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) rank[e] += x > keys[e] || (x == keys[e] && b < 32 * e + lane);
+  }
+  const unsigned lo = __ballot_sync(0xffffffffu, lane < p.batch && rank[0] == n);
+  const unsigned hi = __ballot_sync(0xffffffffu, 32 + lane < p.batch && rank[1] == n);
+  return lo ? __ffs(lo) - 1 : 31 + __ffs(hi);
+}
+
 // NT: tiles of 8 query rows (1 or 2).
 template <int D, bool F16, int NT>
-__global__ void __launch_bounds__(XT_THREADS, 2) cross_token_kernel(const XTokenParams a, int csize) {
+__global__ void __launch_bounds__(XT_THREADS, 2) cross_token_kernel(const XTokenParams a, int csize, bool ordered) {
   constexpr int ROWS = 8 * NT;
   constexpr int CH = D / 8;                 // 16-byte chunks of a key
   constexpr int KPI = 32 / CH;              // keys that one copy instruction of a warp covers
@@ -90,8 +111,10 @@ __global__ void __launch_bounds__(XT_THREADS, 2) cross_token_kernel(const XToken
   const XParams& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x % csize, part = blockIdx.x / csize % p.parts, unit = blockIdx.x / csize / p.parts;
-  const int hk = unit % p.kv_heads, b = unit / p.kv_heads;
+  const int hk = unit % p.kv_heads;
+  int b = unit / p.kv_heads;
   grid_dep_wait();
+  if (ordered) b = nth_most_keys(p, b, lane);
   const XSeq sq = make_seq(p, b);
   const int qs = sq.qs, lq = sq.lq, ks = sq.ks, seen = sq.seen;
   const int rows = lq * p.group;  // row m: token m / group, head hk * group + m % group
@@ -341,6 +364,12 @@ static int launch_token(const XTokenParams& a, int csize, int sms, cudaStream_t 
   // The CTAs of a cluster are packed two to an SM where two fit, even when SMs are left empty. A launch that has an
   // SM for every CTA asks for so much shared memory that they spread.
   const int SMEM = ctas <= sms ? ALONE : NEED;
+  // Between one and two waves of CTAs with lengths of their own the long ones start first: 64 sequences of 187 .. 1500
+  // keys, 8 key heads: 25.2 -> 23.9 us (64 columns), 39.9 -> 36.8 (128), 40 of 500 .. 4000: 45.9 -> 37.7, 72.3 -> 65.9.
+  // With shorter keys finding the place costs more (75 .. 600: 15.4 -> 17.5, 21.5 -> 23.6), with more waves the last ones
+  // are of short sequences alone (16 key heads, 128 .. 1024 keys: 33.4 -> 42.8).
+  const bool ordered = (a.p.k_lens || a.p.cu_k) && a.p.batch <= XT_MAX_ORDER && a.p.Lk >= XT_ORDER_KEYS &&
+                       ctas > 2LL * sms && ctas <= 4LL * sms;
   auto kern = cross_token_kernel<D, F16, NT>;
   int rc;
   if ((rc = ensure_smem(kern, ALONE))) return rc;
@@ -362,7 +391,7 @@ static int launch_token(const XTokenParams& a, int csize, int sms, cudaStream_t 
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  if (cudaLaunchKernelEx(&cfg, kern, a, csize) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kern, a, csize, ordered) != cudaSuccess) {
     cudaGetLastError();
     return SA3_ERR_LAUNCH;
   }

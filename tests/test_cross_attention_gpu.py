@@ -312,3 +312,49 @@ def test_order_of_packed_sequences(d, heads, kv):
             assert bool(((want[i][0][r].double() - o).abs() <= room * (2 ** -8 + 2 ** -16) + o.abs() * 2 ** -8 * 1.01).all())
         elif lq:
             assert not want[i][0].any() and bool((want[i][1] == -math.inf).all()) and not want[i][2].any()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("batch", [38, 64])
+def test_order_of_single_tokens(d, packed, batch):
+    """One token of every sequence against long keys of unequal lengths, some of zero: the same bits wherever a sequence
+    stands, and 64-bit values."""
+    from sa3_b200 import ops
+
+    kv, heads, longest = 8, 16, 1300
+    g = torch.Generator(device="cuda").manual_seed(batch)
+    lens = [longest, 0, 1] + [(37 * i * i + 11) % longest for i in range(batch - 3)]
+    q = torch.randn(batch, heads * d, device="cuda", generator=g).bfloat16()
+    k, v = (torch.randn(batch, longest, kv * d, device="cuda", generator=g).bfloat16() for _ in range(2))
+
+    def go(order):
+        how = dict(heads=heads, kv_heads=kv, head_dim=d, batch=batch, max_seqlen_q=1, max_seqlen_k=longest, return_lse=True)
+        n = torch.tensor([lens[i] for i in order], dtype=torch.int32, device="cuda")
+        if packed:
+            cu = torch.cat([n.new_zeros(1), n.cumsum(0).int()])
+            o, lse = ops.cross_attention(q[order], torch.cat([k[i, :lens[i]] for i in order]),
+                                         torch.cat([v[i, :lens[i]] for i in order]), cu_seqlens_k=cu, **how)
+        else:
+            o, lse = ops.cross_attention(q[order], k[order].flatten(0, 1), v[order].flatten(0, 1), k_lens=n, **how)
+        back = torch.empty(batch, dtype=torch.long)
+        back[torch.tensor(order)] = torch.arange(batch)
+        return o[back.cuda()], lse[:, back.cuda()]
+
+    o, lse = go(list(range(batch)))
+    for order in (list(range(batch))[::-1], [(7 * i + 3) % batch for i in range(batch)] if batch % 7 else [(5 * i + 3) % batch for i in range(batch)]):
+        a, b = go(order)
+        assert torch.equal(a, o) and torch.equal(b, lse)
+    for i in range(batch):
+        n = lens[i]
+        if n == 0:
+            assert not o[i].any() and bool((lse[:, i] == -math.inf).all())
+            continue
+        kk, vv = (t[i, :n].double().view(n, kv, d) for t in (k, v))
+        s = torch.einsum("hgd,khd->hgk", q[i].double().view(kv, heads // kv, d), kk) * d ** -0.5
+        p = s.softmax(-1)
+        want = torch.einsum("hgk,khd->hgd", p, vv).flatten()
+        # P and O rounded once each to bf16; 2^-16 for the fp32 work
+        room = torch.einsum("hgk,khd->hgd", p, vv.abs()).flatten() * (2 ** -8 + 2 ** -16) + want.abs() * 2 ** -8 * 1.01
+        assert bool(((o[i].double() - want).abs() <= room).all())
+        assert bool(((lse[:, i].double() - s.logsumexp(-1).flatten()).abs() <= 2 ** -18 * (1 + s.abs().amax())).all())
