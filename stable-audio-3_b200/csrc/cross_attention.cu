@@ -1424,8 +1424,9 @@ __global__ void __launch_bounds__(256) cross_merge_kernel(const XParams p) {
 
 // ------------------------------------------------------------------------------------------------ host
 // Parts of the dK / dV walk: the number that ends soonest, in tiles of 1.2 us (D = 128) or 0.8. A part's set-up and
-// epilogue cost about 12 tiles, the joining launch 4 and its bytes (`bytes` a part, written and read) at 3 TB/s. One part
-// writes its result at once.
+// epilogue cost about 12 tiles, the joining launch 8 and its bytes (`bytes` a part, written and read) at 3 TB/s. One part
+// writes its result at once. (The device alone would have it at 4 tiles: 3 x 77 queries x 33 keys, 8 heads on 2, take 18.1
+// us with one part and 14.7 with four; but such calls wait for the host, for which the launch is 1.3 us more.)
 static double join_tiles(long long bytes, int head_dim) { return bytes / 3e6 / (head_dim == 128 ? 1.2 : 0.8); }
 // Uniform batches: every wave of CTAs costs its longest walk. Backward in all with 1, 2, 4, 8 parts: 24 heads of 64, 2 x
 // 8247 queries x 128 keys 167, 129, 139, 141 us and 115 with 3; x 257 keys 206, 225, 242, 269; 8 heads on one of 128, 700
@@ -1436,7 +1437,7 @@ static int dkv_splits(long long ctas, long long tiles, long long bytes, int head
   double cost = -1.;
   for (long long n = 1; n <= 32 && n <= tiles; ++n) {
     const long long waves = (ctas * n + sms - 1) / sms;
-    const double c = (double)waves * ((tiles + n - 1) / n + 12) + (n > 1 ? 4. + n * join : 0.);
+    const double c = (double)waves * ((tiles + n - 1) / n + 12) + (n > 1 ? 8. + n * join : 0.);
     if (cost < 0. || c < cost) {
       cost = c;
       best = n;
@@ -1455,7 +1456,7 @@ static int dkv_splits_packed(long long ctas, long long tiles_mean, long long til
   const double join = join_tiles(bytes, head_dim);
   for (long long n = 1; n <= 32 && n <= tiles_most; ++n) {
     const double all = (double)ctas * (tiles_mean + 12. * n) / sms + tiles_most / (4. * n), walk = tiles_most / (double)n + 12.;
-    const double c = (all > walk ? all : walk) + (n > 1 ? 4. + n * join : 0.);
+    const double c = (all > walk ? all : walk) + (n > 1 ? 8. + n * join : 0.);
     if (cost < 0. || c < cost) {
       cost = c;
       best = n;
